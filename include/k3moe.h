@@ -308,6 +308,71 @@ int k3moe_import_mxfp4(const uint8_t* packed_rows, const uint8_t* scale_rows, in
 int k3moe_synth_mxfp4(uint64_t seed, long long row0, long long rows, int K, float sd, uint8_t* packed, uint8_t* sf,
                       k3moe_stream_t stream);
 
+/* ---------------------------------------------------------------- the router's training side
+ * The load-balance loss over the top-k's picks, with its counts.  With s = sigmoid(S), p_te = s_te / (sum_e s_te +
+ * 1e-20) and the counted rows of sequence b (seq[b] <= t < seq[b + 1], mask[t] != 0), n_b of them:
+ *   counts[b, e] = picks of expert e, prob[b, e] = sum_t p_te, rows[b] = n_b,
+ *   loss = alpha / B' * sum_b sum_e (E counts / (K n_b)) (prob / n_b), B' = sequences with n_b > 0 (0 if none).
+ * S f32 [T, lds]; idx int32 [T, K], ids outside [0, E) not counted; seq int32 [B + 1], non-decreasing offsets in
+ * [0, T] (rows before the first and from the last on are not counted), or null with B = 1: all T rows are one
+ * sequence; mask uint8 [T] or null.  S is not read in rows that are not counted.  counts int32 [B, E], prob f32
+ * [B, E], rows int32 [B], loss f32 [1].  E <= 1024, K <= 16.  Fixed summation order: equal inputs give equal bytes.
+ * scratch: k3moe_balance_scratch_bytes(T, E, B) bytes, 16-byte aligned, one per call in flight (0: bad sizes).
+ * No counterpart in the reference, which serves only. */
+size_t k3moe_balance_scratch_bytes(int T, int E, int B);
+int k3moe_balance_loss(const float* S, int lds, const int32_t* idx, int T, int E, int K, const int32_t* seq, int B,
+                       const uint8_t* mask, float alpha, void* scratch, int32_t* counts, float* prob, int32_t* rows,
+                       float* loss, k3moe_stream_t stream);
+
+/* The gradient of the router logits, every row of dS [T, ldd] (dtype K3MOE_F32 or K3MOE_BF16) written: the sum of
+ * - the balance term, where counts and rows (k3moe_balance_loss's, held constant) are given:
+ *     f_be = alpha dloss E counts / (B' K n_b^2);  (f_be - sum_j f_bj p_tj) s_te (1 - s_te) / (sum_e s_te + 1e-20)
+ *   in the rows that k3moe_balance_loss counts (same seq, B, mask, alpha, K); dloss f32 [1] on the device (null: 1);
+ * - the weight term, where dwts f32 [T, K] (dloss/dw of k3moe_route_topk's weights) and rs bf16 [1] are given:
+ *     den = sum_k s_k + 1e-20;  rs / den (dwts_k - sum_j dwts_j s_j / den) s_k (1 - s_k) at expert idx[t, k],
+ *   in every row (the mask and the sequences concern the balance term only); picks outside [0, E) are left out of
+ *   the sums, an expert named twice gets both parts.
+ * At least one term is given (else K3MOE_EINVAL).  The selection bias has no gradient; rs is a constant. */
+enum { K3MOE_BF16 = 0, K3MOE_F32 = 1 };
+int k3moe_route_backward(const float* S, int lds, const int32_t* idx, int T, int E, int K, const int32_t* seq, int B,
+                         const uint8_t* mask, float alpha, const int32_t* counts, const int32_t* rows,
+                         const float* dloss, const float* dwts, const void* rs_bf16, void* dS, int ldd, int dtype,
+                         k3moe_stream_t stream);
+
+/* ---------------------------------------------------------------- products in 8-bit integers (W8A8)
+ * Rows to int8 with one scale each (a token's, or a weight channel's): amax = max |x|, scale = amax / 127,
+ * q = round-half-even(127 x / amax) of the exact quotient, so q is in [-127, 127].  A zero row: scale 0, q 0.  A row
+ * holding an infinity or a NaN: scale NaN, q 0 (its products are NaN).  x [rows, ldx] of dtype K3MOE_BF16 or
+ * K3MOE_F32; q [rows, ldq], 16-byte aligned, ldq a multiple of 16 (bytes past cols are left as they were).
+ * cols >= 1. */
+int k3moe_quant_int8(const void* x, int dtype, long long ldx, long long rows, int cols, int8_t* q, long long ldq,
+                     float* scale, k3moe_stream_t stream);
+/* The same of act(gate) * up (f32, K3MOE_ACT_SWIGLU or K3MOE_ACT_SITU): gu bf16 [rows, ldg] holds a row's I gate and
+ * then its I up values.  With cta_limit and meta (k3moe_route_tables, tile 128; at most max_ctas tiles) only the
+ * tables' real rows are read and written; with both null, all. */
+int k3moe_act_quant_int8(const void* gu_bf16, long long ldg, long long rows, int I, int activation,
+                         const int32_t* cta_limit, const int32_t* meta, int max_ctas, int8_t* q, long long ldq,
+                         float* scale, k3moe_stream_t stream);
+/* k3moe_quant_int8 of bf16 row r written to every permuted row it is routed to: exp2perm[r*K + k] >= 0 and, with a
+ * shared expert, meta[2] + r; q_perm [cap_rows, ldq], scale_perm f32 [cap_rows].  Rows past cap_rows are skipped. */
+int k3moe_quant_int8_permute(const void* x_bf16, long long ldx, int R, int cols, int K, const int32_t* exp2perm,
+                             const int32_t* meta, int8_t* q_perm, long long ldq, float* scale_perm, int cap_rows,
+                             k3moe_stream_t stream);
+/* out[t, n] = sx[t] * sw[n] * sum_c q[t, c] w[n, c]: int8 x int8 on the tensor cores, the int32 sum exact, then two f32
+ * products and (dtype K3MOE_BF16) one rounding.  q [T, ldq], w [N, ldw], both 16-byte aligned with leading dimensions
+ * a multiple of 16; out [T, ldo].  C (the reduction length) in [1, 131071]: -128 * -128 * C stays inside int32.
+ * err: the device error words (a bounded wait that ran out), or null. */
+int k3moe_gemm_int8(const int8_t* q, long long ldq, const float* sx, const int8_t* w, long long ldw, const float* sw,
+                    int T, int N, int C, void* out, long long ldo, int dtype, uint32_t* err, k3moe_stream_t stream);
+/* The same for routed rows: permuted row r of a tile of expert e (cta_batch, cta_limit, meta of k3moe_route_tables,
+ * tile 128) times w[e * N + n], w [n_experts * N, ldw], sw [n_experts * N].  q_perm [cap_rows, ldq] with
+ * cap_rows >= 128 max_ctas; out [cap_rows, ldo]: padding rows are left as they were.  A tile whose expert or limit is
+ * out of range is recorded in err and skipped. */
+int k3moe_grouped_gemm_int8(const int8_t* q_perm, long long ldq, const float* sx_perm, const int8_t* w, long long ldw,
+                            const float* sw, const int32_t* cta_batch, const int32_t* cta_limit, const int32_t* meta,
+                            int N, int C, int n_experts, int cap_rows, int max_ctas, void* out, long long ldo,
+                            int dtype, uint32_t* err, k3moe_stream_t stream);
+
 /* ---------------------------------------------------------------- the layer
  * One routed-MoE layer on the experts this GPU holds: top-k -> tables ->
  * MXFP8 permute -> FC1 -> FC2 -> combine (+ the shared expert, stored as

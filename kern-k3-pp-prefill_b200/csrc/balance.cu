@@ -1,0 +1,394 @@
+// The router's training side: the load-balance loss with its per-sequence expert counts, and the gradient of the
+// router logits (from the loss and from the combine weights of the top-k).
+//
+// With s = sigmoid(S) (the top-k's scores), z_t = sum_e s_te + 1e-20 and p_te = s_te / z_t, over the counted rows
+// of sequence b (inside [seq[b], seq[b+1]) and not masked out): n_b rows, c_be picks of expert e, P_be = sum p_te,
+//   loss = alpha / B' * sum_b sum_e (E c_be / (K n_b)) (P_be / n_b),    B' = sequences with a counted row.
+// The counts are constants of the gradient, so with f_be = alpha dloss E c_be / (B' K n_b^2)
+//   dS_te += (f_be - sum_j f_bj p_tj) s_te (1 - s_te) / z_t,
+// and from the weights w_k = rs s_k / den, den = sum_k s_k + 1e-20, of a row's picks
+//   dS_{t, idx_k} += rs / den (g_k - sum_j g_j s_j / den) s_k (1 - s_k),    g = dloss/dw.
+// No counterpart in the reference: it serves only.
+//
+// Both passes read S once.  Sums run in f32 in a fixed order (no floating-point atomics), so equal inputs give equal
+// bytes.  exp(-|S|) is __expf: its error grows with |S|, to 1.5e-6 at |S| = 10, where the score itself is below 5e-5
+// or its slope is.
+#pragma once
+#include "common.cuh"
+
+namespace k3 {
+
+namespace bal {
+constexpr int WARPS = 8;
+constexpr int THREADS = 32 * WARPS;
+constexpr float TINY = 1e-20f;  // the top-k's guard of its own sum
+constexpr int COLS = 32;        // experts a block of the second pass
+}  // namespace bal
+
+struct RouterRows {
+  const float* S;          // [T, lds]
+  long long lds;
+  const int* idx;          // [T, K]
+  const int* seq;          // [B + 1] or null: one sequence of all T rows
+  const uint8_t* mask;     // [T] or null
+  int T, E, K, B;
+  int vec;                 // S rows may be read 16 bytes at a time
+};
+
+// the sequence holding row r: the last b with seq[b] <= r (the caller has checked seq[0] <= r)
+__device__ __forceinline__ int seq_of(const int* __restrict__ seq, int B, int r) {
+  int lo = 0, hi = B - 1;
+  while (lo < hi) {
+    const int m = (lo + hi + 1) >> 1;
+    if (seq[m] <= r) lo = m;
+    else hi = m - 1;
+  }
+  return lo;
+}
+
+// A lane's experts: 4 consecutive ones in each group of 128, (j * 32 + lane) * 4 + i.  Past E: -inf (score 0).
+template <int NV>
+__device__ __forceinline__ void load_row(const float* __restrict__ row, int E, int vec, int lane, float (&v)[4 * NV]) {
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (j * 32 + lane) * 4;
+    if (vec && c + 4 <= E) {
+      const float4 q = *reinterpret_cast<const float4*>(row + c);
+      v[4 * j] = q.x;
+      v[4 * j + 1] = q.y;
+      v[4 * j + 2] = q.z;
+      v[4 * j + 3] = q.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * j + i] = c + i < E ? row[c + i] : -INFINITY;
+    }
+  }
+}
+
+// t = exp(-|x|), r = 1 / (1 + t): sigmoid(x) is r or t r, and its slope t r^2 at either sign, without cancellation
+__device__ __forceinline__ float sigmoid_of(float x, float& t, float& r) {
+  t = __expf(-fabsf(x));
+  r = __fdividef(1.0f, 1.0f + t);
+  return x >= 0.f ? r : t * r;  // a NaN x: t is NaN
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+// ---------------------------------------------------------------- forward
+// First pass: a block takes `chunk` consecutive rows, a warp every eighth of them, each lane summing its experts' p
+// in registers.  At the end of a sequence, or of the block's rows, the eight warps' sums are added and stored as one
+// partial row.  Block i and sequence b meet in slot i + b: along the rows either i or b goes up, so no two pairs
+// share a slot and nothing needs zeroing.
+struct BalanceScratch {
+  float* prob;   // [slots, E]
+  int* count;    // [slots, E]
+  int* rows;     // [slots]
+  float* term;   // [B, ceil(E / 32)]
+  u32* done;
+};
+
+template <int NV>
+__global__ void __launch_bounds__(bal::THREADS) balance_rows_kernel(RouterRows in, BalanceScratch w, int chunk) {
+  using namespace bal;
+  __shared__ float s_acc[WARPS][128 * NV];
+  __shared__ int s_hist[128 * NV];
+  __shared__ int s_rows[WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r0 = blockIdx.x * chunk, r1 = min(in.T, r0 + chunk);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *w.done = 0u;
+  int r = r0, last = r1;
+  if (in.seq) {
+    r = max(r0, in.seq[0]);
+    last = min(r1, in.seq[in.B]);
+  }
+  while (r < last) {
+    int b = 0, end = last;
+    if (in.seq) {
+      b = seq_of(in.seq, in.B, r);
+      end = min(last, in.seq[b + 1]);
+      if (end <= r) break;  // offsets that go down: nothing more is counted
+    }
+    for (int e = threadIdx.x; e < in.E; e += THREADS) s_hist[e] = 0;
+    __syncthreads();
+    float acc[4 * NV];
+#pragma unroll
+    for (int i = 0; i < 4 * NV; ++i) acc[i] = 0.f;
+    int n = 0;
+    for (int t = r + warp; t < end; t += WARPS) {
+      if (in.mask && in.mask[t] == 0) continue;
+      ++n;
+      float v[4 * NV];
+      load_row<NV>(in.S + t * in.lds, in.E, in.vec, lane, v);
+      if (lane < in.K) {
+        const int e = in.idx[(long long)t * in.K + lane];
+        if (e >= 0 && e < in.E) atomicAdd(&s_hist[e], 1);
+      }
+      float z = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4 * NV; ++i) {
+        float u, q;
+        v[i] = sigmoid_of(v[i], u, q);
+        z += v[i];
+      }
+      const float inv = __frcp_rn(warp_sum(z) + TINY);
+#pragma unroll
+      for (int i = 0; i < 4 * NV; ++i) acc[i] += v[i] * inv;
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      *reinterpret_cast<float4*>(&s_acc[warp][(j * 32 + lane) * 4]) =
+          make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+    if (lane == 0) s_rows[warp] = n;
+    __syncthreads();
+    const long long slot = (long long)blockIdx.x + b;
+    for (int e = threadIdx.x; e < in.E; e += THREADS) {
+      float p = 0.f;
+#pragma unroll
+      for (int k = 0; k < WARPS; ++k) p += s_acc[k][e];
+      w.prob[slot * in.E + e] = p;
+      w.count[slot * in.E + e] = s_hist[e];
+    }
+    if (threadIdx.x == 0) {
+      int total = 0;
+      for (int k = 0; k < WARPS; ++k) total += s_rows[k];
+      w.rows[slot] = total;
+    }
+    __syncthreads();
+    r = end;
+  }
+}
+
+// Second pass: a block adds up 32 experts of one sequence over the first pass's blocks that met it (8 warps side by
+// side, joined in order), and the last block of all adds up the loss.
+__global__ void __launch_bounds__(bal::THREADS)
+    balance_join_kernel(RouterRows in, BalanceScratch w, int chunk, float alpha, int* __restrict__ counts,
+                        float* __restrict__ prob, int* __restrict__ rows, float* __restrict__ loss) {
+  using namespace bal;
+  __shared__ float s_p[WARPS][COLS];
+  __shared__ int s_c[WARPS][COLS], s_n[WARPS];
+  __shared__ int s_last;
+  const int groups = (in.E + COLS - 1) / COLS;
+  const int b = blockIdx.x / groups, g = blockIdx.x % groups;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int e = g * COLS + lane;
+  int s0 = 0, s1 = in.T;
+  if (in.seq) {
+    const int lo = max(in.seq[0], 0), hi = min(in.seq[in.B], in.T);
+    s0 = max(lo, in.seq[b]);
+    s1 = min(hi, in.seq[b + 1]);
+  }
+  float p = 0.f;
+  int c = 0, n = 0;
+  if (s0 < s1) {
+    const int i1 = (s1 - 1) / chunk;
+#pragma unroll 4
+    for (int i = s0 / chunk + warp; i <= i1; i += WARPS) {
+      const long long slot = (long long)i + b;
+      if (e < in.E) {
+        p += w.prob[slot * in.E + e];
+        c += w.count[slot * in.E + e];
+      }
+      n += w.rows[slot];
+    }
+  }
+  s_p[warp][lane] = p;
+  s_c[warp][lane] = c;
+  if (lane == 0) s_n[warp] = n;
+  __syncthreads();
+  if (warp == 0) {
+    for (int k = 1; k < WARPS; ++k) {
+      p += s_p[k][lane];
+      c += s_c[k][lane];
+      n += s_n[k];
+    }
+    float term = 0.f;
+    if (e < in.E) {
+      counts[(long long)b * in.E + e] = c;
+      prob[(long long)b * in.E + e] = p;
+      if (n > 0) term = ((float)in.E * (float)c / ((float)in.K * (float)n)) * (p / (float)n);
+    }
+    term = warp_sum(term);
+    if (lane == 0) {
+      w.term[blockIdx.x] = term;
+      if (g == 0) rows[b] = n;
+      __threadfence();
+      s_last = atomicAdd(w.done, 1u) == gridDim.x - 1;
+    }
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  float sum = 0.f;
+  int full = 0;
+  for (long long i = threadIdx.x; i < (long long)gridDim.x; i += THREADS) sum += __ldcg(&w.term[i]);
+  for (int i = threadIdx.x; i < in.B; i += THREADS) full += __ldcg(&rows[i]) > 0;
+  sum = warp_sum(sum);
+  full = __reduce_add_sync(0xffffffffu, full);
+  if (lane == 0) {
+    s_p[warp][0] = sum;
+    s_c[warp][0] = full;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < WARPS; ++k) {
+      sum += s_p[k][0];
+      full += s_c[k][0];
+    }
+    *loss = alpha * sum / (float)max(full, 1);
+  }
+}
+
+// ---------------------------------------------------------------- backward
+struct RouteBackward {
+  float alpha;
+  const int* counts;    // [B, E] or null: no balance term
+  const int* rows;      // [B]
+  const float* dloss;   // [1] or null (1)
+  const float* dwts;    // [T, K] or null: no weight term
+  const bf16* rs;       // [1]
+  void* dS;             // [T, ldd] f32 or bf16
+  long long ldd;
+  int bf16_out;
+  int vec_out;          // rows may be stored 4 elements at a time
+};
+
+// A warp takes consecutive rows, so a sequence's coefficients f stay in registers from row to row.  The weight term
+// touches K experts of a row: it is spread through a row of shared memory that is all zero between rows.
+template <int NV>
+__global__ void __launch_bounds__(bal::THREADS) route_backward_kernel(RouterRows in, RouteBackward q) {
+  using namespace bal;
+  __shared__ float s_add[WARPS][128 * NV];
+  __shared__ int s_full[WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* add = s_add[warp];
+  if (q.dwts) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) *reinterpret_cast<float4*>(add + (j * 32 + lane) * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  float scale = 0.f;  // alpha dloss E / (B' K)
+  if (q.counts) {
+    int full = 0;
+    for (int i = threadIdx.x; i < in.B; i += THREADS) full += q.rows[i] > 0;
+    full = __reduce_add_sync(0xffffffffu, full);
+    if (lane == 0) s_full[warp] = full;
+    __syncthreads();
+    full = 0;
+    for (int k = 0; k < WARPS; ++k) full += s_full[k];
+    scale = q.alpha * (q.dloss ? *q.dloss : 1.0f) * ((float)in.E / ((float)max(full, 1) * (float)in.K));
+  }
+  const float rs = q.dwts ? __bfloat162float(q.rs[0]) : 0.f;
+  const long long warps = (long long)gridDim.x * WARPS, w = (long long)blockIdx.x * WARPS + warp;
+  const int t0 = (int)(w * in.T / warps), t1 = (int)((w + 1) * in.T / warps);
+  int cur = -1;
+  float f[4 * NV];
+#pragma unroll
+  for (int i = 0; i < 4 * NV; ++i) f[i] = 0.f;
+  for (int t = t0; t < t1; ++t) {
+    const float* row = in.S + t * in.lds;
+    int b = -1;
+    if (q.counts && !(in.mask && in.mask[t] == 0)) {
+      if (!in.seq) b = 0;
+      else if (t >= in.seq[0] && t < in.seq[in.B]) b = seq_of(in.seq, in.B, t);
+    }
+    float v[4 * NV];
+#pragma unroll
+    for (int i = 0; i < 4 * NV; ++i) v[i] = 0.f;
+    if (b >= 0) {
+      load_row<NV>(row, in.E, in.vec, lane, v);
+      if (b != cur) {
+        cur = b;
+        const int n = q.rows[b];
+        const float k = n > 0 ? scale / (float)n / (float)n : 0.f;
+        const int* cb = q.counts + (long long)b * in.E;
+#pragma unroll
+        for (int i = 0; i < 4 * NV; ++i) {
+          const int e = ((i >> 2) * 32 + lane) * 4 + (i & 3);
+          f[i] = e < in.E ? k * (float)cb[e] : 0.f;
+        }
+      }
+      float z = 0.f, m = 0.f, slope[4 * NV];
+#pragma unroll
+      for (int i = 0; i < 4 * NV; ++i) {
+        float u, r;
+        const float s = sigmoid_of(v[i], u, r);
+        z += s;
+        m += f[i] * s;
+        slope[i] = u * r * r;
+      }
+      z = warp_sum(z) + TINY;
+      m = warp_sum(m) / z;
+      const float inv = __frcp_rn(z);
+#pragma unroll
+      for (int i = 0; i < 4 * NV; ++i) v[i] = (f[i] - m) * (slope[i] * inv);
+    }
+    if (q.dwts) {
+      int e = -1;
+      float s = 0.f, g = 0.f, slope = 0.f;
+      if (lane < in.K) {
+        e = in.idx[(long long)t * in.K + lane];
+        if (e < 0 || e >= in.E) e = -1;
+        if (e >= 0) {
+          float u, r;
+          s = sigmoid_of(row[e], u, r);
+          slope = u * r * r;
+          g = q.dwts[(long long)t * in.K + lane];
+        }
+      }
+      const float den = warp_sum(s) + TINY;
+      const float mean = warp_sum(g * s) / den;
+      const float mine = rs / den * (g - mean) * slope;
+      // an expert named twice gets both parts, added in pick order
+      const u32 peers = __match_any_sync(0xffffffffu, e);
+      if (__all_sync(0xffffffffu, e < 0 || (peers & (peers - 1)) == 0)) {
+        if (e >= 0) add[e] = mine;
+      } else {
+        for (int k = 0; k < in.K; ++k) {
+          if (lane == k && e >= 0) add[e] += mine;
+          __syncwarp();
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const float4 a = *reinterpret_cast<const float4*>(add + (j * 32 + lane) * 4);
+        v[4 * j] += a.x;
+        v[4 * j + 1] += a.y;
+        v[4 * j + 2] += a.z;
+        v[4 * j + 3] += a.w;
+      }
+      __syncwarp();
+      if (e >= 0) add[e] = 0.f;
+      __syncwarp();
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * 32 + lane) * 4;
+      if (q.bf16_out) {
+        bf16* d = reinterpret_cast<bf16*>(q.dS) + t * q.ldd + c;
+        if (q.vec_out && c + 4 <= in.E) {
+          *reinterpret_cast<uint2*>(d) =
+              make_uint2(f2_to_bf16x2(v[4 * j], v[4 * j + 1]), f2_to_bf16x2(v[4 * j + 2], v[4 * j + 3]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (c + i < in.E) d[i] = __float2bfloat16_rn(v[4 * j + i]);
+        }
+      } else {
+        float* d = reinterpret_cast<float*>(q.dS) + t * q.ldd + c;
+        if (q.vec_out && c + 4 <= in.E) {
+          *reinterpret_cast<float4*>(d) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (c + i < in.E) d[i] = v[4 * j + i];
+        }
+      }
+    }
+  }
+}
+
+}  // namespace k3

@@ -5,6 +5,7 @@
 
 #include <cstdio>
 #include <mutex>
+#include <type_traits>
 #include <vector>
 
 #include "../../include/k3moe.h"
@@ -14,6 +15,8 @@
 #include "ep_peer.cu"
 #include "ep_device.cu"
 #include "router.cu"
+#include "balance.cu"
+#include "int8.cu"
 #include "dropin.cu"
 
 using namespace k3;
@@ -46,7 +49,7 @@ int current_device() {
 template <typename F>
 bool set_smem_once(F kernel, int bytes, int slot) {
   static std::mutex mu;
-  static bool done[kMaxDevices][8] = {};
+  static bool done[kMaxDevices][16] = {};
   const int dev = current_device();
   std::lock_guard<std::mutex> g(mu);
   if (dev >= 0 && dev < kMaxDevices && done[dev][slot]) return true;
@@ -229,6 +232,151 @@ LayerLayout layer_layout(int T, int H, int I, int E, int K, int shared) {
 
 }  // namespace
 
+namespace {
+
+// rows a block of the first pass takes: about two blocks an SM over the rows, a multiple of its 8 warps.  A function
+// of T alone, so that the scratch size is too.
+int balance_chunk(int T) { return std::max(8, (int)align_up((size_t)cdiv(T, 2 * 148), 8)); }
+
+struct BalanceLayout {
+  int chunk, blocks;
+  size_t prob, count, rows, term, done, total;
+};
+BalanceLayout balance_layout(int T, int E, int B) {
+  BalanceLayout L;
+  L.chunk = balance_chunk(T);
+  L.blocks = std::max(1, (int)cdiv(T, L.chunk));
+  const size_t slots = (size_t)L.blocks + B;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at = align_up(at + bytes, 256);
+    return o;
+  };
+  L.prob = take(slots * E * 4);
+  L.count = take(slots * E * 4);
+  L.rows = take(slots * 4);
+  L.term = take((size_t)B * cdiv(E, bal::COLS) * 4);
+  L.done = take(4);
+  L.total = at;
+  return L;
+}
+
+bool router_sizes_ok(int T, int E, int K, int B, const int32_t* seq, int lds) {
+  return T >= 0 && E >= 1 && E <= 1024 && K >= 1 && K <= 16 && lds >= E && B >= 1 && (seq || B == 1) &&
+         (long long)B * cdiv(E, bal::COLS) < 0x7fffffffLL && (long long)B < 0x7fffffffLL - T;
+}
+
+RouterRows router_rows(const float* S, int lds, const int32_t* idx, int T, int E, int K, const int32_t* seq, int B,
+                       const uint8_t* mask) {
+  RouterRows r;
+  r.S = S;
+  r.lds = lds;
+  r.idx = idx;
+  r.seq = seq;
+  r.mask = mask;
+  r.T = T;
+  r.E = E;
+  r.K = K;
+  r.B = B;
+  r.vec = lds % 4 == 0 && reinterpret_cast<uintptr_t>(S) % 16 == 0;
+  return r;
+}
+
+// f(std::integral_constant<int, NV>): NV groups of 128 experts cover E
+template <typename F>
+void by_experts(int E, F f) {
+  switch ((E + 127) / 128) {
+    case 1: f(std::integral_constant<int, 1>{}); break;
+    case 2: f(std::integral_constant<int, 2>{}); break;
+    case 3: f(std::integral_constant<int, 3>{}); break;
+    case 4: f(std::integral_constant<int, 4>{}); break;
+    case 5: f(std::integral_constant<int, 5>{}); break;
+    case 6: f(std::integral_constant<int, 6>{}); break;
+    case 7: f(std::integral_constant<int, 7>{}); break;
+    default: f(std::integral_constant<int, 8>{}); break;
+  }
+}
+
+}  // namespace
+
+namespace {
+
+template <int SRC, int LANES, int NV>
+int launch_quant_int8(const QuantRows& p, cudaStream_t s) {
+  const long long blocks = cdiv(p.rows, 256 / LANES);
+  const int grid = (int)std::min<long long>(blocks, (long long)num_sms(current_device()) * 16);
+  quant_int8_kernel<SRC, LANES, NV><<<grid, 256, 0, s>>>(p);
+  return launch_status();
+}
+
+// a warp a row up to 1024 columns, then a block; rows of up to 16384 columns stay in registers
+template <int SRC>
+int quant_int8(const QuantRows& p, cudaStream_t s) {
+  if (p.rows == 0) return K3MOE_OK;
+  const int groups = (p.cols + 15) / 16;
+  if (groups <= 32) return launch_quant_int8<SRC, 32, 1>(p, s);
+  if (groups <= 64) return launch_quant_int8<SRC, 32, 2>(p, s);
+  if (groups <= 256) return launch_quant_int8<SRC, 256, 1>(p, s);
+  if (groups <= 512) return launch_quant_int8<SRC, 256, 2>(p, s);
+  if (groups <= 1024) return launch_quant_int8<SRC, 256, 4>(p, s);
+  return launch_quant_int8<SRC, 256, 0>(p, s);
+}
+
+bool int8_rows_ok(const void* q, long long ldq, int cols) {
+  return q && reinterpret_cast<uintptr_t>(q) % 16 == 0 && ldq % 16 == 0 && cols >= 1 && ldq >= cols;
+}
+
+// a map over int8 rows: boxes of 128 bytes of K by `box` rows, 128-byte swizzle; zeros past the ends
+int encode_int8(CUtensorMap* m, const void* base, long long rows, int cols, long long ld, int box) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return K3MOE_EDRIVER;
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t boxes[2] = {i8::BK, (cuuint32_t)box};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, boxes, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? K3MOE_OK : K3MOE_ETMAP;
+}
+
+int int8_launch(const int8_t* q, long long q_rows, long long ldq, const int8_t* w, long long w_rows, long long ldw,
+                int C, Int8Params& p, int grid, cudaStream_t s) {
+  CUtensorMap tw, tx;
+  int rc = encode_int8(&tw, w, w_rows, C, ldw, i8::BM);
+  if (rc) return rc;
+  rc = encode_int8(&tx, q, q_rows, C, ldq, p.xbox);
+  if (rc) return rc;
+  p.kstages = (int)cdiv(C, i8::BK);
+  p.n_tiles = (int)cdiv(p.N, i8::BM);
+  p.stage_bytes = i8::W_BYTES + p.bn * i8::BK;
+  p.stages = std::min(i8::MAX_STAGES, i8::RING_BYTES / p.stage_bytes);
+  p.tmem_cols = 32;
+  while (p.tmem_cols < 2u * p.bn) p.tmem_cols *= 2;
+  if (!set_smem_once(int8_gemm_kernel, i8::SMEM_BYTES, 4)) return K3MOE_ELAUNCH;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(i8::THREADS);
+  cfg.dynamicSmemBytes = i8::SMEM_BYTES;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  if (p.splits > 1) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)p.splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  if (cudaLaunchKernelEx(&cfg, int8_gemm_kernel, tw, tx, p) != cudaSuccess) {
+    cudaGetLastError();
+    return K3MOE_ELAUNCH;
+  }
+  return launch_status();
+}
+
+}  // namespace
+
 extern "C" {
 
 int k3moe_abi_version(void) { return 1; }
@@ -405,6 +553,196 @@ int k3moe_router_gemm(const void* x_bf16, int ldx, const void* w_bf16, int ldw, 
   if (!set_smem_once(router_gemm_kernel, rgemm::SMEM_BYTES, 3)) return K3MOE_ELAUNCH;
   router_gemm_kernel<<<grid, rgemm::THREADS, rgemm::SMEM_BYTES, reinterpret_cast<cudaStream_t>(stream)>>>(mx, mw, p);
   return launch_status();
+}
+
+// ---------------------------------------------------------------- the router's training side
+
+size_t k3moe_balance_scratch_bytes(int T, int E, int B) {
+  if (T < 0 || E < 1 || E > 1024 || B < 1) return 0;
+  return balance_layout(T, E, B).total;
+}
+
+int k3moe_balance_loss(const float* S, int lds, const int32_t* idx, int T, int E, int K, const int32_t* seq, int B,
+                       const uint8_t* mask, float alpha, void* scratch, int32_t* counts, float* prob, int32_t* rows,
+                       float* loss, k3moe_stream_t stream) {
+  if (!router_sizes_ok(T, E, K, B, seq, lds) || (T > 0 && (!S || !idx)) || !scratch ||
+      reinterpret_cast<uintptr_t>(scratch) % 16 || !counts || !prob || !rows || !loss)
+    return K3MOE_EINVAL;
+  const BalanceLayout L = balance_layout(T, E, B);
+  char* ws = reinterpret_cast<char*>(scratch);
+  BalanceScratch w;
+  w.prob = reinterpret_cast<float*>(ws + L.prob);
+  w.count = reinterpret_cast<int*>(ws + L.count);
+  w.rows = reinterpret_cast<int*>(ws + L.rows);
+  w.term = reinterpret_cast<float*>(ws + L.term);
+  w.done = reinterpret_cast<u32*>(ws + L.done);
+  const RouterRows in = router_rows(S, lds, idx, T, E, K, seq, B, mask);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  by_experts(E, [&](auto nv) {
+    balance_rows_kernel<decltype(nv)::value><<<L.blocks, bal::THREADS, 0, s>>>(in, w, L.chunk);
+  });
+  const long long blocks = (long long)B * cdiv(E, bal::COLS);
+  balance_join_kernel<<<(unsigned)blocks, bal::THREADS, 0, s>>>(in, w, L.chunk, alpha, counts, prob, rows, loss);
+  return launch_status();
+}
+
+int k3moe_route_backward(const float* S, int lds, const int32_t* idx, int T, int E, int K, const int32_t* seq, int B,
+                         const uint8_t* mask, float alpha, const int32_t* counts, const int32_t* rows,
+                         const float* dloss, const float* dwts, const void* rs_bf16, void* dS, int ldd, int dtype,
+                         k3moe_stream_t stream) {
+  if (!router_sizes_ok(T, E, K, B, seq, lds) || ldd < E || (dtype != K3MOE_BF16 && dtype != K3MOE_F32) ||
+      (counts && !rows) || (dwts && !rs_bf16) || (T > 0 && ((!counts && !dwts) || !S || !dS || (dwts && !idx))))
+    return K3MOE_EINVAL;
+  if (T == 0) return K3MOE_OK;
+  const RouterRows in = router_rows(S, lds, idx, T, E, K, seq, B, mask);
+  RouteBackward q;
+  q.alpha = alpha;
+  q.counts = counts;
+  q.rows = rows;
+  q.dloss = dloss;
+  q.dwts = dwts;
+  q.rs = reinterpret_cast<const bf16*>(rs_bf16);
+  q.dS = dS;
+  q.ldd = ldd;
+  q.bf16_out = dtype == K3MOE_BF16;
+  q.vec_out = ldd % 4 == 0 && reinterpret_cast<uintptr_t>(dS) % (q.bf16_out ? 8 : 16) == 0;
+  const int grid = (int)std::min<long long>(cdiv(T, bal::WARPS), (long long)num_sms(current_device()) * 4);
+  by_experts(E, [&](auto nv) {
+    route_backward_kernel<decltype(nv)::value>
+        <<<grid, bal::THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(in, q);
+  });
+  return launch_status();
+}
+
+// ---------------------------------------------------------------- products in 8-bit integers
+
+int k3moe_quant_int8(const void* x, int dtype, long long ldx, long long rows, int cols, int8_t* q, long long ldq,
+                     float* scale, k3moe_stream_t stream) {
+  if (rows < 0 || (dtype != K3MOE_BF16 && dtype != K3MOE_F32) || ldx < cols || cols < 1) return K3MOE_EINVAL;
+  if (rows == 0) return K3MOE_OK;
+  if (!x || !scale || !int8_rows_ok(q, ldq, cols)) return K3MOE_EINVAL;
+  QuantRows p = {};
+  p.x = x;
+  p.ldx = ldx;
+  p.rows = rows;
+  p.cols = cols;
+  p.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx % (dtype == K3MOE_BF16 ? 8 : 4) == 0;
+  p.q = q;
+  p.ldq = ldq;
+  p.scale = scale;
+  p.cap_rows = rows;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == K3MOE_BF16 ? quant_int8<I8_BF16>(p, s) : quant_int8<I8_F32>(p, s);
+}
+
+int k3moe_act_quant_int8(const void* gu_bf16, long long ldg, long long rows, int I, int activation,
+                         const int32_t* cta_limit, const int32_t* meta, int max_ctas, int8_t* q, long long ldq,
+                         float* scale, k3moe_stream_t stream) {
+  if (rows < 0 || I < 1 || ldg < 2LL * I || (activation != K3MOE_ACT_SWIGLU && activation != K3MOE_ACT_SITU) ||
+      (cta_limit == nullptr) != (meta == nullptr) || (meta && max_ctas < 1))
+    return K3MOE_EINVAL;
+  if (rows == 0) return K3MOE_OK;
+  if (!gu_bf16 || !scale || !int8_rows_ok(q, ldq, I)) return K3MOE_EINVAL;
+  QuantRows p = {};
+  p.x = gu_bf16;
+  p.ldx = ldg;
+  p.rows = rows;
+  p.cols = I;
+  p.vec = reinterpret_cast<uintptr_t>(gu_bf16) % 16 == 0 && ldg % 8 == 0 && I % 8 == 0;
+  p.act = activation;
+  p.q = q;
+  p.ldq = ldq;
+  p.scale = scale;
+  p.cta_limit = cta_limit;
+  p.meta = meta;
+  p.max_ctas = max_ctas;
+  p.cap_rows = rows;
+  return quant_int8<I8_GATED>(p, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int k3moe_quant_int8_permute(const void* x_bf16, long long ldx, int R, int cols, int K, const int32_t* exp2perm,
+                             const int32_t* meta, int8_t* q_perm, long long ldq, float* scale_perm, int cap_rows,
+                             k3moe_stream_t stream) {
+  if (R < 0 || cols < 1 || ldx < cols || K < 1 || K > 16 || cap_rows < 1) return K3MOE_EINVAL;
+  if (R == 0) return K3MOE_OK;
+  if (!x_bf16 || !exp2perm || !meta || !scale_perm || !int8_rows_ok(q_perm, ldq, cols)) return K3MOE_EINVAL;
+  QuantRows p = {};
+  p.x = x_bf16;
+  p.ldx = ldx;
+  p.rows = R;
+  p.cols = cols;
+  p.vec = reinterpret_cast<uintptr_t>(x_bf16) % 16 == 0 && ldx % 8 == 0;
+  p.q = q_perm;
+  p.ldq = ldq;
+  p.scale = scale_perm;
+  p.exp2perm = exp2perm;
+  p.K = K;
+  p.meta = meta;
+  p.cap_rows = cap_rows;
+  return quant_int8<I8_BF16>(p, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int k3moe_gemm_int8(const int8_t* q, long long ldq, const float* sx, const int8_t* w, long long ldw, const float* sw,
+                    int T, int N, int C, void* out, long long ldo, int dtype, uint32_t* err, k3moe_stream_t stream) {
+  if (T < 0 || N < 1 || C < 1 || C > 131071 || ldo < N || (dtype != K3MOE_BF16 && dtype != K3MOE_F32))
+    return K3MOE_EINVAL;
+  if (T == 0) return K3MOE_OK;
+  if (!sx || !sw || !out || !int8_rows_ok(q, ldq, C) || !int8_rows_ok(w, ldw, C) ||
+      reinterpret_cast<uintptr_t>(out) % (dtype == K3MOE_F32 ? 4 : 2))
+    return K3MOE_EINVAL;
+  const int sms = num_sms(current_device());
+  Int8Params p = {};
+  p.sx = sx;
+  p.sw = sw;
+  p.out = out;
+  p.ldo = ldo;
+  p.f32_out = dtype == K3MOE_F32;
+  p.T = T;
+  p.N = N;
+  p.err = err;
+  const long long n_tiles = cdiv(N, i8::BM);
+  p.bn = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
+  while (p.bn > 64 && n_tiles * cdiv(T, p.bn) < sms) p.bn /= 2;
+  p.xbox = p.bn;
+  p.t_tiles = (int)cdiv(T, p.bn);
+  const long long units = n_tiles * p.t_tiles;
+  if (units > 0x7fffffffLL) return K3MOE_EINVAL;
+  p.splits = 1;
+  while (p.splits < 8 && units * p.splits * 2 <= sms && cdiv(C, i8::BK) >= 8 * p.splits) p.splits *= 2;
+  const int grid = p.splits > 1 ? (int)units * p.splits : (int)std::min<long long>(units, sms);
+  return int8_launch(q, T, ldq, w, N, ldw, C, p, grid, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int k3moe_grouped_gemm_int8(const int8_t* q_perm, long long ldq, const float* sx_perm, const int8_t* w, long long ldw,
+                            const float* sw, const int32_t* cta_batch, const int32_t* cta_limit, const int32_t* meta,
+                            int N, int C, int n_experts, int cap_rows, int max_ctas, void* out, long long ldo,
+                            int dtype, uint32_t* err, k3moe_stream_t stream) {
+  if (N < 1 || C < 1 || C > 131071 || n_experts < 1 || max_ctas < 1 || (long long)max_ctas * 128 > cap_rows ||
+      ldo < N || (dtype != K3MOE_BF16 && dtype != K3MOE_F32) || !sx_perm || !sw || !cta_batch || !cta_limit || !meta ||
+      !out || !int8_rows_ok(q_perm, ldq, C) || !int8_rows_ok(w, ldw, C) ||
+      reinterpret_cast<uintptr_t>(out) % (dtype == K3MOE_F32 ? 4 : 2) || (long long)n_experts * N > 0x7fffffffLL ||
+      max_ctas * cdiv(N, i8::BM) > 0x7fffffffLL)
+    return K3MOE_EINVAL;
+  Int8Params p = {};
+  p.sx = sx_perm;
+  p.sw = sw;
+  p.out = out;
+  p.ldo = ldo;
+  p.f32_out = dtype == K3MOE_F32;
+  p.N = N;
+  p.err = err;
+  p.bn = 128;
+  p.xbox = 32;
+  p.splits = 1;
+  p.cta_batch = cta_batch;
+  p.cta_limit = cta_limit;
+  p.meta = meta;
+  p.n_experts = n_experts;
+  p.max_ctas = max_ctas;
+  p.cap_rows = cap_rows;
+  const int grid = (int)std::min<long long>(max_ctas * cdiv(N, i8::BM), num_sms(current_device()));
+  return int8_launch(q_perm, cap_rows, ldq, w, (long long)n_experts * N, ldw, C, p, grid,
+                     reinterpret_cast<cudaStream_t>(stream));
 }
 
 int k3moe_gemm_tensor_maps(int mode, const uint8_t* w, const uint8_t* act, int n_experts, int H, int I, int cap_rows,

@@ -10,6 +10,7 @@ exception is raised.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from dataclasses import dataclass
 
@@ -77,6 +78,14 @@ SIGNATURES = {
     "k3moe_ipc_import": (_I, [_P, _U64, _P]),
     "k3moe_ipc_release": (_I, [_P, _U64]),
     "k3moe_router_gemm": (_I, [_P, _I, _P, _I, _I, _I, _I, _P, _I, _P, _P]),
+    "k3moe_balance_scratch_bytes": (_SZ, [_I, _I, _I]),
+    "k3moe_balance_loss": (_I, [_P, _I, _P, _I, _I, _I, _P, _I, _P, _F, _P, _P, _P, _P, _P, _P]),
+    "k3moe_route_backward": (_I, [_P, _I, _P, _I, _I, _I, _P, _I, _P, _F, _P, _P, _P, _P, _P, _P, _I, _I, _P]),
+    "k3moe_quant_int8": (_I, [_P, _I, _L, _L, _I, _P, _L, _P, _P]),
+    "k3moe_act_quant_int8": (_I, [_P, _L, _L, _I, _I, _P, _P, _I, _P, _L, _P, _P]),
+    "k3moe_quant_int8_permute": (_I, [_P, _L, _I, _I, _I, _P, _P, _P, _L, _P, _I, _P]),
+    "k3moe_gemm_int8": (_I, [_P, _L, _P, _P, _L, _P, _I, _I, _I, _P, _L, _I, _P, _P]),
+    "k3moe_grouped_gemm_int8": (_I, [_P, _L, _P, _P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _L, _I, _P, _P]),
     "k3moe_ep_peer_bytes": (_SZ, [_P]),
     "k3moe_ep_workspace_bytes": (_SZ, [_P]),
     "k3moe_ep_create": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P, _P]),
@@ -330,6 +339,254 @@ def read_error(err: torch.Tensor, clear: bool = True, stream=None):
     out = (ctypes.c_uint32 * 2)()
     rc = lib().k3moe_read_error(_p(err), ctypes.cast(out, ctypes.c_void_p), int(clear), _stream(stream))
     return rc, (out[0], out[1])
+
+
+# ------------------------------------------------------------------ argument checks of the entries below
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise K3MoeError(what)
+
+
+def _rows(t, name: str, dtypes, cols: int | None = None, rows: int | None = None, dev=None) -> int:
+    """Check a matrix argument (device, dtype, shape, rows that are runs of elements, none shared); its row stride."""
+    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name}: a CUDA tensor is needed")
+    _need(t.dtype in dtypes, f"{name}: dtype {t.dtype} (one of {dtypes} is needed)")
+    _need(t.dim() == 2 and (cols is None or t.shape[1] == cols) and (rows is None or t.shape[0] == rows),
+          f"{name}: shape {tuple(t.shape)} (rows {rows}, columns {cols} are needed)")
+    _need(dev is None or t.device == dev, f"{name}: on {t.device}, the other tensors on {dev}")
+    n, c = t.shape
+    if n > 1:
+        _need((t.stride(1) == 1 or c == 1) and t.stride(0) >= c, f"{name}: strides {t.stride()} (contiguous rows are needed)")
+        return t.stride(0)
+    _need(t.stride(1) == 1 or c <= 1, f"{name}: strides {t.stride()} (contiguous rows are needed)")
+    return c
+
+
+def _vec(t, name: str, dtypes, n: int | None, dev) -> None:
+    """Check a contiguous array argument of n elements (None: any number)."""
+    _need(isinstance(t, torch.Tensor) and t.device == dev and t.dtype in dtypes and t.is_contiguous()
+          and (n is None or t.numel() == n), f"{name}: a contiguous tensor of {n} elements of {dtypes} on {dev} is needed")
+
+
+def _int8_rows(t, name: str, dev=None, cols: int | None = None, rows: int | None = None) -> int:
+    """_rows of an int8 operand: 16-byte aligned, row stride a multiple of 16 (of one row: rounded up)."""
+    ld = _rows(t, name, (torch.int8,), cols, rows, dev)
+    if t.shape[0] <= 1:
+        ld = -(-max(t.shape[1], 1) // 16) * 16
+    _need(ld % 16 == 0 and t.data_ptr() % 16 == 0, f"{name}: 16-byte aligned rows are needed (quant_int8 pads them)")
+    return ld
+
+
+def _launch(fn, what: str, dev, *args) -> None:
+    """Call an entry on `dev`'s current stream, with `dev` the current device."""
+    if dev.index == torch.cuda.current_device():
+        _check(fn(*args, torch.cuda.current_stream().cuda_stream), what)
+    else:
+        with torch.cuda.device(dev):
+            _check(fn(*args, torch.cuda.current_stream().cuda_stream), what)
+
+
+def _on_stream(f):
+    """The `stream` argument of the entries below: the call, its allocations included, on that stream."""
+    @functools.wraps(f)
+    def call(*args, stream=None, **kw):
+        if stream is None:
+            return f(*args, **kw)
+        with torch.cuda.stream(stream):
+            return f(*args, **kw)
+    return call
+
+
+def _out_dtype(dtype) -> int:
+    _need(dtype in (torch.bfloat16, torch.float32), f"dtype {dtype} (torch.bfloat16 or torch.float32 is needed)")
+    return F32 if dtype == torch.float32 else BF16
+
+
+BF16, F32 = 0, 1  # include/k3moe.h K3MOE_BF16, K3MOE_F32
+
+
+# ------------------------------------------------------------------ the router's training side
+@dataclass
+class BalanceStats:
+    loss: torch.Tensor    # f32 [1]
+    counts: torch.Tensor  # int32 [B, E]: picks of an expert in a sequence
+    prob: torch.Tensor    # f32 [B, E]: sums of the normalised scores
+    rows: torch.Tensor    # int32 [B]: counted rows
+
+
+def _router_args(S, idx, seq, mask):
+    ld = _rows(S, "S", (torch.float32,))
+    dev, (T, E) = S.device, S.shape
+    _need(idx.dim() == 2 and idx.shape[0] == T, f"idx: shape {tuple(idx.shape)} ([{T}, K] is needed)")
+    _vec(idx, "idx", (torch.int32,), None, dev)
+    B = 1
+    if seq is not None:
+        _vec(seq, "seq", (torch.int32,), None, dev)
+        B = seq.numel() - 1
+        _need(seq.dim() == 1 and B >= 1, "seq: int32 offsets [B + 1] are needed")
+    if mask is not None:
+        _vec(mask, "mask", (torch.uint8, torch.bool), T, dev)
+    return dev, T, E, idx.shape[1], B, max(ld, E)
+
+
+@_on_stream
+def balance_loss(S: torch.Tensor, idx: torch.Tensor, alpha: float, seq: torch.Tensor | None = None,
+                 mask: torch.Tensor | None = None) -> BalanceStats:
+    """The router's load-balance loss over the top-k's picks, and its counts (k3moe_balance_loss).
+
+    S f32 [T, E] router logits; idx int32 [T, K] (route_topk's); seq int32 [B + 1] offsets of packed sequences (None:
+    one sequence); mask [T] uint8 or bool, rows with 0 are not counted."""
+    dev, T, E, K, B, ld = _router_args(S, idx, seq, mask)
+    L = lib()
+    scratch = torch.empty(max(L.k3moe_balance_scratch_bytes(T, E, B), 16), dtype=torch.uint8, device=dev)
+    s = BalanceStats(loss=torch.empty(1, dtype=torch.float32, device=dev),
+                     counts=torch.empty((B, E), dtype=torch.int32, device=dev),
+                     prob=torch.empty((B, E), dtype=torch.float32, device=dev),
+                     rows=torch.empty(B, dtype=torch.int32, device=dev))
+    _launch(L.k3moe_balance_loss, "balance_loss", dev, _p(S), ld, _p(idx), T, E, K, _p(seq), B, _p(mask), alpha,
+            _p(scratch), _p(s.counts), _p(s.prob), _p(s.rows), _p(s.loss))
+    return s
+
+
+@_on_stream
+def route_backward(S: torch.Tensor, idx: torch.Tensor, alpha: float = 0.0, counts: torch.Tensor | None = None,
+                   rows: torch.Tensor | None = None, dloss: torch.Tensor | None = None,
+                   dwts: torch.Tensor | None = None, rs: torch.Tensor | None = None, seq: torch.Tensor | None = None,
+                   mask: torch.Tensor | None = None, dtype: torch.dtype = torch.float32,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """dS [T, E] (k3moe_route_backward): the balance term where counts and rows (balance_loss's, with its alpha, seq
+    and mask) are given, dloss its scalar gradient (None: 1); plus the weight term where dwts [T, K], the gradient of
+    route_topk's weights, and rs are given."""
+    dev, T, E, K, B, ld = _router_args(S, idx, seq, mask)
+    _need((counts is None) == (rows is None), "counts and rows are given together")
+    _need((dwts is None) or (rs is not None), "dwts needs rs")
+    _need(counts is not None or dwts is not None, "counts and rows, or dwts and rs, are needed")
+    if counts is not None:
+        _vec(counts, "counts", (torch.int32,), B * E, dev)
+        _vec(rows, "rows", (torch.int32,), B, dev)
+    if dloss is not None:
+        _vec(dloss, "dloss", (torch.float32,), 1, dev)
+    if dwts is not None:
+        _vec(dwts, "dwts", (torch.float32,), T * K, dev)
+        _vec(rs, "rs", (torch.bfloat16,), 1, dev)
+    if out is None:
+        out = torch.empty((T, E), dtype=dtype, device=dev)
+    code = _out_dtype(out.dtype)
+    ldd = max(_rows(out, "out", (out.dtype,), E, T, dev), E)
+    _launch(lib().k3moe_route_backward, "route_backward", dev, _p(S), ld, _p(idx), T, E, K, _p(seq), B, _p(mask),
+            alpha, _p(counts), _p(rows), _p(dloss), _p(dwts), _p(rs), _p(out), ldd, code)
+    return out
+
+
+# ------------------------------------------------------------------ products in 8-bit integers
+def _int8_out(rows: int, cols: int, dev, out):
+    if out is None:
+        q = torch.empty((rows, -(-cols // 16) * 16), dtype=torch.int8, device=dev)[:, :cols]
+        return q, q.stride(0), torch.empty(rows, dtype=torch.float32, device=dev)
+    q, scale = out
+    ld = _int8_rows(q, "out q", dev, cols, rows)
+    _vec(scale, "out scale", (torch.float32,), rows, dev)
+    return q, ld, scale
+
+
+@_on_stream
+def quant_int8(x: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """Rows of x (bf16 or f32 [rows, cols]; tokens, or a weight's channels) to int8 with a scale each
+    (k3moe_quant_int8): (q int8 [rows, cols], its rows padded to 16 bytes; scale f32 [rows])."""
+    ldx = _rows(x, "x", (torch.bfloat16, torch.float32))
+    rows, cols = x.shape
+    q, ldq, scale = _int8_out(rows, cols, x.device, out)
+    _launch(lib().k3moe_quant_int8, "quant_int8", x.device, _p(x), F32 if x.dtype == torch.float32 else BF16,
+            max(ldx, cols), rows, cols, _p(q), ldq, _p(scale))
+    return q, scale
+
+
+@_on_stream
+def act_quant_int8(gu: torch.Tensor, activation: int = ACT_SWIGLU, tables: Tables | None = None,
+                   out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """act(gate) * up of bf16 rows [gate | up] to int8 (k3moe_act_quant_int8): (q [rows, cols / 2], scale).  With
+    tables, gu is [cap_rows, 2I] and only the tables' real rows are read and written."""
+    ldg = _rows(gu, "gu", (torch.bfloat16,))
+    rows, cols = gu.shape
+    _need(cols >= 2 and cols % 2 == 0, f"gu: {cols} columns (gate and up halves are needed)")
+    limit = meta = None
+    ctas = 0
+    if tables is not None:
+        _need(rows <= tables.max_ctas * 128, f"gu: {rows} rows, the tables cover {tables.max_ctas * 128}")
+        limit, meta, ctas = tables.cta_limit, tables.meta, tables.max_ctas
+        _vec(limit, "tables.cta_limit", (torch.int32,), ctas, gu.device)
+        _vec(meta, "tables.meta", (torch.int32,), None, gu.device)
+    q, ldq, scale = _int8_out(rows, cols // 2, gu.device, out)
+    _launch(lib().k3moe_act_quant_int8, "act_quant_int8", gu.device, _p(gu), max(ldg, cols), rows, cols // 2,
+            activation, _p(limit), _p(meta), ctas, _p(q), ldq, _p(scale))
+    return q, scale
+
+
+@_on_stream
+def quant_int8_permute(x: torch.Tensor, tables: Tables, out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """quant_int8 of bf16 rows, each written to every permuted row it is routed to (k3moe_quant_int8_permute):
+    (q [cap_rows, cols], scale [cap_rows]); padding rows are not written."""
+    ldx = _rows(x, "x", (torch.bfloat16,))
+    R, cols = x.shape
+    K = tables.exp2perm.shape[1]
+    _vec(tables.exp2perm, "tables.exp2perm", (torch.int32,), R * K, x.device)
+    _vec(tables.meta, "tables.meta", (torch.int32,), None, x.device)
+    q, ldq, scale = _int8_out(tables.cap_rows, cols, x.device, out)
+    _launch(lib().k3moe_quant_int8_permute, "quant_int8_permute", x.device, _p(x), max(ldx, cols), R, cols, K,
+            _p(tables.exp2perm), _p(tables.meta), _p(q), ldq, _p(scale), tables.cap_rows)
+    return q, scale
+
+
+def _product_args(q, sx, w, sw, dtype, out, err):
+    ldq = _int8_rows(q, "q")
+    dev, (T, C) = q.device, q.shape
+    ldw = _int8_rows(w, "w", dev, C)
+    _vec(sx, "sx", (torch.float32,), T, dev)
+    _vec(sw, "sw", (torch.float32,), w.shape[0], dev)
+    if err is not None:
+        _vec(err, "err", (torch.int32, torch.uint32), None, dev)
+        _need(err.numel() >= 2, "err: two words are needed")
+    return dev, T, C, ldq, ldw
+
+
+@_on_stream
+def gemm_int8(q: torch.Tensor, sx: torch.Tensor, w: torch.Tensor, sw: torch.Tensor,
+              dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
+              err: torch.Tensor | None = None) -> torch.Tensor:
+    """out[t, n] = sx[t] sw[n] (q[t] . w[n]) (k3moe_gemm_int8): q int8 [T, C], w int8 [N, C], rows 16-byte aligned as
+    quant_int8 gives them; out [T, N] bf16 or f32.  err: the device error words, or None."""
+    dev, T, C, ldq, ldw = _product_args(q, sx, w, sw, dtype, out, err)
+    N = w.shape[0]
+    if out is None:
+        out = torch.empty((T, N), dtype=dtype, device=dev)
+    code = _out_dtype(out.dtype)
+    ldo = max(_rows(out, "out", (out.dtype,), N, T, dev), N)
+    _launch(lib().k3moe_gemm_int8, "gemm_int8", dev, _p(q), ldq, _p(sx), _p(w), ldw, _p(sw), T, N, C, _p(out), ldo,
+            code, _p(err))
+    return out
+
+
+@_on_stream
+def grouped_gemm_int8(q: torch.Tensor, sx: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, tables: Tables,
+                      n_experts: int, dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
+                      err: torch.Tensor | None = None) -> torch.Tensor:
+    """The products of routed rows with their experts' weights (k3moe_grouped_gemm_int8): q int8 [cap_rows, C] permuted
+    rows, w int8 [n_experts * N, C], out [cap_rows, N]; padding rows of out are not written."""
+    dev, cap, C, ldq, ldw = _product_args(q, sx, w, sw, dtype, out, err)
+    _need(n_experts >= 1 and w.shape[0] % n_experts == 0, f"w: {w.shape[0]} rows are not {n_experts} experts'")
+    _need(cap == tables.cap_rows, f"q: {cap} rows, the tables' capacity is {tables.cap_rows}")
+    _vec(tables.cta_batch, "tables.cta_batch", (torch.int32,), tables.max_ctas, dev)
+    _vec(tables.cta_limit, "tables.cta_limit", (torch.int32,), tables.max_ctas, dev)
+    _vec(tables.meta, "tables.meta", (torch.int32,), None, dev)
+    N = w.shape[0] // n_experts
+    if out is None:
+        out = torch.empty((cap, N), dtype=dtype, device=dev)
+    code = _out_dtype(out.dtype)
+    ldo = max(_rows(out, "out", (out.dtype,), N, cap, dev), N)
+    _launch(lib().k3moe_grouped_gemm_int8, "grouped_gemm_int8", dev, _p(q), ldq, _p(sx), _p(w), ldw, _p(sw),
+            _p(tables.cta_batch), _p(tables.cta_limit), _p(tables.meta), N, C, n_experts, cap, tables.max_ctas,
+            _p(out), ldo, code, _p(err))
+    return out
 
 
 # ------------------------------------------------------------------ the layer
