@@ -19,8 +19,10 @@
 namespace k3 {
 
 namespace bal {
-constexpr int WARPS = 8;
+constexpr int WARPS = 8;         // of a block of the join and of the gradient
 constexpr int THREADS = 32 * WARPS;
+constexpr int ROW_WARPS = 16;    // of a block of the first pass
+constexpr int SEQ_MAX = 1024;    // offsets kept in shared memory
 constexpr float TINY = 1e-20f;  // the top-k's guard of its own sum
 constexpr int COLS = 32;        // experts a block of the second pass
 }  // namespace bal
@@ -79,10 +81,10 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // ---------------------------------------------------------------- forward
-// First pass: a block takes `chunk` consecutive rows, a warp every eighth of them, each lane summing its experts' p
-// in registers.  At the end of a sequence, or of the block's rows, the eight warps' sums are added and stored as one
-// partial row.  Block i and sequence b meet in slot i + b: along the rows either i or b goes up, so no two pairs
-// share a slot and nothing needs zeroing.
+// First pass: a block an SM takes `chunk` consecutive rows, a warp every sixteenth of them, each lane summing its
+// experts' p in registers while its next row is on the way.  At the end of a sequence, or of the block's rows, the
+// warps' sums are added in order and stored as one partial row.  Block i and sequence b meet in slot i + b: along the
+// rows either i or b goes up, so no two pairs share a slot and nothing needs zeroing.
 struct BalanceScratch {
   float* prob;   // [slots, E]
   int* count;    // [slots, E]
@@ -92,11 +94,13 @@ struct BalanceScratch {
 };
 
 template <int NV>
-__global__ void __launch_bounds__(bal::THREADS) balance_rows_kernel(RouterRows in, BalanceScratch w, int chunk) {
+__global__ void __launch_bounds__(32 * bal::ROW_WARPS) balance_rows_kernel(RouterRows in, BalanceScratch w, int chunk) {
   using namespace bal;
-  __shared__ float s_acc[WARPS][128 * NV];
+  constexpr int N = 4 * NV;
+  __shared__ float s_acc[ROW_WARPS / 2][128 * NV];
   __shared__ int s_hist[128 * NV];
-  __shared__ int s_rows[WARPS];
+  __shared__ int s_rows[ROW_WARPS];
+  grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r0 = blockIdx.x * chunk, r1 = min(in.T, r0 + chunk);
   if (blockIdx.x == 0 && threadIdx.x == 0) *w.done = 0u;
@@ -105,6 +109,11 @@ __global__ void __launch_bounds__(bal::THREADS) balance_rows_kernel(RouterRows i
     r = max(r0, in.seq[0]);
     last = min(r1, in.seq[in.B]);
   }
+  // the next counted row from t on in steps of the warps, or `end`
+  auto counted = [&](int t, int end) {
+    while (t < end && in.mask && in.mask[t] == 0) t += ROW_WARPS;
+    return t;
+  };
   while (r < last) {
     int b = 0, end = last;
     if (in.seq) {
@@ -112,49 +121,66 @@ __global__ void __launch_bounds__(bal::THREADS) balance_rows_kernel(RouterRows i
       end = min(last, in.seq[b + 1]);
       if (end <= r) break;  // offsets that go down: nothing more is counted
     }
-    for (int e = threadIdx.x; e < in.E; e += THREADS) s_hist[e] = 0;
-    __syncthreads();
-    float acc[4 * NV];
-#pragma unroll
-    for (int i = 0; i < 4 * NV; ++i) acc[i] = 0.f;
-    int n = 0;
-    for (int t = r + warp; t < end; t += WARPS) {
-      if (in.mask && in.mask[t] == 0) continue;
-      ++n;
-      float v[4 * NV];
+    float acc[N], v[N];
+    int pick = -1, n = 0;
+    int t = counted(r + warp, end);
+    if (t < end) {
       load_row<NV>(in.S + t * in.lds, in.E, in.vec, lane, v);
-      if (lane < in.K) {
-        const int e = in.idx[(long long)t * in.K + lane];
-        if (e >= 0 && e < in.E) atomicAdd(&s_hist[e], 1);
-      }
-      float z = 0.f;
+      if (lane < in.K) pick = in.idx[(long long)t * in.K + lane];
+    }
+    for (int e = threadIdx.x; e < in.E; e += 32 * ROW_WARPS) s_hist[e] = 0;
 #pragma unroll
-      for (int i = 0; i < 4 * NV; ++i) {
+    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    __syncthreads();
+    while (t < end) {
+      ++n;
+      float z = 0.f, s[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
         float u, q;
-        v[i] = sigmoid_of(v[i], u, q);
-        z += v[i];
+        s[i] = sigmoid_of(v[i], u, q);
+        z += s[i];
+      }
+      if (lane < in.K && pick >= 0 && pick < in.E) atomicAdd(&s_hist[pick], 1);
+      t = counted(t + ROW_WARPS, end);
+      if (t < end) {
+        load_row<NV>(in.S + t * in.lds, in.E, in.vec, lane, v);
+        if (lane < in.K) pick = in.idx[(long long)t * in.K + lane];
       }
       const float inv = __frcp_rn(warp_sum(z) + TINY);
 #pragma unroll
-      for (int i = 0; i < 4 * NV; ++i) acc[i] += v[i] * inv;
+      for (int i = 0; i < N; ++i) acc[i] += s[i] * inv;
     }
+    // the upper half of the warps, then the lower half onto them
+    float* mine = s_acc[warp % (ROW_WARPS / 2)];
+    if (warp >= ROW_WARPS / 2) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      *reinterpret_cast<float4*>(&s_acc[warp][(j * 32 + lane) * 4]) =
-          make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+      for (int j = 0; j < NV; ++j)
+        *reinterpret_cast<float4*>(mine + (j * 32 + lane) * 4) =
+            make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+    }
     if (lane == 0) s_rows[warp] = n;
     __syncthreads();
+    if (warp < ROW_WARPS / 2) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float4* q = reinterpret_cast<float4*>(mine + (j * 32 + lane) * 4);
+        const float4 o = *q;
+        *q = make_float4(o.x + acc[4 * j], o.y + acc[4 * j + 1], o.z + acc[4 * j + 2], o.w + acc[4 * j + 3]);
+      }
+    }
+    __syncthreads();
     const long long slot = (long long)blockIdx.x + b;
-    for (int e = threadIdx.x; e < in.E; e += THREADS) {
+    for (int e = threadIdx.x; e < in.E; e += 32 * ROW_WARPS) {
       float p = 0.f;
 #pragma unroll
-      for (int k = 0; k < WARPS; ++k) p += s_acc[k][e];
+      for (int k = 0; k < ROW_WARPS / 2; ++k) p += s_acc[k][e];
       w.prob[slot * in.E + e] = p;
       w.count[slot * in.E + e] = s_hist[e];
     }
     if (threadIdx.x == 0) {
       int total = 0;
-      for (int k = 0; k < WARPS; ++k) total += s_rows[k];
+      for (int k = 0; k < ROW_WARPS; ++k) total += s_rows[k];
       w.rows[slot] = total;
     }
     __syncthreads();
@@ -171,6 +197,7 @@ __global__ void __launch_bounds__(bal::THREADS)
   __shared__ float s_p[WARPS][COLS];
   __shared__ int s_c[WARPS][COLS], s_n[WARPS];
   __shared__ int s_last;
+  grid_wait_previous();  // the first pass's partial rows
   const int groups = (in.E + COLS - 1) / COLS;
   const int b = blockIdx.x / groups, g = blockIdx.x % groups;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -256,91 +283,114 @@ struct RouteBackward {
   int vec_out;          // rows may be stored 4 elements at a time
 };
 
-// A warp takes consecutive rows, so a sequence's coefficients f stay in registers from row to row.  The weight term
-// touches K experts of a row: it is spread through a row of shared memory that is all zero between rows.
+// A warp takes consecutive rows, with the next row's logits on their way while one is computed; the counts, which
+// neighbouring rows share, come from L1.  The weight term touches K experts of a row: it is spread through a row of
+// shared memory that is all zero between rows.
 template <int NV>
-__global__ void __launch_bounds__(bal::THREADS) route_backward_kernel(RouterRows in, RouteBackward q) {
+__global__ void __launch_bounds__(bal::THREADS, 2) route_backward_kernel(RouterRows in, RouteBackward q) {
   using namespace bal;
+  constexpr int N = 4 * NV;
   __shared__ float s_add[WARPS][128 * NV];
   __shared__ int s_full[WARPS];
+  __shared__ int s_seq[SEQ_MAX];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float* add = s_add[warp];
+  const long long warps = (long long)gridDim.x * WARPS, w = (long long)blockIdx.x * WARPS + warp;
+  const int t0 = (int)(w * in.T / warps), t1 = (int)((w + 1) * in.T / warps);
+  float v[N];
+  // a row's logits, where the balance term wants them
+  auto load = [&](int t) {
+    if (t < t1 && q.counts && !(in.mask && in.mask[t] == 0))
+      load_row<NV>(in.S + t * in.lds, in.E, in.vec, lane, v);
+  };
+  load(t0);
   if (q.dwts) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) *reinterpret_cast<float4*>(add + (j * 32 + lane) * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
   }
   float scale = 0.f;  // alpha dloss E / (B' K)
+  const int* seq = in.seq;
   if (q.counts) {
     int full = 0;
     for (int i = threadIdx.x; i < in.B; i += THREADS) full += q.rows[i] > 0;
     full = __reduce_add_sync(0xffffffffu, full);
     if (lane == 0) s_full[warp] = full;
+    if (seq && in.B < SEQ_MAX) {
+      for (int i = threadIdx.x; i <= in.B; i += THREADS) s_seq[i] = in.seq[i];
+      seq = s_seq;
+    }
     __syncthreads();
     full = 0;
     for (int k = 0; k < WARPS; ++k) full += s_full[k];
     scale = q.alpha * (q.dloss ? *q.dloss : 1.0f) * ((float)in.E / ((float)max(full, 1) * (float)in.K));
   }
   const float rs = q.dwts ? __bfloat162float(q.rs[0]) : 0.f;
-  const long long warps = (long long)gridDim.x * WARPS, w = (long long)blockIdx.x * WARPS + warp;
-  const int t0 = (int)(w * in.T / warps), t1 = (int)((w + 1) * in.T / warps);
-  int cur = -1;
-  float f[4 * NV];
-#pragma unroll
-  for (int i = 0; i < 4 * NV; ++i) f[i] = 0.f;
+  const int vec_counts = in.E % 4 == 0 && reinterpret_cast<uintptr_t>(q.counts) % 16 == 0;
   for (int t = t0; t < t1; ++t) {
     const float* row = in.S + t * in.lds;
+    int e = -1;
+    float es = 0.f, eg = 0.f, eslope = 0.f;  // the lane's pick: score, gradient of its weight, slope
+    if (q.dwts && lane < in.K) {
+      e = in.idx[(long long)t * in.K + lane];
+      if (e < 0 || e >= in.E) e = -1;
+      if (e >= 0) {
+        float u, r;
+        es = sigmoid_of(row[e], u, r);
+        eslope = u * r * r;
+        eg = q.dwts[(long long)t * in.K + lane];
+      }
+    }
     int b = -1;
     if (q.counts && !(in.mask && in.mask[t] == 0)) {
-      if (!in.seq) b = 0;
-      else if (t >= in.seq[0] && t < in.seq[in.B]) b = seq_of(in.seq, in.B, t);
+      if (!seq) b = 0;
+      else if (t >= seq[0] && t < seq[in.B]) b = seq_of(seq, in.B, t);
     }
-    float v[4 * NV];
-#pragma unroll
-    for (int i = 0; i < 4 * NV; ++i) v[i] = 0.f;
+    float d[N];
     if (b >= 0) {
-      load_row<NV>(row, in.E, in.vec, lane, v);
-      if (b != cur) {
-        cur = b;
-        const int n = q.rows[b];
-        const float k = n > 0 ? scale / (float)n / (float)n : 0.f;
-        const int* cb = q.counts + (long long)b * in.E;
+      const int n = q.rows[b];
+      const float k = n > 0 ? scale / (float)n / (float)n : 0.f;
+      const int* cb = q.counts + (long long)b * in.E;
+      float z = 0.f, m = 0.f, f[N];
 #pragma unroll
-        for (int i = 0; i < 4 * NV; ++i) {
-          const int e = ((i >> 2) * 32 + lane) * 4 + (i & 3);
-          f[i] = e < in.E ? k * (float)cb[e] : 0.f;
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * 32 + lane) * 4;
+        int4 g = make_int4(0, 0, 0, 0);
+        if (vec_counts) {
+          if (c < in.E) g = *reinterpret_cast<const int4*>(cb + c);
+        } else {
+          if (c < in.E) g.x = cb[c];
+          if (c + 1 < in.E) g.y = cb[c + 1];
+          if (c + 2 < in.E) g.z = cb[c + 2];
+          if (c + 3 < in.E) g.w = cb[c + 3];
         }
+        f[4 * j] = k * (float)g.x;
+        f[4 * j + 1] = k * (float)g.y;
+        f[4 * j + 2] = k * (float)g.z;
+        f[4 * j + 3] = k * (float)g.w;
       }
-      float z = 0.f, m = 0.f, slope[4 * NV];
 #pragma unroll
-      for (int i = 0; i < 4 * NV; ++i) {
+      for (int i = 0; i < N; ++i) {
         float u, r;
         const float s = sigmoid_of(v[i], u, r);
         z += s;
         m += f[i] * s;
-        slope[i] = u * r * r;
+        d[i] = u * r * r;
       }
+      load(t + 1);
       z = warp_sum(z) + TINY;
       m = warp_sum(m) / z;
       const float inv = __frcp_rn(z);
 #pragma unroll
-      for (int i = 0; i < 4 * NV; ++i) v[i] = (f[i] - m) * (slope[i] * inv);
+      for (int i = 0; i < N; ++i) d[i] = (f[i] - m) * (d[i] * inv);
+    } else {
+      load(t + 1);
+#pragma unroll
+      for (int i = 0; i < N; ++i) d[i] = 0.f;
     }
     if (q.dwts) {
-      int e = -1;
-      float s = 0.f, g = 0.f, slope = 0.f;
-      if (lane < in.K) {
-        e = in.idx[(long long)t * in.K + lane];
-        if (e < 0 || e >= in.E) e = -1;
-        if (e >= 0) {
-          float u, r;
-          s = sigmoid_of(row[e], u, r);
-          slope = u * r * r;
-          g = q.dwts[(long long)t * in.K + lane];
-        }
-      }
-      const float den = warp_sum(s) + TINY;
-      const float mean = warp_sum(g * s) / den;
-      const float mine = rs / den * (g - mean) * slope;
+      const float den = warp_sum(es) + TINY;
+      const float mean = warp_sum(eg * es) / den;
+      const float mine = rs / den * (eg - mean) * eslope;
       // an expert named twice gets both parts, added in pick order
       const u32 peers = __match_any_sync(0xffffffffu, e);
       if (__all_sync(0xffffffffu, e < 0 || (peers & (peers - 1)) == 0)) {
@@ -355,10 +405,10 @@ __global__ void __launch_bounds__(bal::THREADS) route_backward_kernel(RouterRows
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const float4 a = *reinterpret_cast<const float4*>(add + (j * 32 + lane) * 4);
-        v[4 * j] += a.x;
-        v[4 * j + 1] += a.y;
-        v[4 * j + 2] += a.z;
-        v[4 * j + 3] += a.w;
+        d[4 * j] += a.x;
+        d[4 * j + 1] += a.y;
+        d[4 * j + 2] += a.z;
+        d[4 * j + 3] += a.w;
       }
       __syncwarp();
       if (e >= 0) add[e] = 0.f;
@@ -368,23 +418,23 @@ __global__ void __launch_bounds__(bal::THREADS) route_backward_kernel(RouterRows
     for (int j = 0; j < NV; ++j) {
       const int c = (j * 32 + lane) * 4;
       if (q.bf16_out) {
-        bf16* d = reinterpret_cast<bf16*>(q.dS) + t * q.ldd + c;
+        bf16* o = reinterpret_cast<bf16*>(q.dS) + t * q.ldd + c;
         if (q.vec_out && c + 4 <= in.E) {
-          *reinterpret_cast<uint2*>(d) =
-              make_uint2(f2_to_bf16x2(v[4 * j], v[4 * j + 1]), f2_to_bf16x2(v[4 * j + 2], v[4 * j + 3]));
+          *reinterpret_cast<uint2*>(o) =
+              make_uint2(f2_to_bf16x2(d[4 * j], d[4 * j + 1]), f2_to_bf16x2(d[4 * j + 2], d[4 * j + 3]));
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (c + i < in.E) d[i] = __float2bfloat16_rn(v[4 * j + i]);
+            if (c + i < in.E) o[i] = __float2bfloat16_rn(d[4 * j + i]);
         }
       } else {
-        float* d = reinterpret_cast<float*>(q.dS) + t * q.ldd + c;
+        float* o = reinterpret_cast<float*>(q.dS) + t * q.ldd + c;
         if (q.vec_out && c + 4 <= in.E) {
-          *reinterpret_cast<float4*>(d) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          *reinterpret_cast<float4*>(o) = make_float4(d[4 * j], d[4 * j + 1], d[4 * j + 2], d[4 * j + 3]);
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (c + i < in.E) d[i] = v[4 * j + i];
+            if (c + i < in.E) o[i] = d[4 * j + i];
         }
       }
     }

@@ -234,9 +234,9 @@ LayerLayout layer_layout(int T, int H, int I, int E, int K, int shared) {
 
 namespace {
 
-// rows a block of the first pass takes: about two blocks an SM over the rows, a multiple of its 8 warps.  A function
-// of T alone, so that the scratch size is too.
-int balance_chunk(int T) { return std::max(8, (int)align_up((size_t)cdiv(T, 2 * 148), 8)); }
+// rows a block of the first pass takes: a block an SM over the rows, in eights.  A function of T alone, so that the
+// scratch size is too.
+int balance_chunk(int T) { return std::max(8, (int)align_up((size_t)cdiv(T, 148), 8)); }
 
 struct BalanceLayout {
   int chunk, blocks;
@@ -302,11 +302,12 @@ void by_experts(int E, F f) {
 
 namespace {
 
-template <int SRC, int LANES, int NV>
+template <int SRC, int LANES, int NV, int MINB>
 int launch_quant_int8(const QuantRows& p, cudaStream_t s) {
-  const long long blocks = cdiv(p.rows, 256 / LANES);
-  const int grid = (int)std::min<long long>(blocks, (long long)num_sms(current_device()) * 16);
-  quant_int8_kernel<SRC, LANES, NV><<<grid, 256, 0, s>>>(p);
+  const int threads = LANES > 32 ? LANES : 256;
+  const long long blocks = cdiv(p.rows, threads / LANES);
+  const int grid = (int)std::min<long long>(blocks, (long long)num_sms(current_device()) * MINB);
+  quant_int8_kernel<SRC, LANES, NV, MINB><<<grid, threads, 0, s>>>(p);
   return launch_status();
 }
 
@@ -314,13 +315,13 @@ int launch_quant_int8(const QuantRows& p, cudaStream_t s) {
 template <int SRC>
 int quant_int8(const QuantRows& p, cudaStream_t s) {
   if (p.rows == 0) return K3MOE_OK;
-  const int groups = (p.cols + 15) / 16;
-  if (groups <= 32) return launch_quant_int8<SRC, 32, 1>(p, s);
-  if (groups <= 64) return launch_quant_int8<SRC, 32, 2>(p, s);
-  if (groups <= 256) return launch_quant_int8<SRC, 256, 1>(p, s);
-  if (groups <= 512) return launch_quant_int8<SRC, 256, 2>(p, s);
-  if (groups <= 1024) return launch_quant_int8<SRC, 256, 4>(p, s);
-  return launch_quant_int8<SRC, 256, 0>(p, s);
+  if (p.cols <= 512) return launch_quant_int8<SRC, 32, 2, 5>(p, s);
+  if (p.cols <= 1024) return launch_quant_int8<SRC, 32, 4, 4>(p, s);
+  if (p.cols <= 2048) return launch_quant_int8<SRC, 128, 2, 10>(p, s);
+  if (p.cols <= 4096) return launch_quant_int8<SRC, 128, 4, SRC == I8_BF16 ? 10 : 7>(p, s);
+  if (p.cols <= 8192) return launch_quant_int8<SRC, 256, 4, SRC == I8_BF16 ? 5 : 3>(p, s);
+  if (p.cols <= 16384) return launch_quant_int8<SRC, 512, 4, SRC == I8_BF16 ? 2 : 1>(p, s);
+  return launch_quant_int8<SRC, 512, 0, 2>(p, s);
 }
 
 bool int8_rows_ok(const void* q, long long ldq, int cols) {
@@ -342,7 +343,7 @@ int encode_int8(CUtensorMap* m, const void* base, long long rows, int cols, long
 }
 
 int int8_launch(const int8_t* q, long long q_rows, long long ldq, const int8_t* w, long long w_rows, long long ldw,
-                int C, Int8Params& p, int grid, cudaStream_t s) {
+                int C, Int8Params& p, int dtype, int grid, cudaStream_t s) {
   CUtensorMap tw, tx;
   int rc = encode_int8(&tw, w, w_rows, C, ldw, i8::BM);
   if (rc) return rc;
@@ -354,21 +355,26 @@ int int8_launch(const int8_t* q, long long q_rows, long long ldq, const int8_t* 
   p.stages = std::min(i8::MAX_STAGES, i8::RING_BYTES / p.stage_bytes);
   p.tmem_cols = 32;
   while (p.tmem_cols < 2u * p.bn) p.tmem_cols *= 2;
-  if (!set_smem_once(int8_gemm_kernel, i8::SMEM_BYTES, 4)) return K3MOE_ELAUNCH;
+  const bool f32 = dtype == K3MOE_F32;
+  if (!(f32 ? set_smem_once(int8_gemm_kernel<float>, i8::SMEM_BYTES, 4)
+            : set_smem_once(int8_gemm_kernel<bf16>, i8::SMEM_BYTES, 5)))
+    return K3MOE_ELAUNCH;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(i8::THREADS);
   cfg.dynamicSmemBytes = i8::SMEM_BYTES;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  if (p.splits > 1) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)p.splits;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-  }
-  if (cudaLaunchKernelEx(&cfg, int8_gemm_kernel, tw, tx, p) != cudaSuccess) {
+  // the prologue overlaps the end of the kernel before (usually the quantiser)
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)p.splits;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.splits > 1 ? 2 : 1;
+  if ((f32 ? cudaLaunchKernelEx(&cfg, int8_gemm_kernel<float>, tw, tx, p)
+           : cudaLaunchKernelEx(&cfg, int8_gemm_kernel<bf16>, tw, tx, p)) != cudaSuccess) {
     cudaGetLastError();
     return K3MOE_ELAUNCH;
   }
@@ -579,10 +585,22 @@ int k3moe_balance_loss(const float* S, int lds, const int32_t* idx, int T, int E
   const RouterRows in = router_rows(S, lds, idx, T, E, K, seq, B, mask);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   by_experts(E, [&](auto nv) {
-    balance_rows_kernel<decltype(nv)::value><<<L.blocks, bal::THREADS, 0, s>>>(in, w, L.chunk);
+    balance_rows_kernel<decltype(nv)::value><<<L.blocks, 32 * bal::ROW_WARPS, 0, s>>>(in, w, L.chunk);
   });
   const long long blocks = (long long)B * cdiv(E, bal::COLS);
-  balance_join_kernel<<<(unsigned)blocks, bal::THREADS, 0, s>>>(in, w, L.chunk, alpha, counts, prob, rows, loss);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(bal::THREADS);
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, balance_join_kernel, in, w, L.chunk, alpha, counts, prob, rows, loss) != cudaSuccess) {
+    cudaGetLastError();
+    return K3MOE_ELAUNCH;
+  }
   return launch_status();
 }
 
@@ -606,7 +624,7 @@ int k3moe_route_backward(const float* S, int lds, const int32_t* idx, int T, int
   q.ldd = ldd;
   q.bf16_out = dtype == K3MOE_BF16;
   q.vec_out = ldd % 4 == 0 && reinterpret_cast<uintptr_t>(dS) % (q.bf16_out ? 8 : 16) == 0;
-  const int grid = (int)std::min<long long>(cdiv(T, bal::WARPS), (long long)num_sms(current_device()) * 4);
+  const int grid = (int)std::min<long long>(cdiv(T, bal::WARPS), (long long)num_sms(current_device()) * 2);
   by_experts(E, [&](auto nv) {
     route_backward_kernel<decltype(nv)::value>
         <<<grid, bal::THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(in, q);
@@ -696,7 +714,6 @@ int k3moe_gemm_int8(const int8_t* q, long long ldq, const float* sx, const int8_
   p.sw = sw;
   p.out = out;
   p.ldo = ldo;
-  p.f32_out = dtype == K3MOE_F32;
   p.T = T;
   p.N = N;
   p.err = err;
@@ -710,7 +727,7 @@ int k3moe_gemm_int8(const int8_t* q, long long ldq, const float* sx, const int8_
   p.splits = 1;
   while (p.splits < 8 && units * p.splits * 2 <= sms && cdiv(C, i8::BK) >= 8 * p.splits) p.splits *= 2;
   const int grid = p.splits > 1 ? (int)units * p.splits : (int)std::min<long long>(units, sms);
-  return int8_launch(q, T, ldq, w, N, ldw, C, p, grid, reinterpret_cast<cudaStream_t>(stream));
+  return int8_launch(q, T, ldq, w, N, ldw, C, p, dtype, grid, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int k3moe_grouped_gemm_int8(const int8_t* q_perm, long long ldq, const float* sx_perm, const int8_t* w, long long ldw,
@@ -728,7 +745,6 @@ int k3moe_grouped_gemm_int8(const int8_t* q_perm, long long ldq, const float* sx
   p.sw = sw;
   p.out = out;
   p.ldo = ldo;
-  p.f32_out = dtype == K3MOE_F32;
   p.N = N;
   p.err = err;
   p.bn = 128;
@@ -741,7 +757,7 @@ int k3moe_grouped_gemm_int8(const int8_t* q_perm, long long ldq, const float* sx
   p.max_ctas = max_ctas;
   p.cap_rows = cap_rows;
   const int grid = (int)std::min<long long>(max_ctas * cdiv(N, i8::BM), num_sms(current_device()));
-  return int8_launch(q_perm, cap_rows, ldq, w, (long long)n_experts * N, ldw, C, p, grid,
+  return int8_launch(q_perm, cap_rows, ldq, w, (long long)n_experts * N, ldw, C, p, dtype, grid,
                      reinterpret_cast<cudaStream_t>(stream));
 }
 

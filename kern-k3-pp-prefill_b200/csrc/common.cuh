@@ -191,6 +191,12 @@ __device__ __forceinline__ void prefetch_tmap(const void* tmap) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(tmap) : "memory");
 }
 
+// ---------------------------------------------------------------- programmatic dependent launch
+// Let the next kernel of the stream start its prologue once every block of this one has come here or ended ...
+__device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// ... and wait there until this one has ended and its writes are visible (at once in a kernel launched without it).
+__device__ __forceinline__ void grid_wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- cp.async (LDGSTS)
 // 16 bytes global -> shared, through L2 only; both addresses 16-byte aligned
 __device__ __forceinline__ void cp_async16(u32 dst, const void* src) {

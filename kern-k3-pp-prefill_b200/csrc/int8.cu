@@ -11,10 +11,12 @@ namespace k3 {
 
 // ============================================================ quantiser
 // amax = the row's largest magnitude, scale = amax / 127, q = round-half-even(127 x / amax): the rounding of the real
-// quotient, not of a float product.  y = x * (127 / amax) is within 2e-5 of it, which settles every element but those
-// within 1e-4 of a half; these compare 254 |x| with (2k + 1) amax, both exact in double.
+// quotient, not of a float product.  One FMA rounds x * inv, inv = fl(127 / amax), to an integer (1.5 * 2^23 + x inv);
+// inv's error moves the quotient by at most 127 * 2^-24 = 7.6e-6, so every element whose x * inv is further than 1e-5
+// from a half is settled, and the others compare 254 |x| with (2k + 1) amax, both exact in double.
 // A row with an infinity or a NaN has scale NaN and q = 0, so every result it enters is NaN; a zero row scale 0, q = 0.
-// HBM-bound: a row is read once and kept in registers between the maximum and the codes.
+// HBM-bound: a row is read once and kept in registers (bf16 as it came) between the maximum and the codes; what counts
+// beside the bytes is the instructions an element, about 6.
 enum { I8_BF16 = 0, I8_F32 = 1, I8_GATED = 2 };
 
 struct QuantRows {
@@ -37,80 +39,72 @@ struct QuantRows {
   long long cap_rows;  // output rows
 };
 
-// 16 consecutive elements of a row as f32, zero past `cols`
+// 8 consecutive elements of a row as they are kept: bf16 pairs, or f32
 template <int SRC>
-__device__ __forceinline__ void load16(const QuantRows& p, long long r, int c, float (&v)[16]) {
+struct Kept {
+  u32 w[SRC == I8_BF16 ? 4 : 8];
+  __device__ __forceinline__ float operator[](int i) const {
+    if (SRC == I8_BF16) return __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+    return __uint_as_float(w[SRC == I8_BF16 ? i >> 1 : i]);
+  }
+};
+
+// 8 bf16 from s (zero past `left`)
+__device__ __forceinline__ uint4 load_bf16x8(const bf16* s, int left, int vec) {
+  if (vec && left >= 8) return *reinterpret_cast<const uint4*>(s);
+  u32 h[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) h[i] = i < left ? (u32)__bfloat16_as_ushort(s[i]) : 0u;
+  return make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+}
+
+template <int SRC>
+__device__ __forceinline__ void load8(const QuantRows& p, long long r, int c, Kept<SRC>& v) {
+  const int left = p.cols - c;
   if (SRC == I8_F32) {
     const float* s = reinterpret_cast<const float*>(p.x) + r * p.ldx + c;
-    if (p.vec && c + 16 <= p.cols) {
+    if (p.vec && left >= 8) {
+      const uint4 a = reinterpret_cast<const uint4*>(s)[0], b = reinterpret_cast<const uint4*>(s)[1];
+      const u32 w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 f = reinterpret_cast<const float4*>(s)[i];
-        v[4 * i] = f.x;
-        v[4 * i + 1] = f.y;
-        v[4 * i + 2] = f.z;
-        v[4 * i + 3] = f.w;
-      }
+      for (int i = 0; i < 8; ++i) v.w[i % (SRC == I8_BF16 ? 4 : 8)] = w[i];
     } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = c + i < p.cols ? s[i] : 0.f;
+      for (int i = 0; i < 8; ++i) v.w[i % (SRC == I8_BF16 ? 4 : 8)] = i < left ? __float_as_uint(s[i]) : 0u;
     }
     return;
   }
   const bf16* s = reinterpret_cast<const bf16*>(p.x) + r * p.ldx + c;
-  if (p.vec && c + 16 <= p.cols) {
+  const uint4 a = load_bf16x8(s, left, p.vec);
+  if (SRC == I8_BF16) {
+    v.w[0] = a.x;
+    v.w[1] = a.y;
+    v.w[2] = a.z;
+    v.w[3] = a.w;
+    return;
+  }
+  const uint4 b = load_bf16x8(s + p.cols, left, p.vec);
+  const u32 g[4] = {a.x, a.y, a.z, a.w}, u[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint4 a = reinterpret_cast<const uint4*>(s)[i];
-      const u32 w[4] = {a.x, a.y, a.z, a.w};
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = bf16x2_to_f2(g[i]), y = bf16x2_to_f2(u[i]);
+    v.w[(2 * i) % (SRC == I8_BF16 ? 4 : 8)] = __float_as_uint(gated_act(x.x, y.x, p.act));
+    v.w[(2 * i + 1) % (SRC == I8_BF16 ? 4 : 8)] = __float_as_uint(gated_act(x.y, y.y, p.act));
+  }
+}
+
+// The running maximum of magnitudes as ordered bits (a NaN above an infinity above all numbers): bf16 pairs as two
+// 16-bit halves, f32 whole.
+template <int SRC>
+__device__ __forceinline__ u32 max_bits(u32 m, const Kept<SRC>& v) {
+  if (SRC == I8_BF16) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 f = bf16x2_to_f2(w[k]);
-        v[8 * i + 2 * k] = f.x;
-        v[8 * i + 2 * k + 1] = f.y;
-      }
-    }
+    for (int i = 0; i < 4; ++i) asm("max.s16x2 %0, %0, %1;" : "+r"(m) : "r"(v.w[i] & 0x7fff7fffu));
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = c + i < p.cols ? __bfloat162float(s[i]) : 0.f;
+    for (int i = 0; i < (SRC == I8_BF16 ? 4 : 8); ++i) m = max(m, v.w[i] & 0x7fffffffu);
   }
-  if (SRC == I8_GATED) {
-    const bf16* u = s + p.cols;
-    if (p.vec && c + 16 <= p.cols) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint4 a = reinterpret_cast<const uint4*>(u)[i];
-        const u32 w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float2 f = bf16x2_to_f2(w[k]);
-          v[8 * i + 2 * k] = gated_act(v[8 * i + 2 * k], f.x, p.act);
-          v[8 * i + 2 * k + 1] = gated_act(v[8 * i + 2 * k + 1], f.y, p.act);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (c + i < p.cols) v[i] = gated_act(v[i], __bfloat162float(u[i]), p.act);
-    }
-  }
-}
-
-// the code of an element whose quotient lies near a half: y its float quotient
-__device__ __noinline__ int code_near_half(float x, float y, float amax) {
-  const int k = (int)fabsf(y);
-  const double a = 254.0 * fabs((double)x), h = (double)(2 * k + 1) * (double)amax;
-  const int m = a > h || (a == h && (k & 1)) ? k + 1 : k;
-  return x < 0.f ? -m : m;
-}
-
-// bytes lo .. hi of four codes
-__device__ __forceinline__ u32 pack_s8(int a, int b, int c, int d) {
-  u32 r;
-  asm("{\n .reg .b32 t;\n cvt.pack.sat.s8.s32.b32 t, %4, %3, 0;\n cvt.pack.sat.s8.s32.b32 %0, %2, %1, t;\n}\n"
-      : "=r"(r)
-      : "r"(a), "r"(b), "r"(c), "r"(d));
-  return r;
+  return m;
 }
 
 struct RowScale {
@@ -132,94 +126,147 @@ __device__ __forceinline__ RowScale row_scale(u32 amax_bits) {
   return s;
 }
 
-__device__ __forceinline__ uint4 encode16(const RowScale& s, const float (&v)[16]) {
-  int k[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float y = (v[i] * s.pre) * s.inv, n = rintf(y);
-    k[i] = s.inv == 0.f ? 0 : (int)n;  // a non-finite row: 0
-    if (fabsf(fabsf(y - n) - 0.5f) < 1e-4f) k[i] = code_near_half(v[i], y, s.amax);
-  }
-  return make_uint4(pack_s8(k[0], k[1], k[2], k[3]), pack_s8(k[4], k[5], k[6], k[7]),
-                    pack_s8(k[8], k[9], k[10], k[11]), pack_s8(k[12], k[13], k[14], k[15]));
+// the code of an element whose quotient lies near k + 1/2 in magnitude
+__device__ __noinline__ int code_near_half(float x, int k, float amax) {
+  const double a = 254.0 * fabs((double)x), h = (double)(2 * k + 1) * (double)amax;
+  const int m = a > h || (a == h && (k & 1)) ? k + 1 : k;
+  return x < 0.f ? -m : m;
 }
-__device__ __forceinline__ void put16(int8_t* dst, int left, uint4 w) {
-  if (left >= 16) {
-    *reinterpret_cast<uint4*>(dst) = w;
-  } else {
-    const u32 b[4] = {w.x, w.y, w.z, w.w};
+
+template <int SRC>
+__device__ __forceinline__ uint2 encode8(const RowScale& s, const Kept<SRC>& v) {
+  constexpr float ROUND = 12582912.f;  // 1.5 * 2^23: the integer sits in the low bits
+  if (s.inv == 0.f) return make_uint2(0u, 0u);
+  float x[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (i < left) dst[i] = (int8_t)(b[i >> 2] >> (8 * (i & 3)));
+  for (int i = 0; i < 8; ++i) x[i] = v[i];
+  if (s.pre != 1.f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] *= s.pre;
+  }
+  u32 t[8];
+  float far = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float n = __fmaf_rn(x[i], s.inv, ROUND);
+    far = fmaxf(far, fabsf(__fmaf_rn(x[i], s.inv, -(n - ROUND))));
+    t[i] = __float_as_uint(n);
+  }
+  if (far > 0.5f - 1e-5f) {  // one group in a thousand
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      float xi = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) xi = k == i ? x[k] : xi;
+      const float n = __fmaf_rn(xi, s.inv, ROUND) - ROUND, d = __fmaf_rn(xi, s.inv, -n);
+      if (fabsf(d) > 0.5f - 1e-5f) {
+        // |quotient| = |n| + d (with n's sign): the integer below it
+        const int k0 = (int)fabsf(n) - (n != 0.f && (d < 0.f) == (n > 0.f) ? 1 : 0);
+        const int c = code_near_half(xi, k0, s.amax * s.pre);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[k] = k == i ? (u32)c : t[k];
+      }
+    }
+  }
+  const u32 a = __byte_perm(t[0], t[1], 0x0040), b = __byte_perm(t[2], t[3], 0x0040);
+  const u32 c = __byte_perm(t[4], t[5], 0x0040), d = __byte_perm(t[6], t[7], 0x0040);
+  return make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410));
+}
+__device__ __forceinline__ void put8(int8_t* dst, int left, uint2 w) {
+  if (left >= 8) {
+    *reinterpret_cast<uint2*>(dst) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) dst[i] = (int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3)));
   }
 }
 
-// LANES threads a row (a warp, or the block of 256), NV groups of 16 elements a thread kept in registers; NV = 0: rows
-// too long for that are read a second time (from L2).
-template <int SRC, int LANES, int NV>
-__global__ void __launch_bounds__(256) quant_int8_kernel(QuantRows p) {
-  __shared__ u32 s_max[2][8];
-  constexpr int PER = 256 / LANES;
+// LANES threads a row (a warp of a block of 256, or a block), NV groups of 8 elements a thread kept in registers;
+// NV = 0: rows too long for that are read a second time (from L2).  MINB blocks an SM: enough loads in flight.
+template <int SRC, int LANES, int NV, int MINB>
+__global__ void __launch_bounds__(LANES > 32 ? LANES : 256, MINB) quant_int8_kernel(QuantRows p) {
+  __shared__ u32 s_max[2][LANES > 32 ? LANES / 32 : 1];
+  constexpr int PER = LANES > 32 ? 1 : 8;
+  constexpr int STEP = LANES * 8;
   const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
-  const int step = LANES * 16;
-  const int nne = p.meta && p.cta_limit ? min(p.meta[0], p.max_ctas) : 0;
+  grid_launch_dependents();
+  const int nne = p.cta_limit ? min(p.meta[0], p.max_ctas) : 0;
+  const int shared_row = p.exp2perm ? p.meta[2] : -1;
   int buf = 0;
   for (long long r = (long long)blockIdx.x * PER + sub; r < p.rows; r += (long long)gridDim.x * PER) {
     if (p.cta_limit && ((r >> 7) >= nne || r >= p.cta_limit[r >> 7])) continue;  // the row's LANES threads together
+    // lane k of a warp holds the row's k-th target, loaded ahead of its elements
+    int target = -1;
+    if (p.exp2perm) {
+      const int k = lane & 31;
+      if (k < p.K) target = p.exp2perm[r * p.K + k];
+      else if (k == p.K && shared_row >= 0) target = shared_row + (int)r;
+    }
     u32 m = 0;
-    float v[NV > 0 ? NV : 1][16];
+    Kept<SRC> v[NV > 0 ? NV : 1];
     if (NV > 0) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int c = j * step + lane * 16;
+        const int c = j * STEP + lane * 8;
         if (c < p.cols) {
-          load16<SRC>(p, r, c, v[j]);
+          load8<SRC>(p, r, c, v[j]);
+        } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[j][i]) & 0x7fffffffu);
+          for (int i = 0; i < (SRC == I8_BF16 ? 4 : 8); ++i) v[j].w[i] = 0u;
         }
       }
-    } else {
-      for (int c = lane * 16; c < p.cols; c += step) {
-        load16<SRC>(p, r, c, v[0]);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[0][i]) & 0x7fffffffu);
+      for (int j = 0; j < NV; ++j) m = max_bits<SRC>(m, v[j]);
+    } else {
+      for (int c = lane * 8; c < p.cols; c += STEP) {
+        load8<SRC>(p, r, c, v[0]);
+        m = max_bits<SRC>(m, v[0]);
       }
     }
+    if (SRC == I8_BF16) m = max(m << 16, m & 0xffff0000u);
     m = __reduce_max_sync(0xffffffffu, m);
     if (LANES > 32) {
       if ((threadIdx.x & 31) == 0) s_max[buf][threadIdx.x >> 5] = m;
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m = max(m, s_max[buf][i]);
+      for (int i = 0; i < LANES / 32; ++i) m = max(m, s_max[buf][i]);
       buf ^= 1;  // the next row's maxima go to the other half: one barrier a row
     }
     const RowScale s = row_scale(m);
-    const int targets = p.exp2perm ? p.K + 1 : 1;
-    uint4 w[NV > 0 ? NV : 1];
     if (NV > 0) {
+      if (!p.exp2perm) {
+        int8_t* dst = p.q + r * p.ldq;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if (j * step + lane * 16 < p.cols) w[j] = encode16(s, v[j]);
-    }
-    for (int k = 0; k < targets; ++k) {
-      long long o = r;
-      if (p.exp2perm) {
-        if (k < p.K) o = p.exp2perm[r * p.K + k];
-        else o = p.meta[2] >= 0 ? p.meta[2] + r : -1;
+        for (int j = 0; j < NV; ++j) {
+          const int c = j * STEP + lane * 8;
+          if (c < p.cols) put8(dst + c, p.cols - c, encode8<SRC>(s, v[j]));
+        }
+        if (lane == 0) p.scale[r] = s.scale;
+        continue;
       }
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const uint2 w = encode8<SRC>(s, v[j]);  // past the row's end: zeros, kept and not stored
+        v[j].w[0] = w.x;
+        v[j].w[1] = w.y;
+      }
+    }
+    const int targets = p.exp2perm ? p.K + 1 : 1;
+    for (int k = 0; k < targets; ++k) {
+      const long long o = p.exp2perm ? (long long)__shfl_sync(0xffffffffu, target, k) : r;
       if (o < 0 || o >= p.cap_rows) continue;
       int8_t* dst = p.q + o * p.ldq;
       if (NV > 0) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          const int c = j * step + lane * 16;
-          if (c < p.cols) put16(dst + c, p.cols - c, w[j]);
+          const int c = j * STEP + lane * 8;
+          if (c < p.cols) put8(dst + c, p.cols - c, make_uint2(v[j].w[0], v[j].w[1]));
         }
       } else {
-        for (int c = lane * 16; c < p.cols; c += step) {
-          load16<SRC>(p, r, c, v[0]);
-          w[0] = encode16(s, v[0]);
-          put16(dst + c, p.cols - c, w[0]);
+        for (int c = lane * 8; c < p.cols; c += STEP) {
+          load8<SRC>(p, r, c, v[0]);
+          put8(dst + c, p.cols - c, encode8<SRC>(s, v[0]));
         }
       }
       if (lane == 0) p.scale[o] = s.scale;
@@ -243,8 +290,9 @@ constexpr int BK = 128;                  // K bytes a stage
 constexpr int W_BYTES = BM * BK;
 constexpr int RING_BYTES = 192 * 1024;
 constexpr int MAX_STAGES = 10;
-constexpr int SMEM_BYTES = RING_BYTES + 1024 + 512;
 constexpr int EPI_WARPS = 8;
+constexpr int BAR_BYTES = 256;
+constexpr int SMEM_BYTES = RING_BYTES + 1024 /*align*/ + BAR_BYTES + EPI_WARPS * 128 * 4 /*token scales*/;
 constexpr int WARPS = 2 + EPI_WARPS;
 constexpr int THREADS = 32 * WARPS;
 }  // namespace i8
@@ -252,9 +300,8 @@ constexpr int THREADS = 32 * WARPS;
 struct Int8Params {
   const float* sx;         // [T] (grouped: permuted rows)
   const float* sw;         // [experts * N]
-  void* out;               // [T, ldo] bf16 or f32
+  void* out;               // [T, ldo] of the kernel's OUT
   long long ldo;
-  int f32_out;
   int T;                   // token rows (dense)
   int N;                   // weight channels (an expert)
   int kstages;
@@ -331,11 +378,18 @@ __device__ __forceinline__ int4 ld_cluster_v4(u32 saddr, u32 rank) {
   return v;
 }
 
-__device__ __forceinline__ void int8_store(const Int8Params& p, long long row, int ch, float v) {
-  if (p.f32_out) reinterpret_cast<float*>(p.out)[row * p.ldo + ch] = v;
-  else reinterpret_cast<bf16*>(p.out)[row * p.ldo + ch] = __float2bfloat16_rn(v);
+template <typename OUT>
+__device__ __forceinline__ OUT int8_value(u32 acc, float sx, float sw);
+template <>
+__device__ __forceinline__ float int8_value<float>(u32 acc, float sx, float sw) {
+  return __int2float_rn((int)acc) * sx * sw;
+}
+template <>
+__device__ __forceinline__ bf16 int8_value<bf16>(u32 acc, float sx, float sw) {
+  return __float2bfloat16_rn(__int2float_rn((int)acc) * sx * sw);
 }
 
+template <typename OUT>
 __global__ void __launch_bounds__(i8::THREADS, 1)
     int8_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, Int8Params p) {
   using namespace i8;
@@ -349,6 +403,7 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
   u64* drain = bars + 2 * MAX_STAGES + 4;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * MAX_STAGES + 5);
   u32* tmem_slot = reinterpret_cast<u32*>(bars + 2 * MAX_STAGES + 6);
+  float* scales = reinterpret_cast<float*>(smem + RING_BYTES + BAR_BYTES);  // [EPI_WARPS][128]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 1) {
@@ -374,6 +429,7 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const u32 tmem_base = *tmem_slot;
+  grid_wait_previous();  // the rows (and whatever else an earlier kernel writes) are there from here on
   const int units = (p.cta_batch ? min(p.meta[0], p.max_ctas) : p.t_tiles) * p.n_tiles;
   // the block's part of K (all of it without a cluster)
   const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
@@ -419,12 +475,12 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
       // ------------------------------------------------ MMA issuer
       int stage = 0, buf = 0;
       u32 phase = 0;
-      u32 acc_phase[2] = {0u, 0u};
+      u32 acc_phase = 0;  // bit b: accumulator b's parity
       bool issued = false;
       for (int u = first; u < units && !*abort_flag; u += stride) {
         const Int8Unit w = int8_unit(p, u);
         if (!w.valid) continue;
-        if (!mbar_wait(&acc_empty[buf], acc_phase[buf] ^ 1u, abort_flag, p.err, 0xD30u)) break;
+        if (!mbar_wait(&acc_empty[buf], ((acc_phase >> buf) & 1u) ^ 1u, abort_flag, p.err, 0xD30u)) break;
         tc_fence_after();
         const u32 idesc = i8_idesc(BM, (w.n + 15) & ~15);
         const u32 d = tmem_base + (u32)(buf * p.bn);
@@ -449,7 +505,7 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
         }
         if (!ok) break;
         tc_commit(&acc_full[buf]);
-        acc_phase[buf] ^= 1u;
+        acc_phase ^= 1u << buf;
         buf ^= 1;
       }
       if (issued) {
@@ -459,40 +515,64 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
     }
   } else {
     // ------------------------------------------------ epilogue (warps 2..9): a lane is a channel, columns are tokens;
-    // the two warps of a sub-partition take 16 tokens in turn
-    const int sub = warp & 3;
+    // the two warps of a sub-partition take 16 tokens in turn, the next 16 on their way while these are scaled and
+    // stored (a token's 32 channels a warp store).  The tokens' scales come by broadcast from shared memory.
+    const int sub = warp & 3, half = (warp - 2) >> 2;
     const u32 lane_base = (u32)(sub * 32) << 16;
     int* red = reinterpret_cast<int*>(smem);
-    u32 acc_phase[2] = {0u, 0u};
+    float* sxs = scales + (warp - 2) * 128;  // this warp's tokens: 16 of every 32
+    const long long row_step = p.ldo;
+    u32 acc_phase = 0;
     int buf = 0;
     for (int u = first; u < units && !*abort_flag; u += stride) {
       const Int8Unit w = int8_unit(p, u);
       if (!w.valid) continue;
-      if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], acc_phase[buf], abort_flag, p.err, 0xD60u))) break;
-      tc_fence_after();
       const int ch = w.ch0 + sub * 32 + lane;
       const float swc = ch < p.N ? p.sw[(long long)w.e * p.N + ch] : 0.f;
-      for (int c = ((warp - 2) >> 2) * 16; c < w.n; c += 32) {
-        u32 v[16];
-        i8_ld16(tmem_base + lane_base + (u32)(buf * p.bn + c), v);
-        const float sx = lane < 16 && c + lane < w.n ? p.sx[w.row0 + c + lane] : 0.f;
+      for (int i = lane; i < 128; i += 32) {
+        const int t = (i >> 4) * 32 + half * 16 + (i & 15);
+        sxs[i] = t < w.n ? p.sx[w.row0 + t] : 0.f;
+      }
+      __syncwarp();
+      if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (acc_phase >> buf) & 1u, abort_flag, p.err, 0xD60u))) break;
+      tc_fence_after();
+      const u32 acc = tmem_base + lane_base + (u32)(buf * p.bn);
+      int c = half * 16;
+      u32 v[16];
+      if (c < w.n) i8_ld16(acc + (u32)c, v);
+      OUT* dst = reinterpret_cast<OUT*>(p.out) + ((long long)w.row0 + c) * row_step + ch;
+      const float* sx = sxs;
+      const bool whole = w.ch0 + BM <= p.N;
+#pragma unroll 1
+      for (; c < w.n; c += 32, dst += 32 * row_step, sx += 16) {
         tmem_wait_ld();
+        u32 x[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = v[j];
+        if (c + 32 < w.n) i8_ld16(acc + (u32)(c + 32), v);
         if (p.splits > 1) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) red[(c + j) * BM + sub * 32 + lane] = (int)v[j];
-        } else {
+          for (int j = 0; j < 16; ++j) red[(c + j) * BM + sub * 32 + lane] = (int)x[j];
+        } else if (whole && c + 16 <= w.n) {
+          OUT* d = dst;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float s = __shfl_sync(0xffffffffu, sx, j);
-            if (ch < p.N && c + j < w.n)
-              int8_store(p, (long long)w.row0 + c + j, ch, __int2float_rn((int)v[j]) * s * swc);
+          for (int j = 0; j < 16; j += 4) {
+            const float4 s = *reinterpret_cast<const float4*>(sx + j);
+            const float q[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i, d += row_step) *d = int8_value<OUT>(x[j + i], q[i], swc);
           }
+        } else {
+          OUT* d = dst;
+#pragma unroll
+          for (int j = 0; j < 16; ++j, d += row_step)
+            if (ch < p.N && c + j < w.n) *d = int8_value<OUT>(x[j], sx[j], swc);
         }
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&acc_empty[buf]);
-      acc_phase[buf] ^= 1u;
+      acc_phase ^= 1u << buf;
       buf ^= 1;
     }
   }
@@ -519,9 +599,10 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
       const int ch = w.ch0 + lane * 4;
       const float s = p.sx[w.row0 + t];
       const int q[4] = {a.x, a.y, a.z, a.w};
+      OUT* dst = reinterpret_cast<OUT*>(p.out) + ((long long)w.row0 + t) * p.ldo + ch;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (ch + i < p.N) int8_store(p, (long long)w.row0 + t, ch + i, __int2float_rn(q[i]) * s * p.sw[ch + i]);
+        if (ch + i < p.N) dst[i] = int8_value<OUT>((u32)q[i], s, p.sw[ch + i]);
     }
     cluster_sync();  // no block leaves while another reads its part
   }

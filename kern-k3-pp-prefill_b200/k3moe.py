@@ -342,48 +342,61 @@ def read_error(err: torch.Tensor, clear: bool = True, stream=None):
 
 
 # ------------------------------------------------------------------ argument checks of the entries below
+# A decode step calls these entries every few microseconds, so the checks that pass are a few attribute reads; what is
+# wrong with an argument is worked out only when one of them fails.
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise K3MoeError(what)
 
 
-def _rows(t, name: str, dtypes, cols: int | None = None, rows: int | None = None, dev=None) -> int:
-    """Check a matrix argument (device, dtype, shape, rows that are runs of elements, none shared); its row stride."""
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name}: a CUDA tensor is needed")
+def _rows(t, name: str, dtypes, dev=None, cols: int | None = None, rows: int | None = None) -> int:
+    """Check a matrix argument (dtype, device, shape, rows that are runs of elements, none shared); its row stride."""
+    try:
+        (n, c), (ld, one) = t.shape, t.stride()
+        if (one == 1 and ld >= c and t.dtype in dtypes and t.is_cuda and (dev is None or t.device == dev)
+                and (cols is None or c == cols) and (rows is None or n == rows)):
+            return ld
+    except (AttributeError, TypeError, ValueError):
+        raise K3MoeError(f"{name}: a matrix on a CUDA device is needed") from None
     _need(t.dtype in dtypes, f"{name}: dtype {t.dtype} (one of {dtypes} is needed)")
-    _need(t.dim() == 2 and (cols is None or t.shape[1] == cols) and (rows is None or t.shape[0] == rows),
-          f"{name}: shape {tuple(t.shape)} (rows {rows}, columns {cols} are needed)")
+    _need(t.is_cuda, f"{name}: a CUDA tensor is needed")
     _need(dev is None or t.device == dev, f"{name}: on {t.device}, the other tensors on {dev}")
-    n, c = t.shape
-    if n > 1:
-        _need((t.stride(1) == 1 or c == 1) and t.stride(0) >= c, f"{name}: strides {t.stride()} (contiguous rows are needed)")
-        return t.stride(0)
-    _need(t.stride(1) == 1 or c <= 1, f"{name}: strides {t.stride()} (contiguous rows are needed)")
-    return c
+    _need(cols in (None, c) and rows in (None, n), f"{name}: shape {(n, c)} ({rows} rows of {cols} are needed)")
+    # one row, or rows of one element, or none: their strides say nothing
+    _need((one == 1 or c <= 1) and (ld >= c or n <= 1), f"{name}: strides {(ld, one)} (contiguous rows are needed)")
+    return max(ld, c) if n > 1 else c
 
 
 def _vec(t, name: str, dtypes, n: int | None, dev) -> None:
     """Check a contiguous array argument of n elements (None: any number)."""
-    _need(isinstance(t, torch.Tensor) and t.device == dev and t.dtype in dtypes and t.is_contiguous()
-          and (n is None or t.numel() == n), f"{name}: a contiguous tensor of {n} elements of {dtypes} on {dev} is needed")
+    try:
+        if t.dtype in dtypes and t.device == dev and t.is_contiguous() and (n is None or t.numel() == n):
+            return
+    except AttributeError:
+        pass
+    raise K3MoeError(f"{name}: a contiguous tensor of {n} elements of {dtypes} on {dev} is needed")
 
 
 def _int8_rows(t, name: str, dev=None, cols: int | None = None, rows: int | None = None) -> int:
     """_rows of an int8 operand: 16-byte aligned, row stride a multiple of 16 (of one row: rounded up)."""
-    ld = _rows(t, name, (torch.int8,), cols, rows, dev)
-    if t.shape[0] <= 1:
-        ld = -(-max(t.shape[1], 1) // 16) * 16
-    _need(ld % 16 == 0 and t.data_ptr() % 16 == 0, f"{name}: 16-byte aligned rows are needed (quant_int8 pads them)")
+    ld = _rows(t, name, _I8, dev, cols, rows)
+    if ld % 16 and t.shape[0] <= 1:
+        ld = -(-ld // 16) * 16
+    if ld % 16 or t.data_ptr() % 16:
+        raise K3MoeError(f"{name}: 16-byte aligned rows are needed (quant_int8 pads them)")
     return ld
 
 
 def _launch(fn, what: str, dev, *args) -> None:
     """Call an entry on `dev`'s current stream, with `dev` the current device."""
-    if dev.index == torch.cuda.current_device():
-        _check(fn(*args, torch.cuda.current_stream().cuda_stream), what)
+    i = dev.index
+    if i == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(dev):
-            _check(fn(*args, torch.cuda.current_stream().cuda_stream), what)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        _check(rc, what)
 
 
 def _on_stream(f):
@@ -398,10 +411,15 @@ def _on_stream(f):
 
 
 def _out_dtype(dtype) -> int:
-    _need(dtype in (torch.bfloat16, torch.float32), f"dtype {dtype} (torch.bfloat16 or torch.float32 is needed)")
-    return F32 if dtype == torch.float32 else BF16
+    if dtype is torch.bfloat16:
+        return BF16
+    if dtype is torch.float32:
+        return F32
+    raise K3MoeError(f"dtype {dtype} (torch.bfloat16 or torch.float32 is needed)")
 
 
+_I8, _I32, _F32, _BF16 = (torch.int8,), (torch.int32,), (torch.float32,), (torch.bfloat16,)
+_FLOATS, _FLAGS, _WORDS = (torch.bfloat16, torch.float32), (torch.uint8, torch.bool), (torch.int32, torch.uint32)
 BF16, F32 = 0, 1  # include/k3moe.h K3MOE_BF16, K3MOE_F32
 
 
@@ -415,18 +433,20 @@ class BalanceStats:
 
 
 def _router_args(S, idx, seq, mask):
-    ld = _rows(S, "S", (torch.float32,))
+    ld = _rows(S, "S", _F32)
     dev, (T, E) = S.device, S.shape
-    _need(idx.dim() == 2 and idx.shape[0] == T, f"idx: shape {tuple(idx.shape)} ([{T}, K] is needed)")
-    _vec(idx, "idx", (torch.int32,), None, dev)
+    _vec(idx, "idx", _I32, None, dev)
+    if idx.dim() != 2 or idx.shape[0] != T:
+        raise K3MoeError(f"idx: shape {tuple(idx.shape)} ([{T}, K] is needed)")
     B = 1
     if seq is not None:
-        _vec(seq, "seq", (torch.int32,), None, dev)
+        _vec(seq, "seq", _I32, None, dev)
         B = seq.numel() - 1
-        _need(seq.dim() == 1 and B >= 1, "seq: int32 offsets [B + 1] are needed")
+        if B < 1:
+            raise K3MoeError("seq: int32 offsets [B + 1] are needed")
     if mask is not None:
-        _vec(mask, "mask", (torch.uint8, torch.bool), T, dev)
-    return dev, T, E, idx.shape[1], B, max(ld, E)
+        _vec(mask, "mask", _FLAGS, T, dev)
+    return dev, T, E, idx.shape[1], B, ld
 
 
 @_on_stream
@@ -438,14 +458,14 @@ def balance_loss(S: torch.Tensor, idx: torch.Tensor, alpha: float, seq: torch.Te
     one sequence); mask [T] uint8 or bool, rows with 0 are not counted."""
     dev, T, E, K, B, ld = _router_args(S, idx, seq, mask)
     L = lib()
-    scratch = torch.empty(max(L.k3moe_balance_scratch_bytes(T, E, B), 16), dtype=torch.uint8, device=dev)
-    s = BalanceStats(loss=torch.empty(1, dtype=torch.float32, device=dev),
-                     counts=torch.empty((B, E), dtype=torch.int32, device=dev),
-                     prob=torch.empty((B, E), dtype=torch.float32, device=dev),
-                     rows=torch.empty(B, dtype=torch.int32, device=dev))
-    _launch(L.k3moe_balance_loss, "balance_loss", dev, _p(S), ld, _p(idx), T, E, K, _p(seq), B, _p(mask), alpha,
-            _p(scratch), _p(s.counts), _p(s.prob), _p(s.rows), _p(s.loss))
-    return s
+    scratch = S.new_empty(-(-L.k3moe_balance_scratch_bytes(T, E, B) // 4))
+    prob = S.new_empty((B, E))
+    counts = idx.new_empty((B, E))
+    rows = idx.new_empty(B)
+    loss = S.new_empty(1)
+    _launch(L.k3moe_balance_loss, "balance_loss", dev, S.data_ptr(), ld, idx.data_ptr(), T, E, K, _p(seq), B, _p(mask),
+            alpha, scratch.data_ptr(), counts.data_ptr(), prob.data_ptr(), rows.data_ptr(), loss.data_ptr())
+    return BalanceStats(loss, counts, prob, rows)
 
 
 @_on_stream
@@ -458,34 +478,36 @@ def route_backward(S: torch.Tensor, idx: torch.Tensor, alpha: float = 0.0, count
     and mask) are given, dloss its scalar gradient (None: 1); plus the weight term where dwts [T, K], the gradient of
     route_topk's weights, and rs are given."""
     dev, T, E, K, B, ld = _router_args(S, idx, seq, mask)
-    _need((counts is None) == (rows is None), "counts and rows are given together")
-    _need((dwts is None) or (rs is not None), "dwts needs rs")
-    _need(counts is not None or dwts is not None, "counts and rows, or dwts and rs, are needed")
-    if counts is not None:
-        _vec(counts, "counts", (torch.int32,), B * E, dev)
-        _vec(rows, "rows", (torch.int32,), B, dev)
+    if counts is not None and rows is not None:
+        _vec(counts, "counts", _I32, B * E, dev)
+        _vec(rows, "rows", _I32, B, dev)
+    else:
+        _need(counts is None and rows is None, "counts and rows are given together")
+        _need(dwts is not None, "counts and rows, or dwts and rs, are needed")
     if dloss is not None:
-        _vec(dloss, "dloss", (torch.float32,), 1, dev)
+        _vec(dloss, "dloss", _F32, 1, dev)
     if dwts is not None:
-        _vec(dwts, "dwts", (torch.float32,), T * K, dev)
-        _vec(rs, "rs", (torch.bfloat16,), 1, dev)
+        _vec(dwts, "dwts", _F32, T * K, dev)
+        _vec(rs, "rs", _BF16, 1, dev)
     if out is None:
-        out = torch.empty((T, E), dtype=dtype, device=dev)
-    code = _out_dtype(out.dtype)
-    ldd = max(_rows(out, "out", (out.dtype,), E, T, dev), E)
-    _launch(lib().k3moe_route_backward, "route_backward", dev, _p(S), ld, _p(idx), T, E, K, _p(seq), B, _p(mask),
-            alpha, _p(counts), _p(rows), _p(dloss), _p(dwts), _p(rs), _p(out), ldd, code)
+        code, ldd = _out_dtype(dtype), E
+        out = S.new_empty((T, E), dtype=dtype)
+    else:
+        code, ldd = _out_dtype(out.dtype), _rows(out, "out", _FLOATS, dev, E, T)
+    _launch(lib().k3moe_route_backward, "route_backward", dev, S.data_ptr(), ld, idx.data_ptr(), T, E, K, _p(seq), B,
+            _p(mask), alpha, _p(counts), _p(rows), _p(dloss), _p(dwts), _p(rs), out.data_ptr(), ldd, code)
     return out
 
 
 # ------------------------------------------------------------------ products in 8-bit integers
-def _int8_out(rows: int, cols: int, dev, out):
+def _int8_out(x, rows: int, cols: int, dev, out):
     if out is None:
-        q = torch.empty((rows, -(-cols // 16) * 16), dtype=torch.int8, device=dev)[:, :cols]
-        return q, q.stride(0), torch.empty(rows, dtype=torch.float32, device=dev)
+        ld = -(-cols // 16) * 16
+        q = x.new_empty((rows, ld), dtype=torch.int8)
+        return q if ld == cols else q[:, :cols], ld, x.new_empty(rows, dtype=torch.float32)
     q, scale = out
     ld = _int8_rows(q, "out q", dev, cols, rows)
-    _vec(scale, "out scale", (torch.float32,), rows, dev)
+    _vec(scale, "out scale", _F32, rows, dev)
     return q, ld, scale
 
 
@@ -493,11 +515,12 @@ def _int8_out(rows: int, cols: int, dev, out):
 def quant_int8(x: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None):
     """Rows of x (bf16 or f32 [rows, cols]; tokens, or a weight's channels) to int8 with a scale each
     (k3moe_quant_int8): (q int8 [rows, cols], its rows padded to 16 bytes; scale f32 [rows])."""
-    ldx = _rows(x, "x", (torch.bfloat16, torch.float32))
+    ldx = _rows(x, "x", _FLOATS)
     rows, cols = x.shape
-    q, ldq, scale = _int8_out(rows, cols, x.device, out)
-    _launch(lib().k3moe_quant_int8, "quant_int8", x.device, _p(x), F32 if x.dtype == torch.float32 else BF16,
-            max(ldx, cols), rows, cols, _p(q), ldq, _p(scale))
+    dev = x.device
+    q, ldq, scale = _int8_out(x, rows, cols, dev, out)
+    _launch(lib().k3moe_quant_int8, "quant_int8", dev, x.data_ptr(), _out_dtype(x.dtype), ldx, rows, cols, q.data_ptr(),
+            ldq, scale.data_ptr())
     return q, scale
 
 
@@ -506,19 +529,21 @@ def act_quant_int8(gu: torch.Tensor, activation: int = ACT_SWIGLU, tables: Table
                    out: tuple[torch.Tensor, torch.Tensor] | None = None):
     """act(gate) * up of bf16 rows [gate | up] to int8 (k3moe_act_quant_int8): (q [rows, cols / 2], scale).  With
     tables, gu is [cap_rows, 2I] and only the tables' real rows are read and written."""
-    ldg = _rows(gu, "gu", (torch.bfloat16,))
+    ldg = _rows(gu, "gu", _BF16)
     rows, cols = gu.shape
-    _need(cols >= 2 and cols % 2 == 0, f"gu: {cols} columns (gate and up halves are needed)")
+    dev = gu.device
+    if cols % 2:
+        raise K3MoeError(f"gu: {cols} columns (gate and up halves are needed)")
     limit = meta = None
     ctas = 0
     if tables is not None:
-        _need(rows <= tables.max_ctas * 128, f"gu: {rows} rows, the tables cover {tables.max_ctas * 128}")
         limit, meta, ctas = tables.cta_limit, tables.meta, tables.max_ctas
-        _vec(limit, "tables.cta_limit", (torch.int32,), ctas, gu.device)
-        _vec(meta, "tables.meta", (torch.int32,), None, gu.device)
-    q, ldq, scale = _int8_out(rows, cols // 2, gu.device, out)
-    _launch(lib().k3moe_act_quant_int8, "act_quant_int8", gu.device, _p(gu), max(ldg, cols), rows, cols // 2,
-            activation, _p(limit), _p(meta), ctas, _p(q), ldq, _p(scale))
+        _need(rows <= ctas * 128, f"gu: {rows} rows, the tables cover {ctas * 128}")
+        _vec(limit, "tables.cta_limit", _I32, ctas, dev)
+        _vec(meta, "tables.meta", _I32, None, dev)
+    q, ldq, scale = _int8_out(gu, rows, cols // 2, dev, out)
+    _launch(lib().k3moe_act_quant_int8, "act_quant_int8", dev, gu.data_ptr(), ldg, rows, cols // 2, activation,
+            _p(limit), _p(meta), ctas, q.data_ptr(), ldq, scale.data_ptr())
     return q, scale
 
 
@@ -526,27 +551,35 @@ def act_quant_int8(gu: torch.Tensor, activation: int = ACT_SWIGLU, tables: Table
 def quant_int8_permute(x: torch.Tensor, tables: Tables, out: tuple[torch.Tensor, torch.Tensor] | None = None):
     """quant_int8 of bf16 rows, each written to every permuted row it is routed to (k3moe_quant_int8_permute):
     (q [cap_rows, cols], scale [cap_rows]); padding rows are not written."""
-    ldx = _rows(x, "x", (torch.bfloat16,))
+    ldx = _rows(x, "x", _BF16)
     R, cols = x.shape
-    K = tables.exp2perm.shape[1]
-    _vec(tables.exp2perm, "tables.exp2perm", (torch.int32,), R * K, x.device)
-    _vec(tables.meta, "tables.meta", (torch.int32,), None, x.device)
-    q, ldq, scale = _int8_out(tables.cap_rows, cols, x.device, out)
-    _launch(lib().k3moe_quant_int8_permute, "quant_int8_permute", x.device, _p(x), max(ldx, cols), R, cols, K,
-            _p(tables.exp2perm), _p(tables.meta), _p(q), ldq, _p(scale), tables.cap_rows)
+    dev, e2p, cap = x.device, tables.exp2perm, tables.cap_rows
+    K = e2p.shape[1]
+    _vec(e2p, "tables.exp2perm", _I32, R * K, dev)
+    _vec(tables.meta, "tables.meta", _I32, None, dev)
+    q, ldq, scale = _int8_out(x, cap, cols, dev, out)
+    _launch(lib().k3moe_quant_int8_permute, "quant_int8_permute", dev, x.data_ptr(), ldx, R, cols, K, e2p.data_ptr(),
+            tables.meta.data_ptr(), q.data_ptr(), ldq, scale.data_ptr(), cap)
     return q, scale
 
 
-def _product_args(q, sx, w, sw, dtype, out, err):
+def _product_args(q, sx, w, sw, err):
     ldq = _int8_rows(q, "q")
     dev, (T, C) = q.device, q.shape
     ldw = _int8_rows(w, "w", dev, C)
-    _vec(sx, "sx", (torch.float32,), T, dev)
-    _vec(sw, "sw", (torch.float32,), w.shape[0], dev)
+    _vec(sx, "sx", _F32, T, dev)
+    _vec(sw, "sw", _F32, w.shape[0], dev)
     if err is not None:
-        _vec(err, "err", (torch.int32, torch.uint32), None, dev)
+        _vec(err, "err", _WORDS, None, dev)
         _need(err.numel() >= 2, "err: two words are needed")
     return dev, T, C, ldq, ldw
+
+
+def _product_out(sx, T, N, dtype, dev, out):
+    if out is None:
+        code = _out_dtype(dtype)
+        return sx.new_empty((T, N), dtype=dtype), N, code
+    return out, _rows(out, "out", _FLOATS, dev, N, T), _out_dtype(out.dtype)
 
 
 @_on_stream
@@ -555,14 +588,11 @@ def gemm_int8(q: torch.Tensor, sx: torch.Tensor, w: torch.Tensor, sw: torch.Tens
               err: torch.Tensor | None = None) -> torch.Tensor:
     """out[t, n] = sx[t] sw[n] (q[t] . w[n]) (k3moe_gemm_int8): q int8 [T, C], w int8 [N, C], rows 16-byte aligned as
     quant_int8 gives them; out [T, N] bf16 or f32.  err: the device error words, or None."""
-    dev, T, C, ldq, ldw = _product_args(q, sx, w, sw, dtype, out, err)
+    dev, T, C, ldq, ldw = _product_args(q, sx, w, sw, err)
     N = w.shape[0]
-    if out is None:
-        out = torch.empty((T, N), dtype=dtype, device=dev)
-    code = _out_dtype(out.dtype)
-    ldo = max(_rows(out, "out", (out.dtype,), N, T, dev), N)
-    _launch(lib().k3moe_gemm_int8, "gemm_int8", dev, _p(q), ldq, _p(sx), _p(w), ldw, _p(sw), T, N, C, _p(out), ldo,
-            code, _p(err))
+    out, ldo, code = _product_out(sx, T, N, dtype, dev, out)
+    _launch(lib().k3moe_gemm_int8, "gemm_int8", dev, q.data_ptr(), ldq, sx.data_ptr(), w.data_ptr(), ldw, sw.data_ptr(),
+            T, N, C, out.data_ptr(), ldo, code, _p(err))
     return out
 
 
@@ -572,20 +602,18 @@ def grouped_gemm_int8(q: torch.Tensor, sx: torch.Tensor, w: torch.Tensor, sw: to
                       err: torch.Tensor | None = None) -> torch.Tensor:
     """The products of routed rows with their experts' weights (k3moe_grouped_gemm_int8): q int8 [cap_rows, C] permuted
     rows, w int8 [n_experts * N, C], out [cap_rows, N]; padding rows of out are not written."""
-    dev, cap, C, ldq, ldw = _product_args(q, sx, w, sw, dtype, out, err)
-    _need(n_experts >= 1 and w.shape[0] % n_experts == 0, f"w: {w.shape[0]} rows are not {n_experts} experts'")
-    _need(cap == tables.cap_rows, f"q: {cap} rows, the tables' capacity is {tables.cap_rows}")
-    _vec(tables.cta_batch, "tables.cta_batch", (torch.int32,), tables.max_ctas, dev)
-    _vec(tables.cta_limit, "tables.cta_limit", (torch.int32,), tables.max_ctas, dev)
-    _vec(tables.meta, "tables.meta", (torch.int32,), None, dev)
+    dev, cap, C, ldq, ldw = _product_args(q, sx, w, sw, err)
+    ctas = tables.max_ctas
+    if n_experts < 1 or w.shape[0] % n_experts or cap != tables.cap_rows:
+        raise K3MoeError(f"q of {cap} rows (capacity {tables.cap_rows}), w of {w.shape[0]} rows for {n_experts} experts")
+    _vec(tables.cta_batch, "tables.cta_batch", _I32, ctas, dev)
+    _vec(tables.cta_limit, "tables.cta_limit", _I32, ctas, dev)
+    _vec(tables.meta, "tables.meta", _I32, None, dev)
     N = w.shape[0] // n_experts
-    if out is None:
-        out = torch.empty((cap, N), dtype=dtype, device=dev)
-    code = _out_dtype(out.dtype)
-    ldo = max(_rows(out, "out", (out.dtype,), N, cap, dev), N)
-    _launch(lib().k3moe_grouped_gemm_int8, "grouped_gemm_int8", dev, _p(q), ldq, _p(sx), _p(w), ldw, _p(sw),
-            _p(tables.cta_batch), _p(tables.cta_limit), _p(tables.meta), N, C, n_experts, cap, tables.max_ctas,
-            _p(out), ldo, code, _p(err))
+    out, ldo, code = _product_out(sx, cap, N, dtype, dev, out)
+    _launch(lib().k3moe_grouped_gemm_int8, "grouped_gemm_int8", dev, q.data_ptr(), ldq, sx.data_ptr(), w.data_ptr(), ldw,
+            sw.data_ptr(), tables.cta_batch.data_ptr(), tables.cta_limit.data_ptr(), tables.meta.data_ptr(), N, C,
+            n_experts, cap, ctas, out.data_ptr(), ldo, code, _p(err))
     return out
 
 

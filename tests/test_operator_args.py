@@ -36,7 +36,7 @@ def test_balance_loss_refusals(lib):
 def test_balance_scratch_covers_every_block_and_sequence(lib):
     # (blocks + B) partial rows of E f32 and E int32
     for T, E, B in ((0, 1, 1), (1, 896, 1), (8192, 896, 16), (65536, 1024, 4096), (2 ** 31 - 1, 8, 3)):
-        chunk = max(8, -(--(-T // 296) // 8) * 8)
+        chunk = max(8, -(--(-T // 148) // 8) * 8)
         blocks = max(1, -(-T // chunk))
         need = (blocks + B) * E * 8 + (blocks + B) * 4 + B * -(-E // 32) * 4 + 4
         got = lib.k3moe_balance_scratch_bytes(T, E, B)
