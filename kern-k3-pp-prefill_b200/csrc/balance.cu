@@ -11,8 +11,8 @@
 // No counterpart in the reference: it serves only.
 //
 // Both passes read S once.  Sums run in f32 in a fixed order (no floating-point atomics), so equal inputs give equal
-// bytes.  exp(-|S|) is __expf: its error grows with |S|, to 1.5e-6 at |S| = 10, where the score itself is below 5e-5
-// or its slope is.
+// bytes.  A score is 1 / (1 + 2^(-S log2 e)) by the approximate exponential and reciprocal: its relative error grows
+// with |S|, to 1.5e-6 at S = -10, where the score itself is below 5e-5.
 #pragma once
 #include "common.cuh"
 
@@ -22,7 +22,6 @@ namespace bal {
 constexpr int WARPS = 8;         // of a block of the join and of the gradient
 constexpr int THREADS = 32 * WARPS;
 constexpr int ROW_WARPS = 16;    // of a block of the first pass
-constexpr int SEQ_MAX = 1024;    // offsets kept in shared memory
 constexpr float TINY = 1e-20f;  // the top-k's guard of its own sum
 constexpr int COLS = 32;        // experts a block of the second pass
 }  // namespace bal
@@ -38,7 +37,13 @@ struct RouterRows {
 };
 
 // the sequence holding row r: the last b with seq[b] <= r (the caller has checked seq[0] <= r)
-__device__ __forceinline__ int seq_of(const int* __restrict__ seq, int B, int r) {
+__device__ __forceinline__ int seq_of(const int* __restrict__ seq, int B, int r, int lane) {
+  if (B <= 128) {  // in one load latency: the offsets up to r, counted by the warp
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) n += i * 32 + lane < B && seq[i * 32 + lane] <= r;
+    return max((int)__reduce_add_sync(0xffffffffu, n) - 1, 0);
+  }
   int lo = 0, hi = B - 1;
   while (lo < hi) {
     const int m = (lo + hi + 1) >> 1;
@@ -67,11 +72,13 @@ __device__ __forceinline__ void load_row(const float* __restrict__ row, int E, i
   }
 }
 
-// t = exp(-|x|), r = 1 / (1 + t): sigmoid(x) is r or t r, and its slope t r^2 at either sign, without cancellation
-__device__ __forceinline__ float sigmoid_of(float x, float& t, float& r) {
-  t = __expf(-fabsf(x));
-  r = __fdividef(1.0f, 1.0f + t);
-  return x >= 0.f ? r : t * r;  // a NaN x: t is NaN
+// e = exp(-x): the score is 1 / (1 + e) and its slope e / (1 + e)^2, without cancellation at either end
+__device__ __forceinline__ float score_of(float x, float& e) {
+  e = ex2_ftz(x * -LOG2E);
+  return rcp_ftz(1.0f + e);
+}
+__device__ __forceinline__ float slope_of(float score, float e) {
+  return fminf(e, 3.402823466e38f) * score * score;  // score 0 (x = -inf): 0, not inf * 0
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -104,6 +111,14 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS) balance_rows_kernel(Route
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r0 = blockIdx.x * chunk, r1 = min(in.T, r0 + chunk);
   if (blockIdx.x == 0 && threadIdx.x == 0) *w.done = 0u;
+  float v[N];
+  int pick = -1, held = r0 + warp;  // v, pick: row `held`'s logits and pick, on their way
+  auto load = [&](int t) {
+    held = t;
+    load_row<NV>(in.S + t * in.lds, in.E, in.vec, lane, v);
+    if (lane < in.K) pick = in.idx[(long long)t * in.K + lane];
+  };
+  if (held < r1) load(held);
   int r = r0, last = r1;
   if (in.seq) {
     r = max(r0, in.seq[0]);
@@ -117,17 +132,14 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS) balance_rows_kernel(Route
   while (r < last) {
     int b = 0, end = last;
     if (in.seq) {
-      b = seq_of(in.seq, in.B, r);
+      b = seq_of(in.seq, in.B, r, lane);
       end = min(last, in.seq[b + 1]);
       if (end <= r) break;  // offsets that go down: nothing more is counted
     }
-    float acc[N], v[N];
-    int pick = -1, n = 0;
+    float acc[N];
+    int n = 0;
     int t = counted(r + warp, end);
-    if (t < end) {
-      load_row<NV>(in.S + t * in.lds, in.E, in.vec, lane, v);
-      if (lane < in.K) pick = in.idx[(long long)t * in.K + lane];
-    }
+    if (t < end && t != held) load(t);
     for (int e = threadIdx.x; e < in.E; e += 32 * ROW_WARPS) s_hist[e] = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = 0.f;
@@ -137,16 +149,13 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS) balance_rows_kernel(Route
       float z = 0.f, s[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        float u, q;
-        s[i] = sigmoid_of(v[i], u, q);
+        float u;
+        s[i] = score_of(v[i], u);
         z += s[i];
       }
       if (lane < in.K && pick >= 0 && pick < in.E) atomicAdd(&s_hist[pick], 1);
       t = counted(t + ROW_WARPS, end);
-      if (t < end) {
-        load_row<NV>(in.S + t * in.lds, in.E, in.vec, lane, v);
-        if (lane < in.K) pick = in.idx[(long long)t * in.K + lane];
-      }
+      if (t < end) load(t);
       const float inv = __frcp_rn(warp_sum(z) + TINY);
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[i] += s[i] * inv;
@@ -197,7 +206,6 @@ __global__ void __launch_bounds__(bal::THREADS)
   __shared__ float s_p[WARPS][COLS];
   __shared__ int s_c[WARPS][COLS], s_n[WARPS];
   __shared__ int s_last;
-  grid_wait_previous();  // the first pass's partial rows
   const int groups = (in.E + COLS - 1) / COLS;
   const int b = blockIdx.x / groups, g = blockIdx.x % groups;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -208,6 +216,7 @@ __global__ void __launch_bounds__(bal::THREADS)
     s0 = max(lo, in.seq[b]);
     s1 = min(hi, in.seq[b + 1]);
   }
+  grid_wait_previous();  // the first pass's partial rows
   float p = 0.f;
   int c = 0, n = 0;
   if (s0 < s1) {
@@ -283,49 +292,60 @@ struct RouteBackward {
   int vec_out;          // rows may be stored 4 elements at a time
 };
 
-// A warp takes consecutive rows, with the next row's logits on their way while one is computed; the counts, which
-// neighbouring rows share, come from L1.  The weight term touches K experts of a row: it is spread through a row of
-// shared memory that is all zero between rows.
+// A warp takes consecutive rows, with the next row's logits on their way while one is computed.  The coefficients f of
+// the sequence that the block's first row is in lie in shared memory; a block's few rows seldom leave it, and those that
+// do read their counts.  The weight term touches K experts of a row: it is spread through a row of shared memory that is
+// all zero between rows.
 template <int NV>
 __global__ void __launch_bounds__(bal::THREADS, 2) route_backward_kernel(RouterRows in, RouteBackward q) {
   using namespace bal;
   constexpr int N = 4 * NV;
+  __shared__ float s_f[128 * NV];
   __shared__ float s_add[WARPS][128 * NV];
   __shared__ int s_full[WARPS];
-  __shared__ int s_seq[SEQ_MAX];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float* add = s_add[warp];
   const long long warps = (long long)gridDim.x * WARPS, w = (long long)blockIdx.x * WARPS + warp;
   const int t0 = (int)(w * in.T / warps), t1 = (int)((w + 1) * in.T / warps);
+  const int block_t0 = (int)((long long)blockIdx.x * WARPS * in.T / warps);
   float v[N];
-  // a row's logits, where the balance term wants them
-  auto load = [&](int t) {
-    if (t < t1 && q.counts && !(in.mask && in.mask[t] == 0))
-      load_row<NV>(in.S + t * in.lds, in.E, in.vec, lane, v);
-  };
-  load(t0);
+  if (q.counts) load_row<NV>(in.S + min(t0, in.T - 1) * in.lds, in.E, in.vec, lane, v);
   if (q.dwts) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) *reinterpret_cast<float4*>(add + (j * 32 + lane) * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
   }
+  // the sequence of row t, or -1; the rows between seq[0] and seq[B] lie in one
+  const int lo = in.seq ? in.seq[0] : 0, hi = in.seq ? in.seq[in.B] : in.T;
+  auto seq_at = [&](int t) { return t < lo || t >= hi ? -1 : in.seq ? seq_of(in.seq, in.B, t, lane) : 0; };
+  int block_b = -1;
   float scale = 0.f;  // alpha dloss E / (B' K)
-  const int* seq = in.seq;
   if (q.counts) {
     int full = 0;
     for (int i = threadIdx.x; i < in.B; i += THREADS) full += q.rows[i] > 0;
     full = __reduce_add_sync(0xffffffffu, full);
     if (lane == 0) s_full[warp] = full;
-    if (seq && in.B < SEQ_MAX) {
-      for (int i = threadIdx.x; i <= in.B; i += THREADS) s_seq[i] = in.seq[i];
-      seq = s_seq;
+    block_b = seq_at(block_t0);
+    int c[(128 * NV + THREADS - 1) / THREADS];
+#pragma unroll
+    for (int i = 0; i < (128 * NV + THREADS - 1) / THREADS; ++i) {
+      const int e = i * THREADS + threadIdx.x;
+      c[i] = block_b >= 0 && e < in.E ? q.counts[(long long)block_b * in.E + e] : 0;
     }
+    const int n = block_b >= 0 ? q.rows[block_b] : 0;
     __syncthreads();
     full = 0;
     for (int k = 0; k < WARPS; ++k) full += s_full[k];
     scale = q.alpha * (q.dloss ? *q.dloss : 1.0f) * ((float)in.E / ((float)max(full, 1) * (float)in.K));
+    const float k = n > 0 ? scale / (float)n / (float)n : 0.f;
+#pragma unroll
+    for (int i = 0; i < (128 * NV + THREADS - 1) / THREADS; ++i) {
+      const int e = i * THREADS + threadIdx.x;
+      if (e < 128 * NV) s_f[e] = k * (float)c[i];
+    }
+    __syncthreads();
   }
   const float rs = q.dwts ? __bfloat162float(q.rs[0]) : 0.f;
-  const int vec_counts = in.E % 4 == 0 && reinterpret_cast<uintptr_t>(q.counts) % 16 == 0;
+  int b = block_b, b_end = -1;  // the sequence up to row b_end is b
   for (int t = t0; t < t1; ++t) {
     const float* row = in.S + t * in.lds;
     int e = -1;
@@ -334,63 +354,64 @@ __global__ void __launch_bounds__(bal::THREADS, 2) route_backward_kernel(RouterR
       e = in.idx[(long long)t * in.K + lane];
       if (e < 0 || e >= in.E) e = -1;
       if (e >= 0) {
-        float u, r;
-        es = sigmoid_of(row[e], u, r);
-        eslope = u * r * r;
+        float u;
+        es = score_of(row[e], u);
+        eslope = slope_of(es, u);
         eg = q.dwts[(long long)t * in.K + lane];
       }
     }
-    int b = -1;
-    if (q.counts && !(in.mask && in.mask[t] == 0)) {
-      if (!seq) b = 0;
-      else if (t >= seq[0] && t < seq[in.B]) b = seq_of(seq, in.B, t);
+    const bool counted = q.counts && !(in.mask && in.mask[t] == 0);
+    if (counted && t >= b_end) {
+      b = seq_at(t);
+      b_end = b < 0 ? t + 1 : in.seq ? in.seq[b + 1] : in.T;
     }
     float d[N];
-    if (b >= 0) {
-      const int n = q.rows[b];
-      const float k = n > 0 ? scale / (float)n / (float)n : 0.f;
-      const int* cb = q.counts + (long long)b * in.E;
-      float z = 0.f, m = 0.f, f[N];
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int c = (j * 32 + lane) * 4;
-        int4 g = make_int4(0, 0, 0, 0);
-        if (vec_counts) {
-          if (c < in.E) g = *reinterpret_cast<const int4*>(cb + c);
-        } else {
-          if (c < in.E) g.x = cb[c];
-          if (c + 1 < in.E) g.y = cb[c + 1];
-          if (c + 2 < in.E) g.z = cb[c + 2];
-          if (c + 3 < in.E) g.w = cb[c + 3];
-        }
-        f[4 * j] = k * (float)g.x;
-        f[4 * j + 1] = k * (float)g.y;
-        f[4 * j + 2] = k * (float)g.z;
-        f[4 * j + 3] = k * (float)g.w;
-      }
+    if (counted && b >= 0) {
+      float z = 0.f, m = 0.f;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        float u, r;
-        const float s = sigmoid_of(v[i], u, r);
+        float u;
+        const float s = score_of(v[i], u);
         z += s;
-        m += f[i] * s;
-        d[i] = u * r * r;
+        d[i] = s;
+        v[i] = slope_of(s, u);
       }
-      load(t + 1);
-      z = warp_sum(z) + TINY;
-      m = warp_sum(m) / z;
-      const float inv = __frcp_rn(z);
+      if (b == block_b) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) d[i] = (f[i] - m) * (d[i] * inv);
+        for (int j = 0; j < NV; ++j) {
+          const float4 f = *reinterpret_cast<const float4*>(s_f + (j * 32 + lane) * 4);
+          m += f.x * d[4 * j] + f.y * d[4 * j + 1] + f.z * d[4 * j + 2] + f.w * d[4 * j + 3];
+          d[4 * j] = f.x;
+          d[4 * j + 1] = f.y;
+          d[4 * j + 2] = f.z;
+          d[4 * j + 3] = f.w;
+        }
+      } else {
+        const int n = q.rows[b];
+        const float k = n > 0 ? scale / (float)n / (float)n : 0.f;
+        const int* cb = q.counts + (long long)b * in.E;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int c = ((i >> 2) * 32 + lane) * 4 + (i & 3);
+          const float f = c < in.E ? k * (float)cb[c] : 0.f;
+          m += f * d[i];
+          d[i] = f;
+        }
+      }
+      z = warp_sum(z) + TINY;
+      const float inv = __frcp_rn(z);
+      m = warp_sum(m) * inv;
+#pragma unroll
+      for (int i = 0; i < N; ++i) d[i] = (d[i] - m) * (v[i] * inv);
     } else {
-      load(t + 1);
 #pragma unroll
       for (int i = 0; i < N; ++i) d[i] = 0.f;
     }
+    if (q.counts && t + 1 < t1) load_row<NV>(row + in.lds, in.E, in.vec, lane, v);
     if (q.dwts) {
-      const float den = warp_sum(es) + TINY;
-      const float mean = warp_sum(eg * es) / den;
-      const float mine = rs / den * (eg - mean) * eslope;
+      const float den = __frcp_rn(warp_sum(es) + TINY);
+      const float mean = warp_sum(eg * es) * den;
+      const float mine = rs * den * (eg - mean) * eslope;
       // an expert named twice gets both parts, added in pick order
       const u32 peers = __match_any_sync(0xffffffffu, e);
       if (__all_sync(0xffffffffu, e < 0 || (peers & (peers - 1)) == 0)) {

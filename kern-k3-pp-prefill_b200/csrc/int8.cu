@@ -39,6 +39,12 @@ struct QuantRows {
   long long cap_rows;  // output rows
 };
 
+// act(g) * u; SwiGLU's sigmoid by one exponential and one reciprocal instruction (g = -inf: 0 * -inf, a NaN, as for
+// any row that holds an infinity)
+__device__ __forceinline__ float gate_of(float g, float u, int act) {
+  return act == 0 ? g * rcp_ftz(1.0f + ex2_ftz(g * -LOG2E)) * u : gated_act(g, u, act);
+}
+
 // 8 consecutive elements of a row as they are kept: bf16 pairs, or f32
 template <int SRC>
 struct Kept {
@@ -88,8 +94,8 @@ __device__ __forceinline__ void load8(const QuantRows& p, long long r, int c, Ke
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 x = bf16x2_to_f2(g[i]), y = bf16x2_to_f2(u[i]);
-    v.w[(2 * i) % (SRC == I8_BF16 ? 4 : 8)] = __float_as_uint(gated_act(x.x, y.x, p.act));
-    v.w[(2 * i + 1) % (SRC == I8_BF16 ? 4 : 8)] = __float_as_uint(gated_act(x.y, y.y, p.act));
+    v.w[(2 * i) % (SRC == I8_BF16 ? 4 : 8)] = __float_as_uint(gate_of(x.x, y.x, p.act));
+    v.w[(2 * i + 1) % (SRC == I8_BF16 ? 4 : 8)] = __float_as_uint(gate_of(x.y, y.y, p.act));
   }
 }
 
@@ -127,7 +133,7 @@ __device__ __forceinline__ RowScale row_scale(u32 amax_bits) {
 }
 
 // the code of an element whose quotient lies near k + 1/2 in magnitude
-__device__ __noinline__ int code_near_half(float x, int k, float amax) {
+__device__ __forceinline__ int code_near_half(float x, int k, float amax) {
   const double a = 254.0 * fabs((double)x), h = (double)(2 * k + 1) * (double)amax;
   const int m = a > h || (a == h && (k & 1)) ? k + 1 : k;
   return x < 0.f ? -m : m;
@@ -136,40 +142,38 @@ __device__ __noinline__ int code_near_half(float x, int k, float amax) {
 template <int SRC>
 __device__ __forceinline__ uint2 encode8(const RowScale& s, const Kept<SRC>& v) {
   constexpr float ROUND = 12582912.f;  // 1.5 * 2^23: the integer sits in the low bits
+  constexpr float NEAR = 0.5f - 1e-5f;
   if (s.inv == 0.f) return make_uint2(0u, 0u);
-  float x[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = v[i];
-  if (s.pre != 1.f) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] *= s.pre;
-  }
-  u32 t[8];
+  const u64 inv = f32x2(s.inv, s.inv), round = f32x2(ROUND, ROUND), minus = f32x2(-1.f, -1.f);
+  u64 t[4];
   float far = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float n = __fmaf_rn(x[i], s.inv, ROUND);
-    far = fmaxf(far, fabsf(__fmaf_rn(x[i], s.inv, -(n - ROUND))));
-    t[i] = __float_as_uint(n);
+  for (int i = 0; i < 4; ++i) {
+    u64 x = f32x2(v[2 * i], v[2 * i + 1]);
+    if (s.pre != 1.f) x = mul_f32x2(x, f32x2(s.pre, s.pre));
+    t[i] = fma_f32x2(x, inv, round);
+    const float2 d = f32x2_get(fma_f32x2(x, inv, fma_f32x2(t[i], minus, round)));  // x inv - its integer
+    far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
   }
-  if (far > 0.5f - 1e-5f) {  // one group in a thousand
-#pragma unroll 1
+  u32 k[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = f32x2_get(t[i]);
+    k[2 * i] = __float_as_uint(f.x);
+    k[2 * i + 1] = __float_as_uint(f.y);
+  }
+  if (far > NEAR) {  // one group in some thousands
+#pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float xi = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) xi = k == i ? x[k] : xi;
-      const float n = __fmaf_rn(xi, s.inv, ROUND) - ROUND, d = __fmaf_rn(xi, s.inv, -n);
-      if (fabsf(d) > 0.5f - 1e-5f) {
-        // |quotient| = |n| + d (with n's sign): the integer below it
-        const int k0 = (int)fabsf(n) - (n != 0.f && (d < 0.f) == (n > 0.f) ? 1 : 0);
-        const int c = code_near_half(xi, k0, s.amax * s.pre);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) t[k] = k == i ? (u32)c : t[k];
-      }
+      const float x = v[i] * s.pre;
+      const float n = __uint_as_float(k[i]) - ROUND, d = __fmaf_rn(x, s.inv, -n);
+      // |quotient| = |n| + d (with n's sign), and the integer below it
+      if (fabsf(d) > NEAR)
+        k[i] = (u32)code_near_half(x, (int)fabsf(n) - (n != 0.f && (d < 0.f) == (n > 0.f) ? 1 : 0), s.amax * s.pre);
     }
   }
-  const u32 a = __byte_perm(t[0], t[1], 0x0040), b = __byte_perm(t[2], t[3], 0x0040);
-  const u32 c = __byte_perm(t[4], t[5], 0x0040), d = __byte_perm(t[6], t[7], 0x0040);
+  const u32 a = __byte_perm(k[0], k[1], 0x0040), b = __byte_perm(k[2], k[3], 0x0040);
+  const u32 c = __byte_perm(k[4], k[5], 0x0040), d = __byte_perm(k[6], k[7], 0x0040);
   return make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410));
 }
 __device__ __forceinline__ void put8(int8_t* dst, int left, uint2 w) {
