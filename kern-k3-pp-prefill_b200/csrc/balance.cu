@@ -19,9 +19,17 @@
 namespace k3 {
 
 namespace bal {
-constexpr int WARPS = 8;         // of a block of the join and of the gradient
+constexpr int WARPS = 8;         // of a block of the join
 constexpr int THREADS = 32 * WARPS;
-constexpr int ROW_WARPS = 16;    // of a block of the first pass
+constexpr int ROW_WARPS = 16;    // of a block that walks rows
+constexpr int PICKS = 16;        // K at most
+// Row slots a warp: as many as fit, four at most.  One block an SM where a row is long, two where it is short.
+__host__ __device__ constexpr int slots(int nv) { return nv <= 5 ? 4 : nv <= 7 ? 3 : 2; }
+__host__ __device__ constexpr int blocks_per_sm(int nv) { return nv <= 2 ? 2 : 1; }
+__host__ __device__ constexpr int slot_floats(int nv) { return 128 * nv + 2 * PICKS; }
+__host__ __device__ constexpr int ring_bytes(int nv) { return ROW_WARPS * slots(nv) * slot_floats(nv) * 4; }
+__host__ __device__ constexpr int rows_smem(int nv) { return ring_bytes(nv) + (ROW_WARPS / 2) * 128 * nv * 4 + 128 * nv * 4; }
+__host__ __device__ constexpr int grad_smem(int nv) { return ring_bytes(nv) + 128 * nv * 4; }
 constexpr float TINY = 1e-20f;  // the top-k's guard of its own sum
 constexpr int COLS = 32;        // experts a block of the second pass
 }  // namespace bal
@@ -53,24 +61,53 @@ __device__ __forceinline__ int seq_of(const int* __restrict__ seq, int B, int r,
   return lo;
 }
 
-// A lane's experts: 4 consecutive ones in each group of 128, (j * 32 + lane) * 4 + i.  Past E: -inf (score 0).
+// A row on its way through shared memory: the logits, the picks, the gradients of their weights.  Each warp keeps a few
+// rows in flight by cp.async, which takes no registers and leaves nothing to spin on.  A lane's experts are 4 consecutive
+// ones in each group of 128, (j * 32 + lane) * 4 + i, and it copies what it will read; experts past E stay at -inf.
 template <int NV>
-__device__ __forceinline__ void load_row(const float* __restrict__ row, int E, int vec, int lane, float (&v)[4 * NV]) {
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int c = (j * 32 + lane) * 4;
-    if (vec && c + 4 <= E) {
-      const float4 q = *reinterpret_cast<const float4*>(row + c);
-      v[4 * j] = q.x;
-      v[4 * j + 1] = q.y;
-      v[4 * j + 2] = q.z;
-      v[4 * j + 3] = q.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[4 * j + i] = c + i < E ? row[c + i] : -INFINITY;
-    }
+struct RowRing {
+  float* base;
+  int lane;
+  __device__ __forceinline__ float* slot(int i) const { return base + (i % bal::slots(NV)) * bal::slot_floats(NV); }
+  __device__ __forceinline__ void init(float* smem, int warp, int lane_, int E) {
+    lane = lane_;
+    base = smem + warp * bal::slots(NV) * bal::slot_floats(NV);
+    for (int s = 0; s < bal::slots(NV); ++s)
+      for (int c = E / 4 * 4 + lane; c < 128 * NV; c += 32) slot(s)[c] = -INFINITY;
+    __syncwarp();
   }
-}
+  // start row t's copy into slot i (t < 0: an empty group, so that the groups count up with the rows)
+  __device__ __forceinline__ void fetch(const RouterRows& in, int i, int t, bool logits, bool picks, const float* dwts) {
+    if (t >= 0) {
+      float* d = slot(i);
+      const u32 s = smem_u32(d);
+      const float* row = in.S + t * in.lds;
+      if (logits) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int c = (j * 32 + lane) * 4;
+          if (in.vec && c + 4 <= in.E) {
+            cp_async16(s + c * 4, row + c);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (c + k < in.E) cp_async4(s + (c + k) * 4, row + c + k);
+          }
+        }
+      }
+      if (picks && lane < in.K) {
+        cp_async4(s + (128 * NV + lane) * 4, in.idx + (long long)t * in.K + lane);
+        if (dwts) cp_async4(s + (128 * NV + bal::PICKS + lane) * 4, dwts + (long long)t * in.K + lane);
+      }
+    }
+    cp_async_commit();
+  }
+  // wait until the oldest of the copies in flight is there (slots - 1 younger ones may be on their way)
+  __device__ __forceinline__ void wait() const {
+    cp_async_wait_group<bal::slots(NV) - 1>();
+    __syncwarp();
+  }
+};
 
 // e = exp(-x): the score is 1 / (1 + e) and its slope e / (1 + e)^2, without cancellation at either end
 __device__ __forceinline__ float score_of(float x, float& e) {
@@ -88,10 +125,10 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // ---------------------------------------------------------------- forward
-// First pass: a block an SM takes `chunk` consecutive rows, a warp every sixteenth of them, each lane summing its
-// experts' p in registers while its next row is on the way.  At the end of a sequence, or of the block's rows, the
-// warps' sums are added in order and stored as one partial row.  Block i and sequence b meet in slot i + b: along the
-// rows either i or b goes up, so no two pairs share a slot and nothing needs zeroing.
+// First pass: a block takes `chunk` consecutive rows, a warp every sixteenth of them, each lane summing its experts' p in
+// registers.  At the end of a sequence, or of the block's rows, the warps' sums are added in order and stored as one
+// partial row.  Block i and sequence b meet in slot i + b: along the rows either i or b goes up, so no two pairs share a
+// slot and nothing needs zeroing.
 struct BalanceScratch {
   float* prob;   // [slots, E]
   int* count;    // [slots, E]
@@ -101,34 +138,31 @@ struct BalanceScratch {
 };
 
 template <int NV>
-__global__ void __launch_bounds__(32 * bal::ROW_WARPS) balance_rows_kernel(RouterRows in, BalanceScratch w, int chunk) {
+__global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
+    balance_rows_kernel(RouterRows in, BalanceScratch w, int chunk) {
   using namespace bal;
   constexpr int N = 4 * NV;
-  __shared__ float s_acc[ROW_WARPS / 2][128 * NV];
-  __shared__ int s_hist[128 * NV];
+  extern __shared__ __align__(16) float ring_smem[];
+  float* s_acc = ring_smem + ring_bytes(NV) / 4;                              // [ROW_WARPS / 2][128 NV]
+  int* s_hist = reinterpret_cast<int*>(s_acc + ROW_WARPS / 2 * 128 * NV);  // [128 NV]
   __shared__ int s_rows[ROW_WARPS];
   grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r0 = blockIdx.x * chunk, r1 = min(in.T, r0 + chunk);
   if (blockIdx.x == 0 && threadIdx.x == 0) *w.done = 0u;
-  float v[N];
-  int pick = -1, held = r0 + warp;  // v, pick: row `held`'s logits and pick, on their way
-  auto load = [&](int t) {
-    held = t;
-    load_row<NV>(in.S + t * in.lds, in.E, in.vec, lane, v);
-    if (lane < in.K) pick = in.idx[(long long)t * in.K + lane];
+  RowRing<NV> ring;
+  ring.init(ring_smem, warp, lane, in.E);
+  int t = r0 + warp, at = 0;  // the warp's next row, in slot `at`
+  auto ahead = [&](int i) {
+    const int u = t + i * ROW_WARPS;
+    return u < r1 ? u : -1;
   };
-  if (held < r1) load(held);
+  for (int i = 0; i < slots(NV) - 1; ++i) ring.fetch(in, i, ahead(i), true, true, nullptr);
   int r = r0, last = r1;
   if (in.seq) {
     r = max(r0, in.seq[0]);
     last = min(r1, in.seq[in.B]);
   }
-  // the next counted row from t on in steps of the warps, or `end`
-  auto counted = [&](int t, int end) {
-    while (t < end && in.mask && in.mask[t] == 0) t += ROW_WARPS;
-    return t;
-  };
   while (r < last) {
     int b = 0, end = last;
     if (in.seq) {
@@ -137,31 +171,39 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS) balance_rows_kernel(Route
       if (end <= r) break;  // offsets that go down: nothing more is counted
     }
     float acc[N];
-    int n = 0;
-    int t = counted(r + warp, end);
-    if (t < end && t != held) load(t);
-    for (int e = threadIdx.x; e < in.E; e += 32 * ROW_WARPS) s_hist[e] = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    int n = 0;
+    for (int e = threadIdx.x; e < in.E; e += 32 * ROW_WARPS) s_hist[e] = 0;
     __syncthreads();
-    while (t < end) {
+    for (; t < end; t += ROW_WARPS, ++at) {
+      ring.fetch(in, at + slots(NV) - 1, ahead(slots(NV) - 1), true, true, nullptr);
+      ring.wait();
+      if (t < r || (in.mask && in.mask[t] == 0)) continue;
       ++n;
+      const float* row = ring.slot(at);
       float z = 0.f, s[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
+      for (int j = 0; j < NV; ++j) {
+        const float4 v = *reinterpret_cast<const float4*>(row + (j * 32 + lane) * 4);
         float u;
-        s[i] = score_of(v[i], u);
-        z += s[i];
+        s[4 * j] = score_of(v.x, u);
+        s[4 * j + 1] = score_of(v.y, u);
+        s[4 * j + 2] = score_of(v.z, u);
+        s[4 * j + 3] = score_of(v.w, u);
+        z += (s[4 * j] + s[4 * j + 1]) + (s[4 * j + 2] + s[4 * j + 3]);
       }
-      if (lane < in.K && pick >= 0 && pick < in.E) atomicAdd(&s_hist[pick], 1);
-      t = counted(t + ROW_WARPS, end);
-      if (t < end) load(t);
+      if (lane < in.K) {
+        const int e = reinterpret_cast<const int*>(row + 128 * NV)[lane];
+        if (e >= 0 && e < in.E) atomicAdd(&s_hist[e], 1);
+      }
       const float inv = __frcp_rn(warp_sum(z) + TINY);
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[i] += s[i] * inv;
+      __syncwarp();  // every lane has read the slot that the next fetch fills
     }
     // the upper half of the warps, then the lower half onto them
-    float* mine = s_acc[warp % (ROW_WARPS / 2)];
+    float* mine = s_acc + warp % (ROW_WARPS / 2) * 128 * NV;
     if (warp >= ROW_WARPS / 2) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
@@ -183,7 +225,7 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS) balance_rows_kernel(Route
     for (int e = threadIdx.x; e < in.E; e += 32 * ROW_WARPS) {
       float p = 0.f;
 #pragma unroll
-      for (int k = 0; k < ROW_WARPS / 2; ++k) p += s_acc[k][e];
+      for (int k = 0; k < ROW_WARPS / 2; ++k) p += s_acc[k * 128 * NV + e];
       w.prob[slot * in.E + e] = p;
       w.count[slot * in.E + e] = s_hist[e];
     }
@@ -195,6 +237,7 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS) balance_rows_kernel(Route
     __syncthreads();
     r = end;
   }
+  cp_async_wait_all();
 }
 
 // Second pass: a block adds up 32 experts of one sequence over the first pass's blocks that met it (8 warps side by
@@ -292,95 +335,100 @@ struct RouteBackward {
   int vec_out;          // rows may be stored 4 elements at a time
 };
 
-// A warp takes consecutive rows, with the next row's logits on their way while one is computed.  The coefficients f of
-// the sequence that the block's first row is in lie in shared memory; a block's few rows seldom leave it, and those that
-// do read their counts.  The weight term touches K experts of a row: it is spread through a row of shared memory that is
-// all zero between rows.
+// A block takes consecutive rows, a warp every sixteenth.  The coefficients f of the sequence that the block's first row
+// is in lie in shared memory; a block's few rows seldom leave it, and those that do read their counts.  The weight term
+// touches K experts of a row: it is spread through the row's own slot, whose logits are in registers by then.
 template <int NV>
-__global__ void __launch_bounds__(bal::THREADS, 2) route_backward_kernel(RouterRows in, RouteBackward q) {
+__global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
+    route_backward_kernel(RouterRows in, RouteBackward q, int chunk) {
   using namespace bal;
   constexpr int N = 4 * NV;
-  __shared__ float s_f[128 * NV];
-  __shared__ float s_add[WARPS][128 * NV];
-  __shared__ int s_full[WARPS];
+  constexpr int PER = (128 * NV + 32 * ROW_WARPS - 1) / (32 * ROW_WARPS);
+  extern __shared__ __align__(16) float ring_smem[];
+  float* s_f = ring_smem + ring_bytes(NV) / 4;  // [128 NV]
+  __shared__ int s_full[ROW_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* add = s_add[warp];
-  const long long warps = (long long)gridDim.x * WARPS, w = (long long)blockIdx.x * WARPS + warp;
-  const int t0 = (int)(w * in.T / warps), t1 = (int)((w + 1) * in.T / warps);
-  const int block_t0 = (int)((long long)blockIdx.x * WARPS * in.T / warps);
-  float v[N];
-  if (q.counts) load_row<NV>(in.S + min(t0, in.T - 1) * in.lds, in.E, in.vec, lane, v);
-  if (q.dwts) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) *reinterpret_cast<float4*>(add + (j * 32 + lane) * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-  // the sequence of row t, or -1; the rows between seq[0] and seq[B] lie in one
+  const int r0 = blockIdx.x * chunk, r1 = min(in.T, r0 + chunk);
+  RowRing<NV> ring;
+  ring.init(ring_smem, warp, lane, in.E);
+  int t = r0 + warp, at = 0;
+  const bool balance = q.counts != nullptr, weights = q.dwts != nullptr;
+  auto ahead = [&](int i) {
+    const int u = t + i * ROW_WARPS;
+    return u < r1 ? u : -1;
+  };
+  for (int i = 0; i < slots(NV) - 1; ++i) ring.fetch(in, i, ahead(i), balance, weights, q.dwts);
+  // the sequence of row t, or -1
   const int lo = in.seq ? in.seq[0] : 0, hi = in.seq ? in.seq[in.B] : in.T;
   auto seq_at = [&](int t) { return t < lo || t >= hi ? -1 : in.seq ? seq_of(in.seq, in.B, t, lane) : 0; };
   int block_b = -1;
   float scale = 0.f;  // alpha dloss E / (B' K)
-  if (q.counts) {
+  if (balance) {
     int full = 0;
-    for (int i = threadIdx.x; i < in.B; i += THREADS) full += q.rows[i] > 0;
+    for (int i = threadIdx.x; i < in.B; i += 32 * ROW_WARPS) full += q.rows[i] > 0;
     full = __reduce_add_sync(0xffffffffu, full);
     if (lane == 0) s_full[warp] = full;
-    block_b = seq_at(block_t0);
-    int c[(128 * NV + THREADS - 1) / THREADS];
+    block_b = seq_at(r0);
+    int c[PER];
 #pragma unroll
-    for (int i = 0; i < (128 * NV + THREADS - 1) / THREADS; ++i) {
-      const int e = i * THREADS + threadIdx.x;
+    for (int i = 0; i < PER; ++i) {
+      const int e = i * 32 * ROW_WARPS + threadIdx.x;
       c[i] = block_b >= 0 && e < in.E ? q.counts[(long long)block_b * in.E + e] : 0;
     }
     const int n = block_b >= 0 ? q.rows[block_b] : 0;
+    const float dloss = q.dloss ? *q.dloss : 1.0f;
     __syncthreads();
     full = 0;
-    for (int k = 0; k < WARPS; ++k) full += s_full[k];
-    scale = q.alpha * (q.dloss ? *q.dloss : 1.0f) * ((float)in.E / ((float)max(full, 1) * (float)in.K));
+    for (int k = 0; k < ROW_WARPS; ++k) full += s_full[k];
+    scale = q.alpha * dloss * ((float)in.E / ((float)max(full, 1) * (float)in.K));
     const float k = n > 0 ? scale / (float)n / (float)n : 0.f;
 #pragma unroll
-    for (int i = 0; i < (128 * NV + THREADS - 1) / THREADS; ++i) {
-      const int e = i * THREADS + threadIdx.x;
+    for (int i = 0; i < PER; ++i) {
+      const int e = i * 32 * ROW_WARPS + threadIdx.x;
       if (e < 128 * NV) s_f[e] = k * (float)c[i];
     }
     __syncthreads();
   }
-  const float rs = q.dwts ? __bfloat162float(q.rs[0]) : 0.f;
-  int b = block_b, b_end = -1;  // the sequence up to row b_end is b
-  for (int t = t0; t < t1; ++t) {
-    const float* row = in.S + t * in.lds;
+  const float rs = weights ? __bfloat162float(q.rs[0]) : 0.f;
+  int b = -1, b_end = -1;  // the sequence up to row b_end is b
+  for (; t < r1; t += ROW_WARPS, ++at) {
+    ring.fetch(in, at + slots(NV) - 1, ahead(slots(NV) - 1), balance, weights, q.dwts);
+    ring.wait();
+    float* row = ring.slot(at);
+    // the lane's pick, its logit and the gradient of its weight
     int e = -1;
-    float es = 0.f, eg = 0.f, eslope = 0.f;  // the lane's pick: score, gradient of its weight, slope
-    if (q.dwts && lane < in.K) {
-      e = in.idx[(long long)t * in.K + lane];
+    float pick = 0.f, eg = 0.f;
+    if (weights && lane < in.K) {
+      e = reinterpret_cast<const int*>(row + 128 * NV)[lane];
       if (e < 0 || e >= in.E) e = -1;
-      if (e >= 0) {
-        float u;
-        es = score_of(row[e], u);
-        eslope = slope_of(es, u);
-        eg = q.dwts[(long long)t * in.K + lane];
-      }
+      eg = row[128 * NV + PICKS + lane];
+      if (e >= 0) pick = balance ? row[e] : in.S[t * in.lds + e];
     }
-    const bool counted = q.counts && !(in.mask && in.mask[t] == 0);
+    const bool counted = balance && !(in.mask && in.mask[t] == 0);
     if (counted && t >= b_end) {
       b = seq_at(t);
       b_end = b < 0 ? t + 1 : in.seq ? in.seq[b + 1] : in.T;
     }
     float d[N];
     if (counted && b >= 0) {
-      float z = 0.f, m = 0.f;
+      float z = 0.f, m = 0.f, slope[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        float u;
-        const float s = score_of(v[i], u);
-        z += s;
-        d[i] = s;
-        v[i] = slope_of(s, u);
+      for (int j = 0; j < NV; ++j) {
+        const float4 v = *reinterpret_cast<const float4*>(row + (j * 32 + lane) * 4);
+        const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float u;
+          d[4 * j + i] = score_of(x[i], u);
+          slope[4 * j + i] = slope_of(d[4 * j + i], u);
+        }
+        z += (d[4 * j] + d[4 * j + 1]) + (d[4 * j + 2] + d[4 * j + 3]);
       }
       if (b == block_b) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           const float4 f = *reinterpret_cast<const float4*>(s_f + (j * 32 + lane) * 4);
-          m += f.x * d[4 * j] + f.y * d[4 * j + 1] + f.z * d[4 * j + 2] + f.w * d[4 * j + 3];
+          m += (f.x * d[4 * j] + f.y * d[4 * j + 1]) + (f.z * d[4 * j + 2] + f.w * d[4 * j + 3]);
           d[4 * j] = f.x;
           d[4 * j + 1] = f.y;
           d[4 * j + 2] = f.z;
@@ -402,38 +450,54 @@ __global__ void __launch_bounds__(bal::THREADS, 2) route_backward_kernel(RouterR
       const float inv = __frcp_rn(z);
       m = warp_sum(m) * inv;
 #pragma unroll
-      for (int i = 0; i < N; ++i) d[i] = (d[i] - m) * (v[i] * inv);
+      for (int i = 0; i < N; ++i) d[i] = (d[i] - m) * (slope[i] * inv);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) d[i] = 0.f;
     }
-    if (q.counts && t + 1 < t1) load_row<NV>(row + in.lds, in.E, in.vec, lane, v);
-    if (q.dwts) {
+    if (weights) {
+      float u, es = 0.f, slope = 0.f;
+      if (e >= 0) {
+        es = score_of(pick, u);
+        slope = slope_of(es, u);
+      } else {
+        eg = 0.f;
+      }
       const float den = __frcp_rn(warp_sum(es) + TINY);
       const float mean = warp_sum(eg * es) * den;
-      const float mine = rs * den * (eg - mean) * eslope;
+      const float mine = rs * den * (eg - mean) * slope;
+      __syncwarp();  // the logits have been read: the slot turns into the row's weight term
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = (j * 32 + lane) * 4;
+        if (c + 4 <= in.E) {
+          *reinterpret_cast<float4*>(row + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (c + i < in.E) row[c + i] = 0.f;
+        }
+      }
+      __syncwarp();
       // an expert named twice gets both parts, added in pick order
       const u32 peers = __match_any_sync(0xffffffffu, e);
       if (__all_sync(0xffffffffu, e < 0 || (peers & (peers - 1)) == 0)) {
-        if (e >= 0) add[e] = mine;
+        if (e >= 0) row[e] = mine;
       } else {
         for (int k = 0; k < in.K; ++k) {
-          if (lane == k && e >= 0) add[e] += mine;
+          if (lane == k && e >= 0) row[e] += mine;
           __syncwarp();
         }
       }
       __syncwarp();
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const float4 a = *reinterpret_cast<const float4*>(add + (j * 32 + lane) * 4);
+        const float4 a = *reinterpret_cast<const float4*>(row + (j * 32 + lane) * 4);
         d[4 * j] += a.x;
         d[4 * j + 1] += a.y;
         d[4 * j + 2] += a.z;
         d[4 * j + 3] += a.w;
       }
-      __syncwarp();
-      if (e >= 0) add[e] = 0.f;
-      __syncwarp();
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -459,7 +523,9 @@ __global__ void __launch_bounds__(bal::THREADS, 2) route_backward_kernel(RouterR
         }
       }
     }
+    __syncwarp();  // every lane has read the slot that the next fetch fills
   }
+  cp_async_wait_all();
 }
 
 }  // namespace k3

@@ -49,7 +49,7 @@ int current_device() {
 template <typename F>
 bool set_smem_once(F kernel, int bytes, int slot) {
   static std::mutex mu;
-  static bool done[kMaxDevices][16] = {};
+  static bool done[kMaxDevices][24] = {};
   const int dev = current_device();
   std::lock_guard<std::mutex> g(mu);
   if (dev >= 0 && dev < kMaxDevices && done[dev][slot]) return true;
@@ -234,9 +234,11 @@ LayerLayout layer_layout(int T, int H, int I, int E, int K, int shared) {
 
 namespace {
 
-// rows a block of the first pass takes: a block an SM over the rows, in eights.  A function of T alone, so that the
-// scratch size is too.
-int balance_chunk(int T) { return std::max(8, (int)align_up((size_t)cdiv(T, 148), 8)); }
+// rows a block takes that walks rows: one block an SM (more where rows are short), at least half a row a warp.  A function
+// of the sizes alone, so that the scratch size is too.
+int router_chunk(int T, int E) {
+  return std::max(bal::ROW_WARPS / 2, (int)cdiv(T, 148 * bal::blocks_per_sm((E + 127) / 128)));
+}
 
 struct BalanceLayout {
   int chunk, blocks;
@@ -244,7 +246,7 @@ struct BalanceLayout {
 };
 BalanceLayout balance_layout(int T, int E, int B) {
   BalanceLayout L;
-  L.chunk = balance_chunk(T);
+  L.chunk = router_chunk(T, E);
   L.blocks = std::max(1, (int)cdiv(T, L.chunk));
   const size_t slots = (size_t)L.blocks + B;
   size_t at = 0;
@@ -263,7 +265,7 @@ BalanceLayout balance_layout(int T, int E, int B) {
 }
 
 bool router_sizes_ok(int T, int E, int K, int B, const int32_t* seq, int lds) {
-  return T >= 0 && E >= 1 && E <= 1024 && K >= 1 && K <= 16 && lds >= E && B >= 1 && (seq || B == 1) &&
+  return T >= 0 && T <= 1 << 30 && E >= 1 && E <= 1024 && K >= 1 && K <= 16 && lds >= E && B >= 1 && (seq || B == 1) &&
          (long long)B * cdiv(E, bal::COLS) < 0x7fffffffLL && (long long)B < 0x7fffffffLL - T;
 }
 
@@ -564,7 +566,7 @@ int k3moe_router_gemm(const void* x_bf16, int ldx, const void* w_bf16, int ldw, 
 // ---------------------------------------------------------------- the router's training side
 
 size_t k3moe_balance_scratch_bytes(int T, int E, int B) {
-  if (T < 0 || E < 1 || E > 1024 || B < 1) return 0;
+  if (T < 0 || T > 1 << 30 || E < 1 || E > 1024 || B < 1) return 0;
   return balance_layout(T, E, B).total;
 }
 
@@ -584,9 +586,13 @@ int k3moe_balance_loss(const float* S, int lds, const int32_t* idx, int T, int E
   w.done = reinterpret_cast<u32*>(ws + L.done);
   const RouterRows in = router_rows(S, lds, idx, T, E, K, seq, B, mask);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  bool ready = false;
   by_experts(E, [&](auto nv) {
-    balance_rows_kernel<decltype(nv)::value><<<L.blocks, 32 * bal::ROW_WARPS, 0, s>>>(in, w, L.chunk);
+    constexpr int NV = decltype(nv)::value, bytes = bal::rows_smem(NV);
+    ready = set_smem_once(balance_rows_kernel<NV>, bytes, 5 + NV);
+    if (ready) balance_rows_kernel<NV><<<L.blocks, 32 * bal::ROW_WARPS, bytes, s>>>(in, w, L.chunk);
   });
+  if (!ready) return K3MOE_ELAUNCH;
   const long long blocks = (long long)B * cdiv(E, bal::COLS);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
@@ -624,11 +630,16 @@ int k3moe_route_backward(const float* S, int lds, const int32_t* idx, int T, int
   q.ldd = ldd;
   q.bf16_out = dtype == K3MOE_BF16;
   q.vec_out = ldd % 4 == 0 && reinterpret_cast<uintptr_t>(dS) % (q.bf16_out ? 8 : 16) == 0;
-  const int grid = (int)std::min<long long>(cdiv(T, bal::WARPS), (long long)num_sms(current_device()) * 2);
+  const int chunk = router_chunk(T, E), grid = (int)cdiv(T, chunk);
+  bool ready = false;
   by_experts(E, [&](auto nv) {
-    route_backward_kernel<decltype(nv)::value>
-        <<<grid, bal::THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(in, q);
+    constexpr int NV = decltype(nv)::value, bytes = bal::grad_smem(NV);
+    ready = set_smem_once(route_backward_kernel<NV>, bytes, 13 + NV);
+    if (ready)
+      route_backward_kernel<NV>
+          <<<grid, 32 * bal::ROW_WARPS, bytes, reinterpret_cast<cudaStream_t>(stream)>>>(in, q, chunk);
   });
+  if (!ready) return K3MOE_ELAUNCH;
   return launch_status();
 }
 

@@ -242,6 +242,16 @@ __device__ __forceinline__ void grid_wait_previous() { asm volatile("griddepcont
 __device__ __forceinline__ void cp_async16(u32 dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+// 4 bytes, for what is not 16-byte aligned
+__device__ __forceinline__ void cp_async4(u32 dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// until at most N of this thread's groups are still on their way
+template <int N>
+__device__ __forceinline__ void cp_async_wait_group() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 // arrive on `bar` once every cp.async this thread issued so far has landed (the barrier counts the arrival)
 __device__ __forceinline__ void cp_async_mbar_arrive_noinc(u64* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");

@@ -11,12 +11,18 @@ namespace k3 {
 
 // ============================================================ quantiser
 // amax = the row's largest magnitude, scale = amax / 127, q = round-half-even(127 x / amax): the rounding of the real
-// quotient, not of a float product.  One FMA rounds x * inv, inv = fl(127 / amax), to an integer (1.5 * 2^23 + x inv);
-// inv's error moves the quotient by at most 127 * 2^-24 = 7.6e-6, so every element whose x * inv is further than 1e-5
-// from a half is settled, and the others compare 254 |x| with (2k + 1) amax, both exact in double.
+// quotient, not of a float product.
+// bf16: with inv = 127 / amax rounded up and down, one FMA each (1.5 * 2^23 + x inv) rounds the quotient seen from either
+// side.  The quotient of two 8-bit mantissas is a half exactly or at least 2^-9 |q| / 256 from one, far more than the 2^-23
+// |q| that inv is off by, so the two integers are equal, or the neighbours of an exact half: then the even one is it, bit
+// arithmetic on pairs, no branch (ties are common: rows whose maximum has few mantissa bits have them by the hundred, and
+// a branch for them took 30% of the kernel's instructions).  The gate's values are rounded themselves, so the same rule
+// serves there, a quotient within 2^-15 of a half taken as one.
+// f32: one FMA, and the elements whose x inv is within 1e-5 of a half (inv moves the quotient by 7.6e-6 at most) compare
+// 254 |x| with (2k + 1) amax, both exact in double.
 // A row with an infinity or a NaN has scale NaN and q = 0, so every result it enters is NaN; a zero row scale 0, q = 0.
 // HBM-bound: a row is read once and kept in registers (bf16 as it came) between the maximum and the codes; what counts
-// beside the bytes is the instructions an element, about 6.
+// beside the bytes is the instructions an element, about 7.
 enum { I8_BF16 = 0, I8_F32 = 1, I8_GATED = 2 };
 
 struct QuantRows {
@@ -114,19 +120,21 @@ __device__ __forceinline__ u32 max_bits(u32 m, const Kept<SRC>& v) {
 }
 
 struct RowScale {
-  float amax, pre, inv, scale;  // pre: a power of two that keeps 127 / amax finite
+  float amax, pre, inv, up, down, scale;  // pre: a power of two that keeps 127 / amax finite
 };
 __device__ __forceinline__ RowScale row_scale(u32 amax_bits) {
   RowScale s;
   s.amax = __uint_as_float(amax_bits);
   if (amax_bits >= 0x7f800000u) {
-    s.pre = s.inv = 0.f;
+    s.pre = s.inv = s.up = s.down = 0.f;
     s.scale = __uint_as_float(0x7fc00000u);
   } else if (amax_bits == 0u) {
-    s.pre = s.inv = s.scale = 0.f;
+    s.pre = s.inv = s.up = s.down = s.scale = 0.f;
   } else {
     s.pre = s.amax < 0x1p-60f ? 0x1p64f : s.amax > 0x1p60f ? 0x1p-64f : 1.f;
     s.inv = __fdiv_rn(127.f, s.amax * s.pre);
+    s.up = __fdiv_ru(127.f, s.amax * s.pre);
+    s.down = __fdiv_rd(127.f, s.amax * s.pre);
     s.scale = __fdiv_rn(s.amax, 127.f);
   }
   return s;
@@ -141,26 +149,34 @@ __device__ __forceinline__ int code_near_half(float x, int k, float amax) {
 
 template <int SRC>
 __device__ __forceinline__ uint2 encode8(const RowScale& s, const Kept<SRC>& v) {
+  if (s.inv == 0.f) return make_uint2(0u, 0u);
+  if (SRC != I8_F32) {
+    constexpr float ROUND = 12582912.f + 256.f;  // the integer, plus 256, in the low 16 bits
+    const u64 up = f32x2(s.up, s.up), down = f32x2(s.down, s.down), round = f32x2(ROUND, ROUND);
+    u32 k[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u64 x = f32x2(v[2 * i], v[2 * i + 1]);
+      if (s.pre != 1.f) x = mul_f32x2(x, f32x2(s.pre, s.pre));
+      const float2 a = f32x2_get(fma_f32x2(x, up, round)), b = f32x2_get(fma_f32x2(x, down, round));
+      // two elements' integers in the halves of a word; their sum is odd where the two roundings differ, and half of it
+      // rounded up to even is the code
+      const u32 sum = __byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x5410) +
+                      __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x5410);
+      const u32 half = sum >> 1;
+      k[i] = half + (sum & half & 0x00010001u);
+    }
+    return make_uint2(__byte_perm(k[0], k[1], 0x6420), __byte_perm(k[2], k[3], 0x6420));
+  }
   constexpr float ROUND = 12582912.f;  // 1.5 * 2^23: the integer sits in the low bits
   constexpr float NEAR = 0.5f - 1e-5f;
-  if (s.inv == 0.f) return make_uint2(0u, 0u);
-  const u64 inv = f32x2(s.inv, s.inv), round = f32x2(ROUND, ROUND), minus = f32x2(-1.f, -1.f);
-  u64 t[4];
+  u32 k[8];
   float far = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    u64 x = f32x2(v[2 * i], v[2 * i + 1]);
-    if (s.pre != 1.f) x = mul_f32x2(x, f32x2(s.pre, s.pre));
-    t[i] = fma_f32x2(x, inv, round);
-    const float2 d = f32x2_get(fma_f32x2(x, inv, fma_f32x2(t[i], minus, round)));  // x inv - its integer
-    far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
-  }
-  u32 k[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = f32x2_get(t[i]);
-    k[2 * i] = __float_as_uint(f.x);
-    k[2 * i + 1] = __float_as_uint(f.y);
+  for (int i = 0; i < 8; ++i) {
+    const float x = v[i] * s.pre, t = __fmaf_rn(x, s.inv, ROUND);
+    far = fmaxf(far, fabsf(__fmaf_rn(x, s.inv, ROUND - t)));  // x inv - its integer
+    k[i] = __float_as_uint(t);
   }
   if (far > NEAR) {  // one group in some thousands
 #pragma unroll
