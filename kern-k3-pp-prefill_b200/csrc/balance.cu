@@ -19,7 +19,7 @@
 namespace k3 {
 
 namespace bal {
-constexpr int WARPS = 8;         // of a block of the join
+constexpr int WARPS = 32;        // of a block of the join
 constexpr int THREADS = 32 * WARPS;
 constexpr int ROW_WARPS = 16;    // of a block that walks rows
 constexpr int PICKS = 16;        // K at most
@@ -109,13 +109,20 @@ struct RowRing {
   }
 };
 
-// e = exp(-x): the score is 1 / (1 + e) and its slope e / (1 + e)^2, without cancellation at either end
-__device__ __forceinline__ float score_of(float x, float& e) {
-  e = ex2_ftz(x * -LOG2E);
-  return rcp_ftz(1.0f + e);
+// With e = exp(-x) the score is 1 / (1 + e) and its slope e / (1 + e)^2, without cancellation at either end; two at a time,
+// four multifunction instructions a pair, which bound the passes once the loads keep up.
+__device__ __forceinline__ u64 exp_neg2(u64 x) {
+  const float2 v = f32x2_get(mul_f32x2(x, f32x2(-LOG2E, -LOG2E)));
+  return f32x2(ex2_ftz(v.x), ex2_ftz(v.y));
 }
-__device__ __forceinline__ float slope_of(float score, float e) {
-  return fminf(e, 3.402823466e38f) * score * score;  // score 0 (x = -inf): 0, not inf * 0
+__device__ __forceinline__ u64 score2(u64 e) {
+  const float2 v = f32x2_get(add_f32x2(e, f32x2(1.f, 1.f)));
+  return f32x2(rcp_ftz(v.x), rcp_ftz(v.y));
+}
+__device__ __forceinline__ u64 slope2(u64 score, u64 e) {
+  const float2 v = f32x2_get(e);
+  constexpr float MOST = 3.402823466e38f;  // score 0 (x = -inf): slope 0, not inf * 0
+  return mul_f32x2(mul_f32x2(f32x2(fminf(v.x, MOST), fminf(v.y, MOST)), score), score);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -141,11 +148,12 @@ template <int NV>
 __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
     balance_rows_kernel(RouterRows in, BalanceScratch w, int chunk) {
   using namespace bal;
-  constexpr int N = 4 * NV;
+  constexpr int N = 2 * NV;  // pairs of experts a lane
   extern __shared__ __align__(16) float ring_smem[];
   float* s_acc = ring_smem + ring_bytes(NV) / 4;                              // [ROW_WARPS / 2][128 NV]
   int* s_hist = reinterpret_cast<int*>(s_acc + ROW_WARPS / 2 * 128 * NV);  // [128 NV]
   __shared__ int s_rows[ROW_WARPS];
+  grid_wait_previous();
   grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r0 = blockIdx.x * chunk, r1 = min(in.T, r0 + chunk);
@@ -170,9 +178,9 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
       end = min(last, in.seq[b + 1]);
       if (end <= r) break;  // offsets that go down: nothing more is counted
     }
-    float acc[N];
+    u64 acc[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] = 0.f;
+    for (int i = 0; i < N; ++i) acc[i] = f32x2(0.f, 0.f);
     int n = 0;
     for (int e = threadIdx.x; e < in.E; e += 32 * ROW_WARPS) s_hist[e] = 0;
     __syncthreads();
@@ -182,24 +190,23 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
       if (t < r || (in.mask && in.mask[t] == 0)) continue;
       ++n;
       const float* row = ring.slot(at);
-      float z = 0.f, s[N];
+      u64 z2 = f32x2(0.f, 0.f), s[N];
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const float4 v = *reinterpret_cast<const float4*>(row + (j * 32 + lane) * 4);
-        float u;
-        s[4 * j] = score_of(v.x, u);
-        s[4 * j + 1] = score_of(v.y, u);
-        s[4 * j + 2] = score_of(v.z, u);
-        s[4 * j + 3] = score_of(v.w, u);
-        z += (s[4 * j] + s[4 * j + 1]) + (s[4 * j + 2] + s[4 * j + 3]);
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(row + (j * 32 + lane) * 4);
+        s[2 * j] = score2(exp_neg2(v.x));
+        s[2 * j + 1] = score2(exp_neg2(v.y));
+        z2 = add_f32x2(z2, add_f32x2(s[2 * j], s[2 * j + 1]));
       }
+      const float2 z = f32x2_get(z2);
       if (lane < in.K) {
         const int e = reinterpret_cast<const int*>(row + 128 * NV)[lane];
         if (e >= 0 && e < in.E) atomicAdd(&s_hist[e], 1);
       }
-      const float inv = __frcp_rn(warp_sum(z) + TINY);
+      const float inv = rcp_ftz(warp_sum(z.x + z.y) + TINY);
+      const u64 inv2 = f32x2(inv, inv);
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] += s[i] * inv;
+      for (int i = 0; i < N; ++i) acc[i] = fma_f32x2(s[i], inv2, acc[i]);
       __syncwarp();  // every lane has read the slot that the next fetch fills
     }
     // the upper half of the warps, then the lower half onto them
@@ -207,17 +214,16 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
     if (warp >= ROW_WARPS / 2) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        *reinterpret_cast<float4*>(mine + (j * 32 + lane) * 4) =
-            make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+        *reinterpret_cast<ulonglong2*>(mine + (j * 32 + lane) * 4) = make_ulonglong2(acc[2 * j], acc[2 * j + 1]);
     }
     if (lane == 0) s_rows[warp] = n;
     __syncthreads();
     if (warp < ROW_WARPS / 2) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        float4* q = reinterpret_cast<float4*>(mine + (j * 32 + lane) * 4);
-        const float4 o = *q;
-        *q = make_float4(o.x + acc[4 * j], o.y + acc[4 * j + 1], o.z + acc[4 * j + 2], o.w + acc[4 * j + 3]);
+        ulonglong2* q = reinterpret_cast<ulonglong2*>(mine + (j * 32 + lane) * 4);
+        const ulonglong2 o = *q;
+        *q = make_ulonglong2(add_f32x2(o.x, acc[2 * j]), add_f32x2(o.y, acc[2 * j + 1]));
       }
     }
     __syncthreads();
@@ -240,8 +246,8 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
   cp_async_wait_all();
 }
 
-// Second pass: a block adds up 32 experts of one sequence over the first pass's blocks that met it (8 warps side by
-// side, joined in order), and the last block of all adds up the loss.
+// Second pass: a block adds up 32 experts of one sequence over the first pass's blocks that met it (32 warps side
+// by side, joined in order), and the last block of all adds up the loss.
 __global__ void __launch_bounds__(bal::THREADS)
     balance_join_kernel(RouterRows in, BalanceScratch w, int chunk, float alpha, int* __restrict__ counts,
                         float* __restrict__ prob, int* __restrict__ rows, float* __restrict__ loss) {
@@ -259,12 +265,13 @@ __global__ void __launch_bounds__(bal::THREADS)
     s0 = max(lo, in.seq[b]);
     s1 = min(hi, in.seq[b + 1]);
   }
-  grid_wait_previous();  // the first pass's partial rows
+  grid_wait_previous();  // the first pass's partial rows (that pass lets this one start after its own wait: the offsets
+                         // above are there before)
   float p = 0.f;
   int c = 0, n = 0;
   if (s0 < s1) {
     const int i1 = (s1 - 1) / chunk;
-#pragma unroll 4
+#pragma unroll 5
     for (int i = s0 / chunk + warp; i <= i1; i += WARPS) {
       const long long slot = (long long)i + b;
       if (e < in.E) {
@@ -337,16 +344,18 @@ struct RouteBackward {
 
 // A block takes consecutive rows, a warp every sixteenth.  The coefficients f of the sequence that the block's first row
 // is in lie in shared memory; a block's few rows seldom leave it, and those that do read their counts.  The weight term
-// touches K experts of a row: it is spread through the row's own slot, whose logits are in registers by then.
+// touches K experts of a row: the lanes that hold the picks store those elements' sums after the row.
 template <int NV>
 __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
     route_backward_kernel(RouterRows in, RouteBackward q, int chunk) {
   using namespace bal;
-  constexpr int N = 4 * NV;
+  constexpr int N = 2 * NV;  // pairs of experts a lane
   constexpr int PER = (128 * NV + 32 * ROW_WARPS - 1) / (32 * ROW_WARPS);
   extern __shared__ __align__(16) float ring_smem[];
   float* s_f = ring_smem + ring_bytes(NV) / 4;  // [128 NV]
   __shared__ int s_full[ROW_WARPS];
+  grid_wait_previous();
+  grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r0 = blockIdx.x * chunk, r1 = min(in.T, r0 + chunk);
   RowRing<NV> ring;
@@ -366,8 +375,7 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
   if (balance) {
     int full = 0;
     for (int i = threadIdx.x; i < in.B; i += 32 * ROW_WARPS) full += q.rows[i] > 0;
-    full = __reduce_add_sync(0xffffffffu, full);
-    if (lane == 0) s_full[warp] = full;
+    const float dloss = q.dloss ? *q.dloss : 1.0f;
     block_b = seq_at(r0);
     int c[PER];
 #pragma unroll
@@ -376,7 +384,8 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
       c[i] = block_b >= 0 && e < in.E ? q.counts[(long long)block_b * in.E + e] : 0;
     }
     const int n = block_b >= 0 ? q.rows[block_b] : 0;
-    const float dloss = q.dloss ? *q.dloss : 1.0f;
+    full = __reduce_add_sync(0xffffffffu, full);
+    if (lane == 0) s_full[warp] = full;
     __syncthreads();
     full = 0;
     for (int k = 0; k < ROW_WARPS; ++k) full += s_full[k];
@@ -394,136 +403,115 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
   for (; t < r1; t += ROW_WARPS, ++at) {
     ring.fetch(in, at + slots(NV) - 1, ahead(slots(NV) - 1), balance, weights, q.dwts);
     ring.wait();
-    float* row = ring.slot(at);
-    // the lane's pick, its logit and the gradient of its weight
-    int e = -1;
-    float pick = 0.f, eg = 0.f;
-    if (weights && lane < in.K) {
-      e = reinterpret_cast<const int*>(row + 128 * NV)[lane];
-      if (e < 0 || e >= in.E) e = -1;
-      eg = row[128 * NV + PICKS + lane];
-      if (e >= 0) pick = balance ? row[e] : in.S[t * in.lds + e];
-    }
+    const float* row = ring.slot(at);
     const bool counted = balance && !(in.mask && in.mask[t] == 0);
     if (counted && t >= b_end) {
       b = seq_at(t);
       b_end = b < 0 ? t + 1 : in.seq ? in.seq[b + 1] : in.T;
     }
-    float d[N];
-    if (counted && b >= 0) {
-      float z = 0.f, m = 0.f, slope[N];
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const float4 v = *reinterpret_cast<const float4*>(row + (j * 32 + lane) * 4);
-        const float x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float u;
-          d[4 * j + i] = score_of(x[i], u);
-          slope[4 * j + i] = slope_of(d[4 * j + i], u);
-        }
-        z += (d[4 * j] + d[4 * j + 1]) + (d[4 * j + 2] + d[4 * j + 3]);
-      }
-      if (b == block_b) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          const float4 f = *reinterpret_cast<const float4*>(s_f + (j * 32 + lane) * 4);
-          m += (f.x * d[4 * j] + f.y * d[4 * j + 1]) + (f.z * d[4 * j + 2] + f.w * d[4 * j + 3]);
-          d[4 * j] = f.x;
-          d[4 * j + 1] = f.y;
-          d[4 * j + 2] = f.z;
-          d[4 * j + 3] = f.w;
-        }
-      } else {
+    u64 d[N];
+    float m = 0.f, inv = 0.f, k = 0.f;
+    const int* cb = nullptr;  // the counts of a sequence other than the block's first
+    const bool term = counted && b >= 0;
+    if (term) {
+      u64 z2 = f32x2(0.f, 0.f), m2 = z2, slope[N];
+      if (b != block_b) {
         const int n = q.rows[b];
-        const float k = n > 0 ? scale / (float)n / (float)n : 0.f;
-        const int* cb = q.counts + (long long)b * in.E;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int c = ((i >> 2) * 32 + lane) * 4 + (i & 3);
-          const float f = c < in.E ? k * (float)cb[c] : 0.f;
-          m += f * d[i];
-          d[i] = f;
-        }
+        k = n > 0 ? scale / (float)n / (float)n : 0.f;
+        cb = q.counts + (long long)b * in.E;
       }
-      z = warp_sum(z) + TINY;
-      const float inv = __frcp_rn(z);
-      m = warp_sum(m) * inv;
-#pragma unroll
-      for (int i = 0; i < N; ++i) d[i] = (d[i] - m) * (slope[i] * inv);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) d[i] = 0.f;
-    }
-    if (weights) {
-      float u, es = 0.f, slope = 0.f;
-      if (e >= 0) {
-        es = score_of(pick, u);
-        slope = slope_of(es, u);
-      } else {
-        eg = 0.f;
-      }
-      const float den = __frcp_rn(warp_sum(es) + TINY);
-      const float mean = warp_sum(eg * es) * den;
-      const float mine = rs * den * (eg - mean) * slope;
-      __syncwarp();  // the logits have been read: the slot turns into the row's weight term
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int c = (j * 32 + lane) * 4;
-        if (c + 4 <= in.E) {
-          *reinterpret_cast<float4*>(row + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(row + c);
+        const u64 e0 = exp_neg2(v.x), e1 = exp_neg2(v.y), s0 = score2(e0), s1 = score2(e1);
+        z2 = add_f32x2(z2, add_f32x2(s0, s1));
+        slope[2 * j] = slope2(s0, e0);
+        slope[2 * j + 1] = slope2(s1, e1);
+        ulonglong2 f;
+        if (cb == nullptr) {
+          f = *reinterpret_cast<const ulonglong2*>(s_f + c);
         } else {
+          float g[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (c + i < in.E) row[c + i] = 0.f;
+          for (int i = 0; i < 4; ++i) g[i] = c + i < in.E ? k * (float)cb[c + i] : 0.f;
+          f = make_ulonglong2(f32x2(g[0], g[1]), f32x2(g[2], g[3]));
+        }
+        m2 = fma_f32x2(f.x, s0, fma_f32x2(f.y, s1, m2));
+        d[2 * j] = f.x;
+        d[2 * j + 1] = f.y;
+      }
+      const float2 z = f32x2_get(z2), mm = f32x2_get(m2);
+      inv = rcp_ftz(warp_sum(z.x + z.y) + TINY);
+      m = warp_sum(mm.x + mm.y) * inv;
+      const u64 minus = f32x2(-m, -m), inv2 = f32x2(inv, inv);
+#pragma unroll
+      for (int i = 0; i < N; ++i) d[i] = mul_f32x2(add_f32x2(d[i], minus), mul_f32x2(slope[i], inv2));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) d[i] = 0ull;
+    }
+    // the lane's pick: its element's sum of both terms, stored over the balance term alone
+    int e = -1;
+    float total = 0.f;
+    if (weights) {
+      float x = 0.f, g = 0.f, f = 0.f;
+      if (lane < in.K) {
+        e = reinterpret_cast<const int*>(row + 128 * NV)[lane];
+        if (e < 0 || e >= in.E) e = -1;
+        if (e >= 0) {
+          x = balance ? row[e] : in.S[t * in.lds + e];
+          g = row[128 * NV + PICKS + lane];
+          f = !term ? 0.f : cb == nullptr ? s_f[e] : k * (float)cb[e];
         }
       }
-      __syncwarp();
+      const u64 ex = exp_neg2(f32x2(x, x)), sc = score2(ex);
+      const float s = e >= 0 ? f32x2_get(sc).x : 0.f, slope = f32x2_get(slope2(sc, ex)).x;
+      const float den = rcp_ftz(warp_sum(s) + TINY);
+      const float mean = warp_sum(g * s) * den;
+      const float mine = rs * den * (g - mean) * slope;
+      const float base = term ? (f - m) * (slope * inv) : 0.f;
+      total = base + mine;
       // an expert named twice gets both parts, added in pick order
       const u32 peers = __match_any_sync(0xffffffffu, e);
-      if (__all_sync(0xffffffffu, e < 0 || (peers & (peers - 1)) == 0)) {
-        if (e >= 0) row[e] = mine;
-      } else {
-        for (int k = 0; k < in.K; ++k) {
-          if (lane == k && e >= 0) row[e] += mine;
-          __syncwarp();
+      if (!__all_sync(0xffffffffu, e < 0 || (peers & (peers - 1)) == 0)) {
+        total = base;
+        for (int i = 0; i < in.K; ++i) {
+          const float other = __shfl_sync(0xffffffffu, mine, i);
+          if (peers >> i & 1) total += other;
         }
-      }
-      __syncwarp();
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const float4 a = *reinterpret_cast<const float4*>(row + (j * 32 + lane) * 4);
-        d[4 * j] += a.x;
-        d[4 * j + 1] += a.y;
-        d[4 * j + 2] += a.z;
-        d[4 * j + 3] += a.w;
       }
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * 32 + lane) * 4;
+      const float2 x = f32x2_get(d[2 * j]), y = f32x2_get(d[2 * j + 1]);
+      const float v[4] = {x.x, x.y, y.x, y.y};
       if (q.bf16_out) {
         bf16* o = reinterpret_cast<bf16*>(q.dS) + t * q.ldd + c;
         if (q.vec_out && c + 4 <= in.E) {
-          *reinterpret_cast<uint2*>(o) =
-              make_uint2(f2_to_bf16x2(d[4 * j], d[4 * j + 1]), f2_to_bf16x2(d[4 * j + 2], d[4 * j + 3]));
+          *reinterpret_cast<uint2*>(o) = make_uint2(f2_to_bf16x2(v[0], v[1]), f2_to_bf16x2(v[2], v[3]));
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (c + i < in.E) o[i] = __float2bfloat16_rn(d[4 * j + i]);
+            if (c + i < in.E) o[i] = __float2bfloat16_rn(v[i]);
         }
       } else {
         float* o = reinterpret_cast<float*>(q.dS) + t * q.ldd + c;
         if (q.vec_out && c + 4 <= in.E) {
-          *reinterpret_cast<float4*>(o) = make_float4(d[4 * j], d[4 * j + 1], d[4 * j + 2], d[4 * j + 3]);
+          *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (c + i < in.E) o[i] = d[4 * j + i];
+            if (c + i < in.E) o[i] = v[i];
         }
       }
     }
-    __syncwarp();  // every lane has read the slot that the next fetch fills
+    __syncwarp();  // the row's stores are ordered before the picks', and its slot has been read
+    if (e >= 0) {
+      if (q.bf16_out) reinterpret_cast<bf16*>(q.dS)[t * q.ldd + e] = __float2bfloat16_rn(total);
+      else reinterpret_cast<float*>(q.dS)[t * q.ldd + e] = total;
+    }
   }
   cp_async_wait_all();
 }

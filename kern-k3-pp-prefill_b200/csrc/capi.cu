@@ -112,6 +112,29 @@ unsigned long long* g_trace = nullptr;  // k3moe_set_trace
 
 int launch_status() { return cudaGetLastError() == cudaSuccess ? K3MOE_OK : K3MOE_ELAUNCH; }
 
+// A launch whose prologue may overlap the end of the kernel before it on the stream; the kernel waits for that one
+// (grid_wait_previous) before it touches global memory.  cluster: blocks of a cluster (1: none).
+template <typename... P, typename... A>
+int launch_overlapped(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t s, unsigned cluster,
+                      A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, P(args)...) == cudaSuccess) return K3MOE_OK;
+  cudaGetLastError();
+  return K3MOE_ELAUNCH;
+}
+
 inline long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
@@ -309,8 +332,7 @@ int launch_quant_int8(const QuantRows& p, cudaStream_t s) {
   const int threads = LANES > 32 ? LANES : 256;
   const long long blocks = cdiv(p.rows, threads / LANES);
   const int grid = (int)std::min<long long>(blocks, (long long)num_sms(current_device()) * MINB);
-  quant_int8_kernel<SRC, LANES, NV, MINB><<<grid, threads, 0, s>>>(p);
-  return launch_status();
+  return launch_overlapped(quant_int8_kernel<SRC, LANES, NV, MINB>, grid, threads, 0, s, 1, p);
 }
 
 // a warp a row up to 1024 columns, then a block; rows of up to 16384 columns stay in registers
@@ -361,26 +383,8 @@ int int8_launch(const int8_t* q, long long q_rows, long long ldq, const int8_t* 
   if (!(f32 ? set_smem_once(int8_gemm_kernel<float>, i8::SMEM_BYTES, 4)
             : set_smem_once(int8_gemm_kernel<bf16>, i8::SMEM_BYTES, 5)))
     return K3MOE_ELAUNCH;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(i8::THREADS);
-  cfg.dynamicSmemBytes = i8::SMEM_BYTES;
-  cfg.stream = s;
-  // the prologue overlaps the end of the kernel before (usually the quantiser)
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)p.splits;
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.splits > 1 ? 2 : 1;
-  if ((f32 ? cudaLaunchKernelEx(&cfg, int8_gemm_kernel<float>, tw, tx, p)
-           : cudaLaunchKernelEx(&cfg, int8_gemm_kernel<bf16>, tw, tx, p)) != cudaSuccess) {
-    cudaGetLastError();
-    return K3MOE_ELAUNCH;
-  }
-  return launch_status();
+  return launch_overlapped(f32 ? int8_gemm_kernel<float> : int8_gemm_kernel<bf16>, grid, i8::THREADS, i8::SMEM_BYTES, s,
+                           p.splits, tw, tx, p);
 }
 
 }  // namespace
@@ -586,28 +590,16 @@ int k3moe_balance_loss(const float* S, int lds, const int32_t* idx, int T, int E
   w.done = reinterpret_cast<u32*>(ws + L.done);
   const RouterRows in = router_rows(S, lds, idx, T, E, K, seq, B, mask);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  bool ready = false;
+  int rc = K3MOE_ELAUNCH;
   by_experts(E, [&](auto nv) {
     constexpr int NV = decltype(nv)::value, bytes = bal::rows_smem(NV);
-    ready = set_smem_once(balance_rows_kernel<NV>, bytes, 5 + NV);
-    if (ready) balance_rows_kernel<NV><<<L.blocks, 32 * bal::ROW_WARPS, bytes, s>>>(in, w, L.chunk);
+    if (set_smem_once(balance_rows_kernel<NV>, bytes, 5 + NV))
+      rc = launch_overlapped(balance_rows_kernel<NV>, L.blocks, 32 * bal::ROW_WARPS, bytes, s, 1, in, w, L.chunk);
   });
-  if (!ready) return K3MOE_ELAUNCH;
+  if (rc) return rc;
   const long long blocks = (long long)B * cdiv(E, bal::COLS);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(bal::THREADS);
-  cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, balance_join_kernel, in, w, L.chunk, alpha, counts, prob, rows, loss) != cudaSuccess) {
-    cudaGetLastError();
-    return K3MOE_ELAUNCH;
-  }
-  return launch_status();
+  return launch_overlapped(balance_join_kernel, (unsigned)blocks, bal::THREADS, 0, s, 1, in, w, L.chunk, alpha, counts,
+                           prob, rows, loss);
 }
 
 int k3moe_route_backward(const float* S, int lds, const int32_t* idx, int T, int E, int K, const int32_t* seq, int B,
@@ -631,16 +623,14 @@ int k3moe_route_backward(const float* S, int lds, const int32_t* idx, int T, int
   q.bf16_out = dtype == K3MOE_BF16;
   q.vec_out = ldd % 4 == 0 && reinterpret_cast<uintptr_t>(dS) % (q.bf16_out ? 8 : 16) == 0;
   const int chunk = router_chunk(T, E), grid = (int)cdiv(T, chunk);
-  bool ready = false;
+  int rc = K3MOE_ELAUNCH;
   by_experts(E, [&](auto nv) {
     constexpr int NV = decltype(nv)::value, bytes = bal::grad_smem(NV);
-    ready = set_smem_once(route_backward_kernel<NV>, bytes, 13 + NV);
-    if (ready)
-      route_backward_kernel<NV>
-          <<<grid, 32 * bal::ROW_WARPS, bytes, reinterpret_cast<cudaStream_t>(stream)>>>(in, q, chunk);
+    if (set_smem_once(route_backward_kernel<NV>, bytes, 13 + NV))
+      rc = launch_overlapped(route_backward_kernel<NV>, grid, 32 * bal::ROW_WARPS, bytes,
+                             reinterpret_cast<cudaStream_t>(stream), 1, in, q, chunk);
   });
-  if (!ready) return K3MOE_ELAUNCH;
-  return launch_status();
+  return rc;
 }
 
 // ---------------------------------------------------------------- products in 8-bit integers

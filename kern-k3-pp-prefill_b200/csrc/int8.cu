@@ -12,12 +12,11 @@ namespace k3 {
 // ============================================================ quantiser
 // amax = the row's largest magnitude, scale = amax / 127, q = round-half-even(127 x / amax): the rounding of the real
 // quotient, not of a float product.
-// bf16: with inv = 127 / amax rounded up and down, one FMA each (1.5 * 2^23 + x inv) rounds the quotient seen from either
-// side.  The quotient of two 8-bit mantissas is a half exactly or at least 2^-9 |q| / 256 from one, far more than the 2^-23
-// |q| that inv is off by, so the two integers are equal, or the neighbours of an exact half: then the even one is it, bit
-// arithmetic on pairs, no branch (ties are common: rows whose maximum has few mantissa bits have them by the hundred, and
-// a branch for them took 30% of the kernel's instructions).  The gate's values are rounded themselves, so the same rule
-// serves there, a quotient within 2^-15 of a half taken as one.
+// bf16: with 127 / amax bracketed, 2^-21 of it above and below, one FMA each (1.5 * 2^23 + x inv) rounds the quotient seen
+// from either side.  The quotient of two 8-bit mantissas is a half exactly or at least 2^-17 of itself from one, so the two
+// integers are equal, or the neighbours of an exact half: then the even one is it, bit arithmetic on pairs, no branch (ties
+// are common: rows whose maximum has few mantissa bits have them by the hundred).  The gate's values are rounded
+// themselves, so the same rule serves there, a quotient within 2^-13 of a half taken as one.
 // f32: one FMA, and the elements whose x inv is within 1e-5 of a half (inv moves the quotient by 7.6e-6 at most) compare
 // 254 |x| with (2k + 1) amax, both exact in double.
 // A row with an infinity or a NaN has scale NaN and q = 0, so every result it enters is NaN; a zero row scale 0, q = 0.
@@ -120,24 +119,21 @@ __device__ __forceinline__ u32 max_bits(u32 m, const Kept<SRC>& v) {
 }
 
 struct RowScale {
-  float amax, pre, inv, up, down, scale;  // pre: a power of two that keeps 127 / amax finite
+  float amax, pre, inv;  // pre: a power of two that keeps 127 / amax finite; inv 0: a row of zeros, or with no number
 };
+template <int SRC>
 __device__ __forceinline__ RowScale row_scale(u32 amax_bits) {
   RowScale s;
   s.amax = __uint_as_float(amax_bits);
-  if (amax_bits >= 0x7f800000u) {
-    s.pre = s.inv = s.up = s.down = 0.f;
-    s.scale = __uint_as_float(0x7fc00000u);
-  } else if (amax_bits == 0u) {
-    s.pre = s.inv = s.up = s.down = s.scale = 0.f;
-  } else {
+  s.pre = s.inv = 0.f;
+  if (amax_bits < 0x7f800000u && amax_bits != 0u) {
     s.pre = s.amax < 0x1p-60f ? 0x1p64f : s.amax > 0x1p60f ? 0x1p-64f : 1.f;
-    s.inv = __fdiv_rn(127.f, s.amax * s.pre);
-    s.up = __fdiv_ru(127.f, s.amax * s.pre);
-    s.down = __fdiv_rd(127.f, s.amax * s.pre);
-    s.scale = __fdiv_rn(s.amax, 127.f);
+    s.inv = SRC == I8_F32 ? __fdiv_rn(127.f, s.amax * s.pre) : 127.f * rcp_ftz(s.amax * s.pre);
   }
   return s;
+}
+__device__ __forceinline__ float scale_of(const RowScale& s) {
+  return __float_as_uint(s.amax) >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __fdiv_rn(s.amax, 127.f);
 }
 
 // the code of an element whose quotient lies near k + 1/2 in magnitude
@@ -152,7 +148,8 @@ __device__ __forceinline__ uint2 encode8(const RowScale& s, const Kept<SRC>& v) 
   if (s.inv == 0.f) return make_uint2(0u, 0u);
   if (SRC != I8_F32) {
     constexpr float ROUND = 12582912.f + 256.f;  // the integer, plus 256, in the low 16 bits
-    const u64 up = f32x2(s.up, s.up), down = f32x2(s.down, s.down), round = f32x2(ROUND, ROUND);
+    const float above = s.inv * (1.f + 0x1p-21f), below = s.inv * (1.f - 0x1p-21f);
+    const u64 up = f32x2(above, above), down = f32x2(below, below), round = f32x2(ROUND, ROUND);
     u32 k[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -210,6 +207,7 @@ __global__ void __launch_bounds__(LANES > 32 ? LANES : 256, MINB) quant_int8_ker
   constexpr int PER = LANES > 32 ? 1 : 8;
   constexpr int STEP = LANES * 8;
   const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
+  grid_wait_previous();
   grid_launch_dependents();
   const int nne = p.cta_limit ? min(p.meta[0], p.max_ctas) : 0;
   const int shared_row = p.exp2perm ? p.meta[2] : -1;
@@ -253,7 +251,7 @@ __global__ void __launch_bounds__(LANES > 32 ? LANES : 256, MINB) quant_int8_ker
       for (int i = 0; i < LANES / 32; ++i) m = max(m, s_max[buf][i]);
       buf ^= 1;  // the next row's maxima go to the other half: one barrier a row
     }
-    const RowScale s = row_scale(m);
+    const RowScale s = row_scale<SRC>(m);
     if (NV > 0) {
       if (!p.exp2perm) {
         int8_t* dst = p.q + r * p.ldq;
@@ -262,7 +260,7 @@ __global__ void __launch_bounds__(LANES > 32 ? LANES : 256, MINB) quant_int8_ker
           const int c = j * STEP + lane * 8;
           if (c < p.cols) put8(dst + c, p.cols - c, encode8<SRC>(s, v[j]));
         }
-        if (lane == 0) p.scale[r] = s.scale;
+        if (lane == 0) p.scale[r] = scale_of(s);
         continue;
       }
 #pragma unroll
@@ -289,7 +287,7 @@ __global__ void __launch_bounds__(LANES > 32 ? LANES : 256, MINB) quant_int8_ker
           put8(dst + c, p.cols - c, encode8<SRC>(s, v[0]));
         }
       }
-      if (lane == 0) p.scale[o] = s.scale;
+      if (lane == 0) p.scale[o] = scale_of(s);
     }
   }
 }

@@ -10,7 +10,6 @@ exception is raised.
 from __future__ import annotations
 
 import ctypes
-import functools
 import os
 from dataclasses import dataclass
 
@@ -399,17 +398,6 @@ def _launch(fn, what: str, dev, *args) -> None:
         _check(rc, what)
 
 
-def _on_stream(f):
-    """The `stream` argument of the entries below: the call, its allocations included, on that stream."""
-    @functools.wraps(f)
-    def call(*args, stream=None, **kw):
-        if stream is None:
-            return f(*args, **kw)
-        with torch.cuda.stream(stream):
-            return f(*args, **kw)
-    return call
-
-
 def _out_dtype(dtype) -> int:
     if dtype is torch.bfloat16:
         return BF16
@@ -418,6 +406,7 @@ def _out_dtype(dtype) -> int:
     raise K3MoeError(f"dtype {dtype} (torch.bfloat16 or torch.float32 is needed)")
 
 
+_empty = torch.empty
 _I8, _I32, _F32, _BF16 = (torch.int8,), (torch.int32,), (torch.float32,), (torch.bfloat16,)
 _FLOATS, _FLAGS, _WORDS = (torch.bfloat16, torch.float32), (torch.uint8, torch.bool), (torch.int32, torch.uint32)
 BF16, F32 = 0, 1  # include/k3moe.h K3MOE_BF16, K3MOE_F32
@@ -449,34 +438,38 @@ def _router_args(S, idx, seq, mask):
     return dev, T, E, idx.shape[1], B, ld
 
 
-@_on_stream
 def balance_loss(S: torch.Tensor, idx: torch.Tensor, alpha: float, seq: torch.Tensor | None = None,
-                 mask: torch.Tensor | None = None) -> BalanceStats:
+                 mask: torch.Tensor | None = None, stream=None) -> BalanceStats:
     """The router's load-balance loss over the top-k's picks, and its counts (k3moe_balance_loss).
 
     S f32 [T, E] router logits; idx int32 [T, K] (route_topk's); seq int32 [B + 1] offsets of packed sequences (None:
     one sequence); mask [T] uint8 or bool, rows with 0 are not counted."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return balance_loss(S, idx, alpha, seq, mask)
     dev, T, E, K, B, ld = _router_args(S, idx, seq, mask)
     L = lib()
-    scratch = S.new_empty(-(-L.k3moe_balance_scratch_bytes(T, E, B) // 4))
-    prob = S.new_empty((B, E))
-    counts = idx.new_empty((B, E))
-    rows = idx.new_empty(B)
-    loss = S.new_empty(1)
+    scratch = _empty(L.k3moe_balance_scratch_bytes(T, E, B), dtype=torch.uint8, device=dev)
+    prob = _empty(B, E, dtype=torch.float32, device=dev)
+    counts = _empty(B, E, dtype=torch.int32, device=dev)
+    rows = _empty(B, dtype=torch.int32, device=dev)
+    loss = _empty(1, dtype=torch.float32, device=dev)
     _launch(L.k3moe_balance_loss, "balance_loss", dev, S.data_ptr(), ld, idx.data_ptr(), T, E, K, _p(seq), B, _p(mask),
             alpha, scratch.data_ptr(), counts.data_ptr(), prob.data_ptr(), rows.data_ptr(), loss.data_ptr())
     return BalanceStats(loss, counts, prob, rows)
 
 
-@_on_stream
 def route_backward(S: torch.Tensor, idx: torch.Tensor, alpha: float = 0.0, counts: torch.Tensor | None = None,
                    rows: torch.Tensor | None = None, dloss: torch.Tensor | None = None,
                    dwts: torch.Tensor | None = None, rs: torch.Tensor | None = None, seq: torch.Tensor | None = None,
                    mask: torch.Tensor | None = None, dtype: torch.dtype = torch.float32,
-                   out: torch.Tensor | None = None) -> torch.Tensor:
+                   out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """dS [T, E] (k3moe_route_backward): the balance term where counts and rows (balance_loss's, with its alpha, seq
     and mask) are given, dloss its scalar gradient (None: 1); plus the weight term where dwts [T, K], the gradient of
     route_topk's weights, and rs are given."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return route_backward(S, idx, alpha, counts, rows, dloss, dwts, rs, seq, mask, dtype, out)
     dev, T, E, K, B, ld = _router_args(S, idx, seq, mask)
     if counts is not None and rows is not None:
         _vec(counts, "counts", _I32, B * E, dev)
@@ -491,7 +484,7 @@ def route_backward(S: torch.Tensor, idx: torch.Tensor, alpha: float = 0.0, count
         _vec(rs, "rs", _BF16, 1, dev)
     if out is None:
         code, ldd = _out_dtype(dtype), E
-        out = S.new_empty((T, E), dtype=dtype)
+        out = _empty(T, E, dtype=dtype, device=dev)
     else:
         code, ldd = _out_dtype(out.dtype), _rows(out, "out", _FLOATS, dev, E, T)
     _launch(lib().k3moe_route_backward, "route_backward", dev, S.data_ptr(), ld, idx.data_ptr(), T, E, K, _p(seq), B,
@@ -500,35 +493,39 @@ def route_backward(S: torch.Tensor, idx: torch.Tensor, alpha: float = 0.0, count
 
 
 # ------------------------------------------------------------------ products in 8-bit integers
-def _int8_out(x, rows: int, cols: int, dev, out):
+def _int8_out(rows: int, cols: int, dev, out):
     if out is None:
         ld = -(-cols // 16) * 16
-        q = x.new_empty((rows, ld), dtype=torch.int8)
-        return q if ld == cols else q[:, :cols], ld, x.new_empty(rows, dtype=torch.float32)
+        q = _empty(rows, ld, dtype=torch.int8, device=dev)
+        return q if ld == cols else q[:, :cols], ld, _empty(rows, dtype=torch.float32, device=dev)
     q, scale = out
     ld = _int8_rows(q, "out q", dev, cols, rows)
     _vec(scale, "out scale", _F32, rows, dev)
     return q, ld, scale
 
 
-@_on_stream
-def quant_int8(x: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None):
+def quant_int8(x: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None, stream=None):
     """Rows of x (bf16 or f32 [rows, cols]; tokens, or a weight's channels) to int8 with a scale each
     (k3moe_quant_int8): (q int8 [rows, cols], its rows padded to 16 bytes; scale f32 [rows])."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return quant_int8(x, out)
     ldx = _rows(x, "x", _FLOATS)
     rows, cols = x.shape
     dev = x.device
-    q, ldq, scale = _int8_out(x, rows, cols, dev, out)
+    q, ldq, scale = _int8_out(rows, cols, dev, out)
     _launch(lib().k3moe_quant_int8, "quant_int8", dev, x.data_ptr(), _out_dtype(x.dtype), ldx, rows, cols, q.data_ptr(),
             ldq, scale.data_ptr())
     return q, scale
 
 
-@_on_stream
 def act_quant_int8(gu: torch.Tensor, activation: int = ACT_SWIGLU, tables: Tables | None = None,
-                   out: tuple[torch.Tensor, torch.Tensor] | None = None):
+                   out: tuple[torch.Tensor, torch.Tensor] | None = None, stream=None):
     """act(gate) * up of bf16 rows [gate | up] to int8 (k3moe_act_quant_int8): (q [rows, cols / 2], scale).  With
     tables, gu is [cap_rows, 2I] and only the tables' real rows are read and written."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return act_quant_int8(gu, activation, tables, out)
     ldg = _rows(gu, "gu", _BF16)
     rows, cols = gu.shape
     dev = gu.device
@@ -541,23 +538,25 @@ def act_quant_int8(gu: torch.Tensor, activation: int = ACT_SWIGLU, tables: Table
         _need(rows <= ctas * 128, f"gu: {rows} rows, the tables cover {ctas * 128}")
         _vec(limit, "tables.cta_limit", _I32, ctas, dev)
         _vec(meta, "tables.meta", _I32, None, dev)
-    q, ldq, scale = _int8_out(gu, rows, cols // 2, dev, out)
+    q, ldq, scale = _int8_out(rows, cols // 2, dev, out)
     _launch(lib().k3moe_act_quant_int8, "act_quant_int8", dev, gu.data_ptr(), ldg, rows, cols // 2, activation,
             _p(limit), _p(meta), ctas, q.data_ptr(), ldq, scale.data_ptr())
     return q, scale
 
 
-@_on_stream
-def quant_int8_permute(x: torch.Tensor, tables: Tables, out: tuple[torch.Tensor, torch.Tensor] | None = None):
+def quant_int8_permute(x: torch.Tensor, tables: Tables, out: tuple[torch.Tensor, torch.Tensor] | None = None, stream=None):
     """quant_int8 of bf16 rows, each written to every permuted row it is routed to (k3moe_quant_int8_permute):
     (q [cap_rows, cols], scale [cap_rows]); padding rows are not written."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return quant_int8_permute(x, tables, out)
     ldx = _rows(x, "x", _BF16)
     R, cols = x.shape
     dev, e2p, cap = x.device, tables.exp2perm, tables.cap_rows
     K = e2p.shape[1]
     _vec(e2p, "tables.exp2perm", _I32, R * K, dev)
     _vec(tables.meta, "tables.meta", _I32, None, dev)
-    q, ldq, scale = _int8_out(x, cap, cols, dev, out)
+    q, ldq, scale = _int8_out(cap, cols, dev, out)
     _launch(lib().k3moe_quant_int8_permute, "quant_int8_permute", dev, x.data_ptr(), ldx, R, cols, K, e2p.data_ptr(),
             tables.meta.data_ptr(), q.data_ptr(), ldq, scale.data_ptr(), cap)
     return q, scale
@@ -575,33 +574,37 @@ def _product_args(q, sx, w, sw, err):
     return dev, T, C, ldq, ldw
 
 
-def _product_out(sx, T, N, dtype, dev, out):
+def _product_out(T, N, dtype, dev, out):
     if out is None:
         code = _out_dtype(dtype)
-        return sx.new_empty((T, N), dtype=dtype), N, code
+        return _empty(T, N, dtype=dtype, device=dev), N, code
     return out, _rows(out, "out", _FLOATS, dev, N, T), _out_dtype(out.dtype)
 
 
-@_on_stream
 def gemm_int8(q: torch.Tensor, sx: torch.Tensor, w: torch.Tensor, sw: torch.Tensor,
               dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
-              err: torch.Tensor | None = None) -> torch.Tensor:
+              err: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """out[t, n] = sx[t] sw[n] (q[t] . w[n]) (k3moe_gemm_int8): q int8 [T, C], w int8 [N, C], rows 16-byte aligned as
     quant_int8 gives them; out [T, N] bf16 or f32.  err: the device error words, or None."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return gemm_int8(q, sx, w, sw, dtype, out, err)
     dev, T, C, ldq, ldw = _product_args(q, sx, w, sw, err)
     N = w.shape[0]
-    out, ldo, code = _product_out(sx, T, N, dtype, dev, out)
+    out, ldo, code = _product_out(T, N, dtype, dev, out)
     _launch(lib().k3moe_gemm_int8, "gemm_int8", dev, q.data_ptr(), ldq, sx.data_ptr(), w.data_ptr(), ldw, sw.data_ptr(),
             T, N, C, out.data_ptr(), ldo, code, _p(err))
     return out
 
 
-@_on_stream
 def grouped_gemm_int8(q: torch.Tensor, sx: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, tables: Tables,
                       n_experts: int, dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
-                      err: torch.Tensor | None = None) -> torch.Tensor:
+                      err: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """The products of routed rows with their experts' weights (k3moe_grouped_gemm_int8): q int8 [cap_rows, C] permuted
     rows, w int8 [n_experts * N, C], out [cap_rows, N]; padding rows of out are not written."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return grouped_gemm_int8(q, sx, w, sw, tables, n_experts, dtype, out, err)
     dev, cap, C, ldq, ldw = _product_args(q, sx, w, sw, err)
     ctas = tables.max_ctas
     if n_experts < 1 or w.shape[0] % n_experts or cap != tables.cap_rows:
@@ -610,7 +613,7 @@ def grouped_gemm_int8(q: torch.Tensor, sx: torch.Tensor, w: torch.Tensor, sw: to
     _vec(tables.cta_limit, "tables.cta_limit", _I32, ctas, dev)
     _vec(tables.meta, "tables.meta", _I32, None, dev)
     N = w.shape[0] // n_experts
-    out, ldo, code = _product_out(sx, cap, N, dtype, dev, out)
+    out, ldo, code = _product_out(cap, N, dtype, dev, out)
     _launch(lib().k3moe_grouped_gemm_int8, "grouped_gemm_int8", dev, q.data_ptr(), ldq, sx.data_ptr(), w.data_ptr(), ldw,
             sw.data_ptr(), tables.cta_batch.data_ptr(), tables.cta_limit.data_ptr(), tables.meta.data_ptr(), N, C,
             n_experts, cap, ctas, out.data_ptr(), ldo, code, _p(err))
