@@ -19,8 +19,7 @@
 namespace k3 {
 
 namespace bal {
-constexpr int WARPS = 32;        // of a block of the join
-constexpr int THREADS = 32 * WARPS;
+constexpr int JOIN_WARPS = 32;   // of a block of the join, at most
 constexpr int ROW_WARPS = 16;    // of a block that walks rows
 constexpr int PICKS = 16;        // K at most
 // Row slots a warp: as many as fit, four at most.  One block an SM where a row is long, two where it is short.
@@ -29,7 +28,7 @@ __host__ __device__ constexpr int blocks_per_sm(int nv) { return nv <= 2 ? 2 : 1
 __host__ __device__ constexpr int slot_floats(int nv) { return 128 * nv + 2 * PICKS; }
 __host__ __device__ constexpr int ring_bytes(int nv) { return ROW_WARPS * slots(nv) * slot_floats(nv) * 4; }
 __host__ __device__ constexpr int rows_smem(int nv) { return ring_bytes(nv) + (ROW_WARPS / 2) * 128 * nv * 4 + 128 * nv * 4; }
-__host__ __device__ constexpr int grad_smem(int nv) { return ring_bytes(nv) + 128 * nv * 4; }
+__host__ __device__ constexpr int grad_smem(int nv) { return ring_bytes(nv) + 2 * 128 * nv * 4; }
 constexpr float TINY = 1e-20f;  // the top-k's guard of its own sum
 constexpr int COLS = 32;        // experts a block of the second pass
 }  // namespace bal
@@ -246,14 +245,15 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
   cp_async_wait_all();
 }
 
-// Second pass: a block adds up 32 experts of one sequence over the first pass's blocks that met it (32 warps side
+// Second pass: a block adds up 32 experts of one sequence over the first pass's blocks that met it (its warps side
 // by side, joined in order), and the last block of all adds up the loss.
-__global__ void __launch_bounds__(bal::THREADS)
+__global__ void __launch_bounds__(32 * bal::JOIN_WARPS)
     balance_join_kernel(RouterRows in, BalanceScratch w, int chunk, float alpha, int* __restrict__ counts,
                         float* __restrict__ prob, int* __restrict__ rows, float* __restrict__ loss) {
   using namespace bal;
-  __shared__ float s_p[WARPS][COLS];
-  __shared__ int s_c[WARPS][COLS], s_n[WARPS];
+  const int warps = blockDim.x >> 5;
+  __shared__ float s_p[JOIN_WARPS][COLS];
+  __shared__ int s_c[JOIN_WARPS][COLS], s_n[JOIN_WARPS];
   __shared__ int s_last;
   const int groups = (in.E + COLS - 1) / COLS;
   const int b = blockIdx.x / groups, g = blockIdx.x % groups;
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(bal::THREADS)
   if (s0 < s1) {
     const int i1 = (s1 - 1) / chunk;
 #pragma unroll 5
-    for (int i = s0 / chunk + warp; i <= i1; i += WARPS) {
+    for (int i = s0 / chunk + warp; i <= i1; i += warps) {
       const long long slot = (long long)i + b;
       if (e < in.E) {
         p += w.prob[slot * in.E + e];
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(bal::THREADS)
   if (lane == 0) s_n[warp] = n;
   __syncthreads();
   if (warp == 0) {
-    for (int k = 1; k < WARPS; ++k) {
+    for (int k = 1; k < warps; ++k) {
       p += s_p[k][lane];
       c += s_c[k][lane];
       n += s_n[k];
@@ -310,8 +310,8 @@ __global__ void __launch_bounds__(bal::THREADS)
   __threadfence();
   float sum = 0.f;
   int full = 0;
-  for (long long i = threadIdx.x; i < (long long)gridDim.x; i += THREADS) sum += __ldcg(&w.term[i]);
-  for (int i = threadIdx.x; i < in.B; i += THREADS) full += __ldcg(&rows[i]) > 0;
+  for (long long i = threadIdx.x; i < (long long)gridDim.x; i += blockDim.x) sum += __ldcg(&w.term[i]);
+  for (int i = threadIdx.x; i < in.B; i += blockDim.x) full += __ldcg(&rows[i]) > 0;
   sum = warp_sum(sum);
   full = __reduce_add_sync(0xffffffffu, full);
   if (lane == 0) {
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(bal::THREADS)
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int k = 1; k < WARPS; ++k) {
+    for (int k = 1; k < warps; ++k) {
       sum += s_p[k][0];
       full += s_c[k][0];
     }
@@ -342,8 +342,8 @@ struct RouteBackward {
   int vec_out;          // rows may be stored 4 elements at a time
 };
 
-// A block takes consecutive rows, a warp every sixteenth.  The coefficients f of the sequence that the block's first row
-// is in lie in shared memory; a block's few rows seldom leave it, and those that do read their counts.  The weight term
+// A block takes consecutive rows, a warp every sixteenth.  The coefficients f of the sequences that the block's first and
+// last rows are in lie in shared memory; rows of others, where sequences are short, read their counts.  The weight term
 // touches K experts of a row: the lanes that hold the picks store those elements' sums after the row.
 template <int NV>
 __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
   constexpr int N = 2 * NV;  // pairs of experts a lane
   constexpr int PER = (128 * NV + 32 * ROW_WARPS - 1) / (32 * ROW_WARPS);
   extern __shared__ __align__(16) float ring_smem[];
-  float* s_f = ring_smem + ring_bytes(NV) / 4;  // [128 NV]
+  float* s_f = ring_smem + ring_bytes(NV) / 4;  // [2][128 NV]
   __shared__ int s_full[ROW_WARPS];
   grid_wait_previous();
   grid_launch_dependents();
@@ -370,31 +370,36 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
   // the sequence of row t, or -1
   const int lo = in.seq ? in.seq[0] : 0, hi = in.seq ? in.seq[in.B] : in.T;
   auto seq_at = [&](int t) { return t < lo || t >= hi ? -1 : in.seq ? seq_of(in.seq, in.B, t, lane) : 0; };
-  int block_b = -1;
+  int b0 = -1, b1 = -1;
   float scale = 0.f;  // alpha dloss E / (B' K)
   if (balance) {
     int full = 0;
     for (int i = threadIdx.x; i < in.B; i += 32 * ROW_WARPS) full += q.rows[i] > 0;
     const float dloss = q.dloss ? *q.dloss : 1.0f;
-    block_b = seq_at(r0);
-    int c[PER];
+    b0 = seq_at(r0);
+    b1 = seq_at(r1 - 1);
+    int c0[PER], c1[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int e = i * 32 * ROW_WARPS + threadIdx.x;
-      c[i] = block_b >= 0 && e < in.E ? q.counts[(long long)block_b * in.E + e] : 0;
+      c0[i] = b0 >= 0 && e < in.E ? q.counts[(long long)b0 * in.E + e] : 0;
+      c1[i] = b1 >= 0 && e < in.E ? q.counts[(long long)b1 * in.E + e] : 0;
     }
-    const int n = block_b >= 0 ? q.rows[block_b] : 0;
+    const int n0 = b0 >= 0 ? q.rows[b0] : 0, n1 = b1 >= 0 ? q.rows[b1] : 0;
     full = __reduce_add_sync(0xffffffffu, full);
     if (lane == 0) s_full[warp] = full;
     __syncthreads();
     full = 0;
     for (int k = 0; k < ROW_WARPS; ++k) full += s_full[k];
     scale = q.alpha * dloss * ((float)in.E / ((float)max(full, 1) * (float)in.K));
-    const float k = n > 0 ? scale / (float)n / (float)n : 0.f;
+    const float k0 = n0 > 0 ? scale / (float)n0 / (float)n0 : 0.f, k1 = n1 > 0 ? scale / (float)n1 / (float)n1 : 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int e = i * 32 * ROW_WARPS + threadIdx.x;
-      if (e < 128 * NV) s_f[e] = k * (float)c[i];
+      if (e < 128 * NV) {
+        s_f[e] = k0 * (float)c0[i];
+        s_f[128 * NV + e] = k1 * (float)c1[i];
+      }
     }
     __syncthreads();
   }
@@ -411,11 +416,12 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
     }
     u64 d[N];
     float m = 0.f, inv = 0.f, k = 0.f;
-    const int* cb = nullptr;  // the counts of a sequence other than the block's first
+    const int* cb = nullptr;  // the counts of a sequence other than the block's first and last
+    const float* sf = b == b0 ? s_f : s_f + 128 * NV;
     const bool term = counted && b >= 0;
     if (term) {
       u64 z2 = f32x2(0.f, 0.f), m2 = z2, slope[N];
-      if (b != block_b) {
+      if (b != b0 && b != b1) {
         const int n = q.rows[b];
         k = n > 0 ? scale / (float)n / (float)n : 0.f;
         cb = q.counts + (long long)b * in.E;
@@ -430,7 +436,7 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
         slope[2 * j + 1] = slope2(s1, e1);
         ulonglong2 f;
         if (cb == nullptr) {
-          f = *reinterpret_cast<const ulonglong2*>(s_f + c);
+          f = *reinterpret_cast<const ulonglong2*>(sf + c);
         } else {
           float g[4];
 #pragma unroll
@@ -462,7 +468,7 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
         if (e >= 0) {
           x = balance ? row[e] : in.S[t * in.lds + e];
           g = row[128 * NV + PICKS + lane];
-          f = !term ? 0.f : cb == nullptr ? s_f[e] : k * (float)cb[e];
+          f = !term ? 0.f : cb == nullptr ? sf[e] : k * (float)cb[e];
         }
       }
       const u64 ex = exp_neg2(f32x2(x, x)), sc = score2(ex);

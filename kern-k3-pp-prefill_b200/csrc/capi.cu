@@ -332,7 +332,9 @@ int launch_quant_int8(const QuantRows& p, cudaStream_t s) {
   const int threads = LANES > 32 ? LANES : 256;
   const long long blocks = cdiv(p.rows, threads / LANES);
   const int grid = (int)std::min<long long>(blocks, (long long)num_sms(current_device()) * MINB);
-  return launch_overlapped(quant_int8_kernel<SRC, LANES, NV, MINB>, grid, threads, 0, s, 1, p);
+  return launch_overlapped(p.vec && p.cols % 8 == 0 ? quant_int8_kernel<SRC, LANES, NV, MINB, true>
+                                                    : quant_int8_kernel<SRC, LANES, NV, MINB, false>,
+                           grid, threads, 0, s, 1, p);
 }
 
 // a warp a row up to 1024 columns, then a block; rows of up to 16384 columns stay in registers
@@ -598,7 +600,9 @@ int k3moe_balance_loss(const float* S, int lds, const int32_t* idx, int T, int E
   });
   if (rc) return rc;
   const long long blocks = (long long)B * cdiv(E, bal::COLS);
-  return launch_overlapped(balance_join_kernel, (unsigned)blocks, bal::THREADS, 0, s, 1, in, w, L.chunk, alpha, counts,
+  // a warp a partial row of the average sequence
+  const int warps = (int)std::min<long long>(bal::JOIN_WARPS, cdiv(cdiv(L.blocks, B) + 1, 4) * 4);
+  return launch_overlapped(balance_join_kernel, (unsigned)blocks, 32 * warps, 0, s, 1, in, w, L.chunk, alpha, counts,
                            prob, rows, loss);
 }
 

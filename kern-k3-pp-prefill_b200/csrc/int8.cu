@@ -44,10 +44,14 @@ struct QuantRows {
   long long cap_rows;  // output rows
 };
 
-// act(g) * u; SwiGLU's sigmoid by one exponential and one reciprocal instruction (g = -inf: 0 * -inf, a NaN, as for
-// any row that holds an infinity)
-__device__ __forceinline__ float gate_of(float g, float u, int act) {
-  return act == 0 ? g * rcp_ftz(1.0f + ex2_ftz(g * -LOG2E)) * u : gated_act(g, u, act);
+// act(g) * u of two elements; SwiGLU's sigmoid by one exponential and one reciprocal instruction (g = -inf: 0 * -inf, a
+// NaN, as for any row that holds an infinity)
+__device__ __forceinline__ float2 gate_of(float2 g, float2 u, int act) {
+  if (act != 0) return make_float2(gated_act(g.x, u.x, act), gated_act(g.y, u.y, act));
+  const u64 x = f32x2(g.x, g.y);
+  const float2 t = f32x2_get(mul_f32x2(x, f32x2(-LOG2E, -LOG2E)));
+  const float2 d = f32x2_get(add_f32x2(f32x2(ex2_ftz(t.x), ex2_ftz(t.y)), f32x2(1.f, 1.f)));
+  return f32x2_get(mul_f32x2(mul_f32x2(x, f32x2(rcp_ftz(d.x), rcp_ftz(d.y))), f32x2(u.x, u.y)));
 }
 
 // 8 consecutive elements of a row as they are kept: bf16 pairs, or f32
@@ -60,47 +64,49 @@ struct Kept {
   }
 };
 
-// 8 bf16 from s (zero past `left`)
-__device__ __forceinline__ uint4 load_bf16x8(const bf16* s, int left, int vec) {
-  if (vec && left >= 8) return *reinterpret_cast<const uint4*>(s);
+// 8 bf16 from s; not WHOLE: one at a time, zero past `left`
+template <bool WHOLE>
+__device__ __forceinline__ uint4 load_bf16x8(const bf16* s, int left) {
+  if (WHOLE) return *reinterpret_cast<const uint4*>(s);
   u32 h[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) h[i] = i < left ? (u32)__bfloat16_as_ushort(s[i]) : 0u;
   return make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
 }
 
-template <int SRC>
-__device__ __forceinline__ void load8(const QuantRows& p, long long r, int c, Kept<SRC>& v) {
+// elements c .. c + 7 of a row that starts at x
+template <int SRC, bool WHOLE>
+__device__ __forceinline__ void load8(const QuantRows& p, const void* x, int c, Kept<SRC>& v) {
+  constexpr int M = SRC == I8_BF16 ? 4 : 8;
   const int left = p.cols - c;
   if (SRC == I8_F32) {
-    const float* s = reinterpret_cast<const float*>(p.x) + r * p.ldx + c;
-    if (p.vec && left >= 8) {
+    const u32* s = reinterpret_cast<const u32*>(x) + c;
+    if (WHOLE) {
       const uint4 a = reinterpret_cast<const uint4*>(s)[0], b = reinterpret_cast<const uint4*>(s)[1];
       const u32 w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v.w[i % (SRC == I8_BF16 ? 4 : 8)] = w[i];
+      for (int i = 0; i < 8; ++i) v.w[i % M] = w[i];
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v.w[i % (SRC == I8_BF16 ? 4 : 8)] = i < left ? __float_as_uint(s[i]) : 0u;
+      for (int i = 0; i < 8; ++i) v.w[i % M] = i < left ? s[i] : 0u;
     }
     return;
   }
-  const bf16* s = reinterpret_cast<const bf16*>(p.x) + r * p.ldx + c;
-  const uint4 a = load_bf16x8(s, left, p.vec);
+  const bf16* s = reinterpret_cast<const bf16*>(x) + c;
+  const uint4 a = load_bf16x8<WHOLE>(s, left);
+  const u32 g[4] = {a.x, a.y, a.z, a.w};
   if (SRC == I8_BF16) {
-    v.w[0] = a.x;
-    v.w[1] = a.y;
-    v.w[2] = a.z;
-    v.w[3] = a.w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v.w[i] = g[i];
     return;
   }
-  const uint4 b = load_bf16x8(s + p.cols, left, p.vec);
-  const u32 g[4] = {a.x, a.y, a.z, a.w}, u[4] = {b.x, b.y, b.z, b.w};
+  const uint4 b = load_bf16x8<WHOLE>(s + p.cols, left);
+  const u32 u[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 x = bf16x2_to_f2(g[i]), y = bf16x2_to_f2(u[i]);
-    v.w[(2 * i) % (SRC == I8_BF16 ? 4 : 8)] = __float_as_uint(gate_of(x.x, y.x, p.act));
-    v.w[(2 * i + 1) % (SRC == I8_BF16 ? 4 : 8)] = __float_as_uint(gate_of(x.y, y.y, p.act));
+    const float2 h = gate_of(bf16x2_to_f2(g[i]), bf16x2_to_f2(u[i]), p.act);
+    v.w[(2 * i) % M] = __float_as_uint(h.x);
+    v.w[(2 * i + 1) % M] = __float_as_uint(h.y);
   }
 }
 
@@ -112,8 +118,11 @@ __device__ __forceinline__ u32 max_bits(u32 m, const Kept<SRC>& v) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) asm("max.s16x2 %0, %0, %1;" : "+r"(m) : "r"(v.w[i] & 0x7fff7fffu));
   } else {
+    float f = __uint_as_float(m);
 #pragma unroll
-    for (int i = 0; i < (SRC == I8_BF16 ? 4 : 8); ++i) m = max(m, v.w[i] & 0x7fffffffu);
+    for (int i = 0; i < (SRC == I8_BF16 ? 4 : 8); ++i)
+      asm("max.NaN.f32 %0, %0, %1;" : "+f"(f) : "f"(fabsf(__uint_as_float(v.w[i]))));
+    m = __float_as_uint(f);
   }
   return m;
 }
@@ -135,6 +144,19 @@ __device__ __forceinline__ RowScale row_scale(u32 amax_bits) {
 __device__ __forceinline__ float scale_of(const RowScale& s) {
   return __float_as_uint(s.amax) >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __fdiv_rn(s.amax, 127.f);
 }
+// Rows at the ends of the range: the kept elements times `pre` (exact, but for those far too small to have a code), or
+// zeros where there is no scale.  Every other row skips this.
+template <int SRC>
+__device__ __forceinline__ void settle8(const RowScale& s, Kept<SRC>& v) {
+  if (SRC == I8_BF16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v.w[i] = s.inv == 0.f ? 0u : f2_to_bf16x2(v[2 * i] * s.pre, v[2 * i + 1] * s.pre);
+  } else {
+#pragma unroll
+    for (int i = 0; i < (SRC == I8_BF16 ? 4 : 8); ++i) v.w[i] = s.inv == 0.f ? 0u : __float_as_uint(v[i] * s.pre);
+  }
+}
 
 // the code of an element whose quotient lies near k + 1/2 in magnitude
 __device__ __forceinline__ int code_near_half(float x, int k, float amax) {
@@ -145,7 +167,6 @@ __device__ __forceinline__ int code_near_half(float x, int k, float amax) {
 
 template <int SRC>
 __device__ __forceinline__ uint2 encode8(const RowScale& s, const Kept<SRC>& v) {
-  if (s.inv == 0.f) return make_uint2(0u, 0u);
   if (SRC != I8_F32) {
     constexpr float ROUND = 12582912.f + 256.f;  // the integer, plus 256, in the low 16 bits
     const float above = s.inv * (1.f + 0x1p-21f), below = s.inv * (1.f - 0x1p-21f);
@@ -153,8 +174,7 @@ __device__ __forceinline__ uint2 encode8(const RowScale& s, const Kept<SRC>& v) 
     u32 k[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      u64 x = f32x2(v[2 * i], v[2 * i + 1]);
-      if (s.pre != 1.f) x = mul_f32x2(x, f32x2(s.pre, s.pre));
+      const u64 x = f32x2(v[2 * i], v[2 * i + 1]);
       const float2 a = f32x2_get(fma_f32x2(x, up, round)), b = f32x2_get(fma_f32x2(x, down, round));
       // two elements' integers in the halves of a word; their sum is odd where the two roundings differ, and half of it
       // rounded up to even is the code
@@ -171,26 +191,26 @@ __device__ __forceinline__ uint2 encode8(const RowScale& s, const Kept<SRC>& v) 
   float far = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float x = v[i] * s.pre, t = __fmaf_rn(x, s.inv, ROUND);
-    far = fmaxf(far, fabsf(__fmaf_rn(x, s.inv, ROUND - t)));  // x inv - its integer
+    const float t = __fmaf_rn(v[i], s.inv, ROUND);
+    far = fmaxf(far, fabsf(__fmaf_rn(v[i], s.inv, ROUND - t)));  // x inv - its integer
     k[i] = __float_as_uint(t);
   }
   if (far > NEAR) {  // one group in some thousands
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float x = v[i] * s.pre;
-      const float n = __uint_as_float(k[i]) - ROUND, d = __fmaf_rn(x, s.inv, -n);
+      const float n = __uint_as_float(k[i]) - ROUND, d = __fmaf_rn(v[i], s.inv, -n);
       // |quotient| = |n| + d (with n's sign), and the integer below it
       if (fabsf(d) > NEAR)
-        k[i] = (u32)code_near_half(x, (int)fabsf(n) - (n != 0.f && (d < 0.f) == (n > 0.f) ? 1 : 0), s.amax * s.pre);
+        k[i] = (u32)code_near_half(v[i], (int)fabsf(n) - (n != 0.f && (d < 0.f) == (n > 0.f) ? 1 : 0), s.amax * s.pre);
     }
   }
   const u32 a = __byte_perm(k[0], k[1], 0x0040), b = __byte_perm(k[2], k[3], 0x0040);
   const u32 c = __byte_perm(k[4], k[5], 0x0040), d = __byte_perm(k[6], k[7], 0x0040);
   return make_uint2(__byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410));
 }
+template <bool WHOLE>
 __device__ __forceinline__ void put8(int8_t* dst, int left, uint2 w) {
-  if (left >= 8) {
+  if (WHOLE || left >= 8) {
     *reinterpret_cast<uint2*>(dst) = w;
   } else {
 #pragma unroll
@@ -200,17 +220,20 @@ __device__ __forceinline__ void put8(int8_t* dst, int left, uint2 w) {
 }
 
 // LANES threads a row (a warp of a block of 256, or a block), NV groups of 8 elements a thread kept in registers;
-// NV = 0: rows too long for that are read a second time (from L2).  MINB blocks an SM: enough loads in flight.
-template <int SRC, int LANES, int NV, int MINB>
+// NV = 0: rows too long for that are read a second time (from L2).  MINB blocks an SM: enough loads in flight.  WHOLE:
+// rows are read 16 bytes at a time and end with a group (else an element at a time).
+template <int SRC, int LANES, int NV, int MINB, bool WHOLE>
 __global__ void __launch_bounds__(LANES > 32 ? LANES : 256, MINB) quant_int8_kernel(QuantRows p) {
   __shared__ u32 s_max[2][LANES > 32 ? LANES / 32 : 1];
   constexpr int PER = LANES > 32 ? 1 : 8;
   constexpr int STEP = LANES * 8;
+  constexpr int KEPT = NV > 0 ? NV : 1;
   const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   grid_wait_previous();
   grid_launch_dependents();
   const int nne = p.cta_limit ? min(p.meta[0], p.max_ctas) : 0;
   const int shared_row = p.exp2perm ? p.meta[2] : -1;
+  const long long row_bytes = p.ldx * (SRC == I8_F32 ? 4 : 2);
   int buf = 0;
   for (long long r = (long long)blockIdx.x * PER + sub; r < p.rows; r += (long long)gridDim.x * PER) {
     if (p.cta_limit && ((r >> 7) >= nne || r >= p.cta_limit[r >> 7])) continue;  // the row's LANES threads together
@@ -221,24 +244,22 @@ __global__ void __launch_bounds__(LANES > 32 ? LANES : 256, MINB) quant_int8_ker
       if (k < p.K) target = p.exp2perm[r * p.K + k];
       else if (k == p.K && shared_row >= 0) target = shared_row + (int)r;
     }
+    const char* x = reinterpret_cast<const char*>(p.x) + r * row_bytes;
     u32 m = 0;
-    Kept<SRC> v[NV > 0 ? NV : 1];
+    Kept<SRC> v[KEPT];
     if (NV > 0) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int c = j * STEP + lane * 8;
-        if (c < p.cols) {
-          load8<SRC>(p, r, c, v[j]);
-        } else {
 #pragma unroll
-          for (int i = 0; i < (SRC == I8_BF16 ? 4 : 8); ++i) v[j].w[i] = 0u;
-        }
+        for (int i = 0; i < (SRC == I8_BF16 ? 4 : 8); ++i) v[j].w[i] = 0u;
+        if (c < p.cols) load8<SRC, WHOLE>(p, x, c, v[j]);
       }
 #pragma unroll
       for (int j = 0; j < NV; ++j) m = max_bits<SRC>(m, v[j]);
     } else {
       for (int c = lane * 8; c < p.cols; c += STEP) {
-        load8<SRC>(p, r, c, v[0]);
+        load8<SRC, WHOLE>(p, x, c, v[0]);
         m = max_bits<SRC>(m, v[0]);
       }
     }
@@ -252,17 +273,22 @@ __global__ void __launch_bounds__(LANES > 32 ? LANES : 256, MINB) quant_int8_ker
       buf ^= 1;  // the next row's maxima go to the other half: one barrier a row
     }
     const RowScale s = row_scale<SRC>(m);
-    if (NV > 0) {
-      if (!p.exp2perm) {
-        int8_t* dst = p.q + r * p.ldq;
+    const bool rare = s.pre != 1.f;
+    if (NV > 0 && rare) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          const int c = j * STEP + lane * 8;
-          if (c < p.cols) put8(dst + c, p.cols - c, encode8<SRC>(s, v[j]));
-        }
-        if (lane == 0) p.scale[r] = scale_of(s);
-        continue;
+      for (int j = 0; j < NV; ++j) settle8<SRC>(s, v[j]);
+    }
+    if (NV > 0 && !p.exp2perm) {
+      int8_t* dst = p.q + r * p.ldq;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = j * STEP + lane * 8;
+        if (c < p.cols) put8<WHOLE>(dst + c, p.cols - c, encode8<SRC>(s, v[j]));
       }
+      if (lane == 0) p.scale[r] = scale_of(s);
+      continue;
+    }
+    if (NV > 0) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const uint2 w = encode8<SRC>(s, v[j]);  // past the row's end: zeros, kept and not stored
@@ -279,12 +305,13 @@ __global__ void __launch_bounds__(LANES > 32 ? LANES : 256, MINB) quant_int8_ker
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           const int c = j * STEP + lane * 8;
-          if (c < p.cols) put8(dst + c, p.cols - c, make_uint2(v[j].w[0], v[j].w[1]));
+          if (c < p.cols) put8<WHOLE>(dst + c, p.cols - c, make_uint2(v[j].w[0], v[j].w[1]));
         }
       } else {
         for (int c = lane * 8; c < p.cols; c += STEP) {
-          load8<SRC>(p, r, c, v[0]);
-          put8(dst + c, p.cols - c, encode8<SRC>(s, v[0]));
+          load8<SRC, WHOLE>(p, x, c, v[0]);
+          if (rare) settle8<SRC>(s, v[0]);
+          put8<WHOLE>(dst + c, p.cols - c, encode8<SRC>(s, v[0]));
         }
       }
       if (lane == 0) p.scale[o] = scale_of(s);
