@@ -170,10 +170,13 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
     r = max(r0, in.seq[0]);
     last = min(r1, in.seq[in.B]);
   }
+  int b = -1;
   while (r < last) {
-    int b = 0, end = last;
+    int end = last;
     if (in.seq) {
-      b = seq_of(in.seq, in.B, r, lane);
+      // the next sequence, if it holds row r: one load where sequences are short and follow one another
+      if (b >= 0 && b + 2 <= in.B && in.seq[b + 2] > r) ++b;
+      else b = seq_of(in.seq, in.B, r, lane);
       end = min(last, in.seq[b + 1]);
       if (end <= r) break;  // offsets that go down: nothing more is counted
     }
@@ -226,7 +229,7 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
       }
     }
     __syncthreads();
-    const long long slot = (long long)blockIdx.x + b;
+    const long long slot = (long long)blockIdx.x + max(b, 0);
     for (int e = threadIdx.x; e < in.E; e += 32 * ROW_WARPS) {
       float p = 0.f;
 #pragma unroll
@@ -404,6 +407,7 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
     __syncthreads();
   }
   const float rs = weights ? __bfloat162float(q.rs[0]) : 0.f;
+  const bool vec_counts = in.E % 4 == 0 && reinterpret_cast<uintptr_t>(q.counts) % 16 == 0;
   int b = -1, b_end = -1;  // the sequence up to row b_end is b
   for (; t < r1; t += ROW_WARPS, ++at) {
     ring.fetch(in, at + slots(NV) - 1, ahead(slots(NV) - 1), balance, weights, q.dwts);
@@ -438,10 +442,16 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
         if (cb == nullptr) {
           f = *reinterpret_cast<const ulonglong2*>(sf + c);
         } else {
-          float g[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) g[i] = c + i < in.E ? k * (float)cb[c + i] : 0.f;
-          f = make_ulonglong2(f32x2(g[0], g[1]), f32x2(g[2], g[3]));
+          int4 g = make_int4(0, 0, 0, 0);
+          if (vec_counts) {
+            if (c < in.E) g = *reinterpret_cast<const int4*>(cb + c);
+          } else {
+            g.x = c < in.E ? cb[c] : 0;
+            g.y = c + 1 < in.E ? cb[c + 1] : 0;
+            g.z = c + 2 < in.E ? cb[c + 2] : 0;
+            g.w = c + 3 < in.E ? cb[c + 3] : 0;
+          }
+          f = make_ulonglong2(f32x2(k * (float)g.x, k * (float)g.y), f32x2(k * (float)g.z, k * (float)g.w));
         }
         m2 = fma_f32x2(f.x, s0, fma_f32x2(f.y, s1, m2));
         d[2 * j] = f.x;

@@ -49,7 +49,7 @@ int current_device() {
 template <typename F>
 bool set_smem_once(F kernel, int bytes, int slot) {
   static std::mutex mu;
-  static bool done[kMaxDevices][24] = {};
+  static bool done[kMaxDevices][32] = {};
   const int dev = current_device();
   std::lock_guard<std::mutex> g(mu);
   if (dev >= 0 && dev < kMaxDevices && done[dev][slot]) return true;
@@ -369,24 +369,23 @@ int encode_int8(CUtensorMap* m, const void* base, long long rows, int cols, long
 }
 
 int int8_launch(const int8_t* q, long long q_rows, long long ldq, const int8_t* w, long long w_rows, long long ldw,
-                int C, Int8Params& p, int dtype, int grid, cudaStream_t s) {
+                int C, Int8Params& p, bool pair, int dtype, int grid, cudaStream_t s) {
   CUtensorMap tw, tx;
   int rc = encode_int8(&tw, w, w_rows, C, ldw, i8::BM);
   if (rc) return rc;
   rc = encode_int8(&tx, q, q_rows, C, ldq, p.xbox);
   if (rc) return rc;
   p.kstages = (int)cdiv(C, i8::BK);
-  p.n_tiles = (int)cdiv(p.N, i8::BM);
-  p.stage_bytes = i8::W_BYTES + p.bn * i8::BK;
+  p.n_tiles = (int)cdiv(p.N, pair ? 2 * i8::BM : i8::BM);
+  p.stage_bytes = i8::W_BYTES + (pair ? p.bn / 2 : p.bn) * i8::BK;
   p.stages = std::min(i8::MAX_STAGES, i8::RING_BYTES / p.stage_bytes);
   p.tmem_cols = 32;
   while (p.tmem_cols < 2u * p.bn) p.tmem_cols *= 2;
-  const bool f32 = dtype == K3MOE_F32;
-  if (!(f32 ? set_smem_once(int8_gemm_kernel<float>, i8::SMEM_BYTES, 4)
-            : set_smem_once(int8_gemm_kernel<bf16>, i8::SMEM_BYTES, 5)))
-    return K3MOE_ELAUNCH;
-  return launch_overlapped(f32 ? int8_gemm_kernel<float> : int8_gemm_kernel<bf16>, grid, i8::THREADS, i8::SMEM_BYTES, s,
-                           p.splits, tw, tx, p);
+  void (*kernel)(CUtensorMap, CUtensorMap, Int8Params) =
+      dtype == K3MOE_F32 ? (pair ? int8_gemm_kernel<float, true> : int8_gemm_kernel<float, false>)
+                         : (pair ? int8_gemm_kernel<bf16, true> : int8_gemm_kernel<bf16, false>);
+  if (!set_smem_once(kernel, i8::SMEM_BYTES, dtype == K3MOE_F32 ? (pair ? 22 : 4) : (pair ? 23 : 5))) return K3MOE_ELAUNCH;
+  return launch_overlapped(kernel, grid, i8::THREADS, i8::SMEM_BYTES, s, pair ? 2 : p.splits, tw, tx, p);
 }
 
 }  // namespace
@@ -722,17 +721,22 @@ int k3moe_gemm_int8(const int8_t* q, long long ldq, const float* sx, const int8_
   p.T = T;
   p.N = N;
   p.err = err;
-  const long long n_tiles = cdiv(N, i8::BM);
-  p.bn = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
-  while (p.bn > 64 && n_tiles * cdiv(T, p.bn) < sms) p.bn /= 2;
-  p.xbox = p.bn;
+  // pairs of blocks on 256 channels x 256 tokens, where these make a unit for most pairs
+  const long long pair_units = cdiv(N, 2 * i8::BM) * cdiv(T, 256);
+  const bool pair = 4 * pair_units >= 3 * (sms / 2);
+  const long long n_tiles = cdiv(N, pair ? 2 * i8::BM : i8::BM);
+  p.bn = pair ? 256 : T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
+  while (!pair && p.bn > 64 && n_tiles * cdiv(T, p.bn) < sms) p.bn /= 2;
+  p.xbox = pair ? p.bn / 2 : p.bn;
   p.t_tiles = (int)cdiv(T, p.bn);
   const long long units = n_tiles * p.t_tiles;
   if (units > 0x7fffffffLL) return K3MOE_EINVAL;
   p.splits = 1;
-  while (p.splits < 8 && units * p.splits * 2 <= sms && cdiv(C, i8::BK) >= 8 * p.splits) p.splits *= 2;
-  const int grid = p.splits > 1 ? (int)units * p.splits : (int)std::min<long long>(units, sms);
-  return int8_launch(q, T, ldq, w, N, ldw, C, p, dtype, grid, reinterpret_cast<cudaStream_t>(stream));
+  while (!pair && p.splits < 8 && units * p.splits * 2 <= sms && cdiv(C, i8::BK) >= 8 * p.splits) p.splits *= 2;
+  const int grid = pair              ? 2 * (int)std::min<long long>(units, sms / 2)
+                   : p.splits > 1    ? (int)units * p.splits
+                                     : (int)std::min<long long>(units, sms);
+  return int8_launch(q, T, ldq, w, N, ldw, C, p, pair, dtype, grid, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int k3moe_grouped_gemm_int8(const int8_t* q_perm, long long ldq, const float* sx_perm, const int8_t* w, long long ldw,
@@ -762,7 +766,7 @@ int k3moe_grouped_gemm_int8(const int8_t* q_perm, long long ldq, const float* sx
   p.max_ctas = max_ctas;
   p.cap_rows = cap_rows;
   const int grid = (int)std::min<long long>(max_ctas * cdiv(N, i8::BM), num_sms(current_device()));
-  return int8_launch(q_perm, cap_rows, ldq, w, (long long)n_experts * N, ldw, C, p, dtype, grid,
+  return int8_launch(q_perm, cap_rows, ldq, w, (long long)n_experts * N, ldw, C, p, false, dtype, grid,
                      reinterpret_cast<cudaStream_t>(stream));
 }
 

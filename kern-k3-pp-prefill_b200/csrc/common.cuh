@@ -282,6 +282,43 @@ __device__ __forceinline__ void tc_commit(u64* bar) {
                : "memory");
 }
 
+// A pair of blocks (a cluster of two) working on one tile (cta_group::2): both allocate and free the same columns, ...
+__device__ __forceinline__ void tmem_alloc_pair(u32* dst_smem, u32 ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)), "r"(ncols)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish_pair() {
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(u32 taddr, u32 ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// ... the even block issues the MMAs, and their completion arrives on both blocks' `bar`.
+__device__ __forceinline__ void tc_commit_pair(u64* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((unsigned short)3)
+      : "memory");
+}
+// the address of `p`'s counterpart in block `rank` of the cluster
+__device__ __forceinline__ u32 cluster_addr(const void* p, u32 rank) {
+  u32 a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(u32 addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// a TMA load into this block's shared memory that completes on either block's barrier (a cluster address)
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const void* tmap, u32 bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(tmap), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+
 // D[tmem] (+)= A[smem] x B[smem]^T with per-32 UE8M0 scales read from tmem.
 __device__ __forceinline__ void mma_mxf8f6f4(u32 d_tmem, u64 adesc, u64 bdesc, u32 idesc, u32 sfa_tmem, u32 sfb_tmem,
                                              u32 accumulate) {

@@ -326,6 +326,11 @@ __global__ void __launch_bounds__(LANES > 32 ? LANES : 256, MINB) quant_int8_ker
 // ends are zero-filled by the loads.  Roles (320 threads): warp 0 lane 0 issues the TMA boxes, warp 1 lane 0 the MMAs
 // into one of two TMEM accumulators, warps 2-9 scale and store the other.  Every wait is bounded and reports.
 //
+// Where there are tokens enough (PAIR) two blocks share a unit of 256 channels x up to 256 tokens (cta_group::2): each
+// loads its 128 channels and half of the tokens, the even block issues M = 256 MMAs over both blocks' shared memory, and
+// each drains its own channels.  One block alone would write and read 96 KB of shared memory for the 512 MMA cycles of a
+// stage, more than its 128 bytes a cycle; a pair halves the tokens' part.
+//
 // With few units a cluster of `splits` blocks shares one unit, each a part of K; the parts' int32 sums meet in shared
 // memory (each block adds every split-th token of all blocks' tiles through the cluster), so a decode step keeps all
 // SMs loading weights without a workspace or a second launch.
@@ -367,11 +372,12 @@ struct Int8Params {
 struct Int8Unit {
   int valid, e, row0, n, ch0;
 };
-__device__ __forceinline__ Int8Unit int8_unit(const Int8Params& p, int u) {
+template <bool PAIR>
+__device__ __forceinline__ Int8Unit int8_unit(const Int8Params& p, int u, int rank) {
   Int8Unit w;
   const int c = u / p.n_tiles;
-  w.ch0 = (u % p.n_tiles) * i8::BM;
-  if (p.cta_batch) {
+  w.ch0 = PAIR ? (u % p.n_tiles) * 2 * i8::BM + rank * i8::BM : (u % p.n_tiles) * i8::BM;
+  if (!PAIR && p.cta_batch) {
     w.e = p.cta_batch[c];
     w.row0 = c * 128;
     w.n = p.cta_limit[c] - w.row0;
@@ -388,6 +394,13 @@ __device__ __forceinline__ Int8Unit int8_unit(const Int8Params& p, int u) {
 // kind::i8 instruction descriptor: s32 accumulator, signed A and B, both K-major, M x N
 __device__ __forceinline__ u32 i8_idesc(int m, int n) {
   return 2u << 4 | 1u << 7 | 1u << 10 | (u32)(n >> 3) << 17 | (u32)(m >> 4) << 24;
+}
+__device__ __forceinline__ void i8_mma_pair(u32 d_tmem, u64 adesc, u64 bdesc, u32 idesc, u32 accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
 __device__ __forceinline__ void i8_mma(u32 d_tmem, u64 adesc, u64 bdesc, u32 idesc, u32 accumulate) {
   asm volatile(
@@ -434,7 +447,7 @@ __device__ __forceinline__ bf16 int8_value<bf16>(u32 acc, float sx, float sw) {
   return __float2bfloat16_rn(__int2float_rn((int)acc) * sx * sw);
 }
 
-template <typename OUT>
+template <typename OUT, bool PAIR>
 __global__ void __launch_bounds__(i8::THREADS, 1)
     int8_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, Int8Params p) {
   using namespace i8;
@@ -452,8 +465,13 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 1) {
-    tmem_alloc(tmem_slot, p.tmem_cols);
-    tmem_relinquish();
+    if (PAIR) {
+      tmem_alloc_pair(tmem_slot, p.tmem_cols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, p.tmem_cols);
+      tmem_relinquish();
+    }
   }
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
@@ -462,7 +480,7 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], EPI_WARPS);
+      mbar_init(&acc_empty[b], PAIR ? 2 * EPI_WARPS : EPI_WARPS);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -472,15 +490,17 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();  // the other block's barriers are there
   tc_fence_after();
   const u32 tmem_base = *tmem_slot;
   grid_wait_previous();  // the rows (and whatever else an earlier kernel writes) are there from here on
   const int units = (p.cta_batch ? min(p.meta[0], p.max_ctas) : p.t_tiles) * p.n_tiles;
   // the block's part of K (all of it without a cluster)
-  const int rank = p.splits > 1 ? (int)cluster_rank() : 0;
-  const int k0 = (int)((long long)rank * p.kstages / p.splits);
-  const int k1 = (int)((long long)(rank + 1) * p.kstages / p.splits);
-  const int first = blockIdx.x / p.splits, stride = gridDim.x / p.splits;
+  const int rank = PAIR || p.splits > 1 ? (int)cluster_rank() : 0;
+  const int k0 = PAIR ? 0 : (int)((long long)rank * p.kstages / p.splits);
+  const int k1 = PAIR ? p.kstages : (int)((long long)(rank + 1) * p.kstages / p.splits);
+  const int share = PAIR ? 2 : p.splits;  // blocks a unit
+  const int first = blockIdx.x / share, stride = gridDim.x / share;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -489,45 +509,57 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
       u32 phase = 0;
       u32 armed = 0;  // fills issued; stage s holds the last of them with index = s mod stages
       for (int u = first; u < units && !*abort_flag; u += stride) {
-        const Int8Unit w = int8_unit(p, u);
+        const Int8Unit w = int8_unit<PAIR>(p, u, rank);
         if (!w.valid) {
           report_error(p.err, ERR_BAD_TABLE, 0xD00u);
           continue;
         }
-        const int boxes = (w.n + p.xbox - 1) / p.xbox;
-        const u32 tx = (u32)(W_BYTES + boxes * p.xbox * BK);
+        const int boxes = PAIR ? 1 : (w.n + p.xbox - 1) / p.xbox;
+        // PAIR: both blocks' loads complete on the even block's barrier, which expects them all
+        const u32 tx = (u32)(W_BYTES + boxes * p.xbox * BK) * (PAIR ? 2u : 1u);
         const int wrow = w.e * p.N + w.ch0;
+        const int xrow = w.row0 + (PAIR ? rank * (((w.n + 31) & ~31) / 2) : 0);
         for (int ks = k0; ks < k1; ++ks) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.err, 0xD10u)) break;
           uint8_t* st = smem + stage * p.stage_bytes;
-          mbar_arrive_expect_tx(&full[stage], tx);
-          ++armed;
-          tma_load_2d(st, &tmW, &full[stage], ks * BK, wrow);
-          for (int i = 0; i < boxes; ++i)
-            tma_load_2d(st + W_BYTES + i * p.xbox * BK, &tmX, &full[stage], ks * BK, w.row0 + i * p.xbox);
+          if (PAIR) {
+            if (rank == 0) {
+              mbar_arrive_expect_tx(&full[stage], tx);
+              ++armed;
+            }
+            const u32 bar = cluster_addr(&full[stage], 0);
+            tma_load_2d_pair(st, &tmW, bar, ks * BK, wrow);
+            tma_load_2d_pair(st + W_BYTES, &tmX, bar, ks * BK, xrow);
+          } else {
+            mbar_arrive_expect_tx(&full[stage], tx);
+            ++armed;
+            tma_load_2d(st, &tmW, &full[stage], ks * BK, wrow);
+            for (int i = 0; i < boxes; ++i)
+              tma_load_2d(st + W_BYTES + i * p.xbox * BK, &tmX, &full[stage], ks * BK, xrow + i * p.xbox);
+          }
           if (++stage == p.stages) {
             stage = 0;
             phase ^= 1u;
           }
         }
       }
-      // every fill has landed before the block may exit
+      // every fill has landed before the block may exit (PAIR: before either may, behind the cluster barrier below)
       for (u32 s = 0; s < (u32)p.stages && s < armed; ++s)
         mbar_wait(&full[s], ((armed - 1 - s) / (u32)p.stages) & 1u, nullptr, p.err, 0xD20u, 100000000ull);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (lane == 0 && (!PAIR || rank == 0)) {
       // ------------------------------------------------ MMA issuer
       int stage = 0, buf = 0;
       u32 phase = 0;
       u32 acc_phase = 0;  // bit b: accumulator b's parity
       bool issued = false;
       for (int u = first; u < units && !*abort_flag; u += stride) {
-        const Int8Unit w = int8_unit(p, u);
+        const Int8Unit w = int8_unit<PAIR>(p, u, rank);
         if (!w.valid) continue;
         if (!mbar_wait(&acc_empty[buf], ((acc_phase >> buf) & 1u) ^ 1u, abort_flag, p.err, 0xD30u)) break;
         tc_fence_after();
-        const u32 idesc = i8_idesc(BM, (w.n + 15) & ~15);
+        const u32 idesc = PAIR ? i8_idesc(2 * BM, (w.n + 31) & ~31) : i8_idesc(BM, (w.n + 15) & ~15);
         const u32 d = tmem_base + (u32)(buf * p.bn);
         bool ok = true;
         for (int ks = k0; ks < k1; ++ks) {
@@ -538,10 +570,13 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
           tc_fence_after();
           const u32 st = smem_u32(smem + stage * p.stage_bytes);
 #pragma unroll
-          for (int kk = 0; kk < BK / 32; ++kk)
-            i8_mma(d, sdesc_k_sw128(st + kk * 32), sdesc_k_sw128(st + W_BYTES + kk * 32), idesc,
-                   ks != k0 || kk != 0);
-          tc_commit(&empty[stage]);
+          for (int kk = 0; kk < BK / 32; ++kk) {
+            const u64 a = sdesc_k_sw128(st + kk * 32), b = sdesc_k_sw128(st + W_BYTES + kk * 32);
+            if (PAIR) i8_mma_pair(d, a, b, idesc, ks != k0 || kk != 0);
+            else i8_mma(d, a, b, idesc, ks != k0 || kk != 0);
+          }
+          if (PAIR) tc_commit_pair(&empty[stage]);
+          else tc_commit(&empty[stage]);
           issued = true;
           if (++stage == p.stages) {
             stage = 0;
@@ -549,12 +584,14 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
           }
         }
         if (!ok) break;
-        tc_commit(&acc_full[buf]);
+        if (PAIR) tc_commit_pair(&acc_full[buf]);
+        else tc_commit(&acc_full[buf]);
         acc_phase ^= 1u << buf;
         buf ^= 1;
       }
       if (issued) {
-        tc_commit(drain);
+        if (PAIR) tc_commit_pair(drain);
+        else tc_commit(drain);
         mbar_wait(drain, 0, nullptr, p.err, 0xD50u, 100000000ull);
       }
     }
@@ -570,7 +607,7 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
     u32 acc_phase = 0;
     int buf = 0;
     for (int u = first; u < units && !*abort_flag; u += stride) {
-      const Int8Unit w = int8_unit(p, u);
+      const Int8Unit w = int8_unit<PAIR>(p, u, rank);
       if (!w.valid) continue;
       const int ch = w.ch0 + sub * 32 + lane;
       const float swc = ch < p.N ? p.sw[(long long)w.e * p.N + ch] : 0.f;
@@ -595,7 +632,7 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] = v[j];
         if (c + 32 < w.n) i8_ld16(acc + (u32)(c + 32), v);
-        if (p.splits > 1) {
+        if (!PAIR && p.splits > 1) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) red[(c + j) * BM + sub * 32 + lane] = (int)x[j];
         } else if (whole && c + 16 <= w.n) {
@@ -616,20 +653,25 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[buf]);
+      if (lane == 0) {
+        if (PAIR) mbar_arrive_cluster(cluster_addr(&acc_empty[buf], 0));
+        else mbar_arrive(&acc_empty[buf]);
+      }
       acc_phase ^= 1u << buf;
       buf ^= 1;
     }
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();  // neither block's shared memory, barriers or accumulators are in use any more
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, p.tmem_cols);
+    if (PAIR) tmem_dealloc_pair(tmem_base, p.tmem_cols);
+    else tmem_dealloc(tmem_base, p.tmem_cols);
   }
-  if (p.splits > 1) {
+  if (!PAIR && p.splits > 1) {
     // one unit a cluster: the parts of K meet
-    const Int8Unit w = int8_unit(p, first);
+    const Int8Unit w = int8_unit<PAIR>(p, first, rank);
     const u32 red = smem_u32(smem);
     cluster_sync();
     for (int t = warp * p.splits + rank; t < w.n; t += WARPS * p.splits) {
