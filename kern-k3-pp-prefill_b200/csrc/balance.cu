@@ -20,6 +20,7 @@ namespace k3 {
 
 namespace bal {
 constexpr int JOIN_WARPS = 32;   // of a block of the join, at most
+constexpr int JOIN_BLOCKS = 8 * 148;
 constexpr int ROW_WARPS = 16;    // of a block that walks rows
 constexpr int PICKS = 16;        // K at most
 // Row slots a warp: as many as fit, four at most.  One block an SM where a row is long, two where it is short.
@@ -43,22 +44,54 @@ struct RouterRows {
   int vec;                 // S rows may be read 16 bytes at a time
 };
 
-// the sequence holding row r: the last b with seq[b] <= r (the caller has checked seq[0] <= r)
-__device__ __forceinline__ int seq_of(const int* __restrict__ seq, int B, int r, int lane) {
-  if (B <= 128) {  // in one load latency: the offsets up to r, counted by the warp
-    int n = 0;
+// A warp's finder of sequences: up to 128 offsets stay in its registers, four a lane, so that a row's sequence is a count
+// of the offsets up to it; of more, a binary search, which neighbouring rows of one sequence share.
+struct SeqFinder {
+  const int* seq;
+  int B, lo, hi;       // rows outside [lo, hi) lie in none
+  int mine[4];
+  int b, end;          // the last answer, good up to row `end`
+  __device__ __forceinline__ void init(const RouterRows& in, int lane) {
+    seq = in.seq;
+    B = in.B;
+    lo = 0;
+    hi = in.T;
+    b = -1;
+    end = -1;
+    if (seq == nullptr) return;
+    lo = max(seq[0], 0);
+    hi = min(seq[B], in.T);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) n += i * 32 + lane < B && seq[i * 32 + lane] <= r;
-    return max((int)__reduce_add_sync(0xffffffffu, n) - 1, 0);
+    for (int i = 0; i < 4; ++i) mine[i] = i * 32 + lane < B && B <= 128 ? seq[i * 32 + lane] : 0x7fffffff;
   }
-  int lo = 0, hi = B - 1;
-  while (lo < hi) {
-    const int m = (lo + hi + 1) >> 1;
-    if (seq[m] <= r) lo = m;
-    else hi = m - 1;
+  // the sequence of row t, the last b with seq[b] <= t, or -1; every lane of the warp asks for the same row
+  __device__ __forceinline__ int operator()(int t) {
+    if (t < lo || t >= hi) return -1;
+    if (seq == nullptr) return 0;
+    if (B <= 128) {
+      int n = __popc(__ballot_sync(0xffffffffu, mine[0] <= t));
+      if (B > 32) {
+#pragma unroll
+        for (int i = 1; i < 4; ++i) n += __popc(__ballot_sync(0xffffffffu, mine[i] <= t));
+      }
+      return max(n - 1, 0);
+    }
+    if (b >= 0 && t >= seq[b] && t < end) return b;
+    if (b >= 0 && b + 2 <= B && t >= end && t < seq[b + 2]) {
+      ++b;  // the next one: sequences are short and follow one another
+    } else {
+      int x = 0, y = B - 1;
+      while (x < y) {
+        const int m = (x + y + 1) >> 1;
+        if (seq[m] <= t) x = m;
+        else y = m - 1;
+      }
+      b = x;
+    }
+    end = seq[b + 1];
+    return b;
   }
-  return lo;
-}
+};
 
 // A row on its way through shared memory: the logits, the picks, the gradients of their weights.  Each warp keeps a few
 // rows in flight by cp.async, which takes no registers and leaves nothing to spin on.  A lane's experts are 4 consecutive
@@ -139,7 +172,7 @@ struct BalanceScratch {
   float* prob;   // [slots, E]
   int* count;    // [slots, E]
   int* rows;     // [slots]
-  float* term;   // [B, ceil(E / 32)]
+  float* term;   // [blocks of the second pass]
   u32* done;
 };
 
@@ -165,21 +198,13 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
     return u < r1 ? u : -1;
   };
   for (int i = 0; i < slots(NV) - 1; ++i) ring.fetch(in, i, ahead(i), true, true, nullptr);
-  int r = r0, last = r1;
-  if (in.seq) {
-    r = max(r0, in.seq[0]);
-    last = min(r1, in.seq[in.B]);
-  }
-  int b = -1;
+  SeqFinder find;
+  find.init(in, lane);
+  int r = max(r0, find.lo);
+  const int last = min(r1, find.hi);
   while (r < last) {
-    int end = last;
-    if (in.seq) {
-      // the next sequence, if it holds row r: one load where sequences are short and follow one another
-      if (b >= 0 && b + 2 <= in.B && in.seq[b + 2] > r) ++b;
-      else b = seq_of(in.seq, in.B, r, lane);
-      end = min(last, in.seq[b + 1]);
-      if (end <= r) break;  // offsets that go down: nothing more is counted
-    }
+    const int b = find(r), end = in.seq ? min(last, in.seq[b + 1]) : last;
+    if (end <= r) break;  // offsets that go down: nothing more is counted
     u64 acc[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = f32x2(0.f, 0.f);
@@ -229,7 +254,7 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
       }
     }
     __syncthreads();
-    const long long slot = (long long)blockIdx.x + max(b, 0);
+    const long long slot = (long long)blockIdx.x + b;
     for (int e = threadIdx.x; e < in.E; e += 32 * ROW_WARPS) {
       float p = 0.f;
 #pragma unroll
@@ -248,8 +273,8 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
   cp_async_wait_all();
 }
 
-// Second pass: a block adds up 32 experts of one sequence over the first pass's blocks that met it (its warps side
-// by side, joined in order), and the last block of all adds up the loss.
+// Second pass: a block adds up 32 experts of one sequence over the first pass's blocks that met it (its warps side by
+// side, joined in order), then the next such group of its share; the last block of all adds up the loss.
 __global__ void __launch_bounds__(32 * bal::JOIN_WARPS)
     balance_join_kernel(RouterRows in, BalanceScratch w, int chunk, float alpha, int* __restrict__ counts,
                         float* __restrict__ prob, int* __restrict__ rows, float* __restrict__ loss) {
@@ -259,61 +284,60 @@ __global__ void __launch_bounds__(32 * bal::JOIN_WARPS)
   __shared__ int s_c[JOIN_WARPS][COLS], s_n[JOIN_WARPS];
   __shared__ int s_last;
   const int groups = (in.E + COLS - 1) / COLS;
-  const int b = blockIdx.x / groups, g = blockIdx.x % groups;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int e = g * COLS + lane;
-  int s0 = 0, s1 = in.T;
-  if (in.seq) {
-    const int lo = max(in.seq[0], 0), hi = min(in.seq[in.B], in.T);
-    s0 = max(lo, in.seq[b]);
-    s1 = min(hi, in.seq[b + 1]);
-  }
-  grid_wait_previous();  // the first pass's partial rows (that pass lets this one start after its own wait: the offsets
-                         // above are there before)
-  float p = 0.f;
-  int c = 0, n = 0;
-  if (s0 < s1) {
-    const int i1 = (s1 - 1) / chunk;
+  const int lo = in.seq ? max(in.seq[0], 0) : 0, hi = in.seq ? min(in.seq[in.B], in.T) : in.T;
+  float terms = 0.f;
+  for (int unit = blockIdx.x; unit < in.B * groups; unit += gridDim.x) {
+    const int b = unit / groups, g = unit % groups, e = g * COLS + lane;
+    const int s0 = in.seq ? max(lo, in.seq[b]) : lo, s1 = in.seq ? min(hi, in.seq[b + 1]) : hi;
+    // the first pass's partial rows (it lets this one start after its own wait: the offsets are there before)
+    if (unit == blockIdx.x) grid_wait_previous();
+    float p = 0.f;
+    int c = 0, n = 0;
+    if (s0 < s1) {
+      const int i1 = (s1 - 1) / chunk;
 #pragma unroll 5
-    for (int i = s0 / chunk + warp; i <= i1; i += warps) {
-      const long long slot = (long long)i + b;
-      if (e < in.E) {
-        p += w.prob[slot * in.E + e];
-        c += w.count[slot * in.E + e];
+      for (int i = s0 / chunk + warp; i <= i1; i += warps) {
+        const long long slot = (long long)i + b;
+        if (e < in.E) {
+          p += w.prob[slot * in.E + e];
+          c += w.count[slot * in.E + e];
+        }
+        n += w.rows[slot];
       }
-      n += w.rows[slot];
     }
+    s_p[warp][lane] = p;
+    s_c[warp][lane] = c;
+    if (lane == 0) s_n[warp] = n;
+    __syncthreads();
+    if (warp == 0) {
+      for (int k = 1; k < warps; ++k) {
+        p += s_p[k][lane];
+        c += s_c[k][lane];
+        n += s_n[k];
+      }
+      float term = 0.f;
+      if (e < in.E) {
+        counts[(long long)b * in.E + e] = c;
+        prob[(long long)b * in.E + e] = p;
+        if (n > 0) term = ((float)in.E * (float)c / ((float)in.K * (float)n)) * (p / (float)n);
+      }
+      terms += warp_sum(term);
+      if (lane == 0 && g == 0) rows[b] = n;
+    }
+    __syncthreads();
   }
-  s_p[warp][lane] = p;
-  s_c[warp][lane] = c;
-  if (lane == 0) s_n[warp] = n;
-  __syncthreads();
-  if (warp == 0) {
-    for (int k = 1; k < warps; ++k) {
-      p += s_p[k][lane];
-      c += s_c[k][lane];
-      n += s_n[k];
-    }
-    float term = 0.f;
-    if (e < in.E) {
-      counts[(long long)b * in.E + e] = c;
-      prob[(long long)b * in.E + e] = p;
-      if (n > 0) term = ((float)in.E * (float)c / ((float)in.K * (float)n)) * (p / (float)n);
-    }
-    term = warp_sum(term);
-    if (lane == 0) {
-      w.term[blockIdx.x] = term;
-      if (g == 0) rows[b] = n;
-      __threadfence();
-      s_last = atomicAdd(w.done, 1u) == gridDim.x - 1;
-    }
+  if (threadIdx.x == 0) {
+    w.term[blockIdx.x] = terms;
+    __threadfence();
+    s_last = atomicAdd(w.done, 1u) == gridDim.x - 1;
   }
   __syncthreads();
   if (!s_last) return;
   __threadfence();
   float sum = 0.f;
   int full = 0;
-  for (long long i = threadIdx.x; i < (long long)gridDim.x; i += blockDim.x) sum += __ldcg(&w.term[i]);
+  for (int i = threadIdx.x; i < gridDim.x; i += blockDim.x) sum += __ldcg(&w.term[i]);
   for (int i = threadIdx.x; i < in.B; i += blockDim.x) full += __ldcg(&rows[i]) > 0;
   sum = warp_sum(sum);
   full = __reduce_add_sync(0xffffffffu, full);
@@ -370,17 +394,16 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
     return u < r1 ? u : -1;
   };
   for (int i = 0; i < slots(NV) - 1; ++i) ring.fetch(in, i, ahead(i), balance, weights, q.dwts);
-  // the sequence of row t, or -1
-  const int lo = in.seq ? in.seq[0] : 0, hi = in.seq ? in.seq[in.B] : in.T;
-  auto seq_at = [&](int t) { return t < lo || t >= hi ? -1 : in.seq ? seq_of(in.seq, in.B, t, lane) : 0; };
+  SeqFinder find;
+  find.init(in, lane);
   int b0 = -1, b1 = -1;
   float scale = 0.f;  // alpha dloss E / (B' K)
   if (balance) {
     int full = 0;
     for (int i = threadIdx.x; i < in.B; i += 32 * ROW_WARPS) full += q.rows[i] > 0;
     const float dloss = q.dloss ? *q.dloss : 1.0f;
-    b0 = seq_at(r0);
-    b1 = seq_at(r1 - 1);
+    b0 = find(r0);
+    b1 = find(r1 - 1);
     int c0[PER], c1[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -408,21 +431,16 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
   }
   const float rs = weights ? __bfloat162float(q.rs[0]) : 0.f;
   const bool vec_counts = in.E % 4 == 0 && reinterpret_cast<uintptr_t>(q.counts) % 16 == 0;
-  int b = -1, b_end = -1;  // the sequence up to row b_end is b
   for (; t < r1; t += ROW_WARPS, ++at) {
     ring.fetch(in, at + slots(NV) - 1, ahead(slots(NV) - 1), balance, weights, q.dwts);
     ring.wait();
     const float* row = ring.slot(at);
-    const bool counted = balance && !(in.mask && in.mask[t] == 0);
-    if (counted && t >= b_end) {
-      b = seq_at(t);
-      b_end = b < 0 ? t + 1 : in.seq ? in.seq[b + 1] : in.T;
-    }
+    const int b = balance && !(in.mask && in.mask[t] == 0) ? find(t) : -1;
     u64 d[N];
     float m = 0.f, inv = 0.f, k = 0.f;
     const int* cb = nullptr;  // the counts of a sequence other than the block's first and last
     const float* sf = b == b0 ? s_f : s_f + 128 * NV;
-    const bool term = counted && b >= 0;
+    const bool term = b >= 0;
     if (term) {
       u64 z2 = f32x2(0.f, 0.f), m2 = z2, slope[N];
       if (b != b0 && b != b1) {

@@ -281,7 +281,7 @@ BalanceLayout balance_layout(int T, int E, int B) {
   L.prob = take(slots * E * 4);
   L.count = take(slots * E * 4);
   L.rows = take(slots * 4);
-  L.term = take((size_t)B * cdiv(E, bal::COLS) * 4);
+  L.term = take((size_t)bal::JOIN_BLOCKS * 4);
   L.done = take(4);
   L.total = at;
   return L;
@@ -598,7 +598,7 @@ int k3moe_balance_loss(const float* S, int lds, const int32_t* idx, int T, int E
       rc = launch_overlapped(balance_rows_kernel<NV>, L.blocks, 32 * bal::ROW_WARPS, bytes, s, 1, in, w, L.chunk);
   });
   if (rc) return rc;
-  const long long blocks = (long long)B * cdiv(E, bal::COLS);
+  const long long blocks = std::min<long long>(bal::JOIN_BLOCKS, (long long)B * cdiv(E, bal::COLS));
   // a warp a partial row of the average sequence
   const int warps = (int)std::min<long long>(bal::JOIN_WARPS, cdiv(cdiv(L.blocks, B) + 1, 4) * 4);
   return launch_overlapped(balance_join_kernel, (unsigned)blocks, 32 * warps, 0, s, 1, in, w, L.chunk, alpha, counts,

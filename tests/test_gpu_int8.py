@@ -176,7 +176,7 @@ def test_permuted_codes(dev, R, K, E, first, shared, cols):
     (1, 1, 1), (1, 128, 128), (1, 4096, 7168), (2, 200, 16), (15, 129, 130), (16, 256, 300), (17, 300, 1000),
     (33, 64, 2047), (64, 7168, 2048), (65, 1003, 640), (100, 2048, 512), (129, 500, 1500), (255, 130, 128),
     (256, 4096, 256), (257, 4096, 129), (300, 4096, 7168), (1000, 896, 1024), (2049, 515, 333), (4096, 2048, 400),
-    (5, 40, 131071)])
+    (2305, 1803, 300), (4100, 1000, 2100), (20000, 130, 64), (260, 14400, 96), (5, 40, 131071)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_product_is_exact(dev, T, N, C, dtype):
     g = torch.Generator(device=dev).manual_seed(T + N + C)

@@ -39,7 +39,7 @@ def test_balance_scratch_covers_every_block_and_sequence(lib):
         nv = -(-E // 128)
         chunk = max(8, -(-T // (148 * (2 if nv <= 2 else 1))))
         blocks = max(1, -(-T // chunk))
-        need = (blocks + B) * E * 8 + (blocks + B) * 4 + B * -(-E // 32) * 4 + 4
+        need = (blocks + B) * E * 8 + (blocks + B) * 4 + 8 * 148 * 4 + 4
         got = lib.k3moe_balance_scratch_bytes(T, E, B)
         assert need <= got <= need + 5 * 256, (T, E, B)
 
