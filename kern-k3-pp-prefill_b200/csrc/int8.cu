@@ -323,8 +323,8 @@ __global__ void __launch_bounds__(LANES > 32 ? LANES : 256, MINB) quant_int8_ker
 // Tiles.  The MMA's M is 128 weight channels and its N the tokens (16 to 256 in steps of 16), so that a decode batch
 // or an expert's few rows cost what they are and not 128 rows: the weights, which bound those shapes, stream through
 // at full rate.  A stage is 128 K bytes (one swizzle atom) of both operands in an mbarrier ring; rows and K past the
-// ends are zero-filled by the loads.  Roles (320 threads): warp 0 lane 0 issues the TMA boxes, warp 1 lane 0 the MMAs
-// into one of two TMEM accumulators, warps 2-9 scale and store the other.  Every wait is bounded and reports.
+// ends are zero-filled by the loads.  Roles: warp 0 lane 0 issues the TMA boxes, warp 1 lane 0 the MMAs
+// into one of two TMEM accumulators, the other warps scale and store the other.  Every wait is bounded and reports.
 //
 // Where there are tokens enough (PAIR) two blocks share a unit of 256 channels x up to 256 tokens (cta_group::2): each
 // loads its 128 channels and half of the tokens, the even block issues M = 256 MMAs over both blocks' shared memory, and
@@ -340,9 +340,11 @@ constexpr int BK = 128;                  // K bytes a stage
 constexpr int W_BYTES = BM * BK;
 constexpr int RING_BYTES = 192 * 1024;
 constexpr int MAX_STAGES = 10;
-constexpr int EPI_WARPS = 8;
+constexpr int EPI_WARPS = 16;            // four a TMEM sub-partition
+constexpr int EPI_STEP = EPI_WARPS / 4 * 16;  // tokens they take in a turn
+constexpr int EPI_SCALES = 256 / (EPI_WARPS / 4);  // tokens of a warp
 constexpr int BAR_BYTES = 256;
-constexpr int SMEM_BYTES = RING_BYTES + 1024 /*align*/ + BAR_BYTES + EPI_WARPS * 128 * 4 /*token scales*/;
+constexpr int SMEM_BYTES = RING_BYTES + 1024 /*align*/ + BAR_BYTES + EPI_WARPS * EPI_SCALES * 4 /*token scales*/;
 constexpr int WARPS = 2 + EPI_WARPS;
 constexpr int THREADS = 32 * WARPS;
 }  // namespace i8
@@ -436,15 +438,26 @@ __device__ __forceinline__ int4 ld_cluster_v4(u32 saddr, u32 rank) {
   return v;
 }
 
-template <typename OUT>
-__device__ __forceinline__ OUT int8_value(u32 acc, float sx, float sw);
-template <>
-__device__ __forceinline__ float int8_value<float>(u32 acc, float sx, float sw) {
-  return __int2float_rn((int)acc) * sx * sw;
+// out = fl(fl(fl(acc) * sx) * sw), rounded once more to bf16
+__device__ __forceinline__ void int8_put(float* d, u32 acc, float sx, float sw) { *d = __int2float_rn((int)acc) * sx * sw; }
+__device__ __forceinline__ void int8_put(bf16* d, u32 acc, float sx, float sw) {
+  *d = __float2bfloat16_rn(__int2float_rn((int)acc) * sx * sw);
 }
-template <>
-__device__ __forceinline__ bf16 int8_value<bf16>(u32 acc, float sx, float sw) {
-  return __float2bfloat16_rn(__int2float_rn((int)acc) * sx * sw);
+// two tokens of one channel, at d and d + step
+__device__ __forceinline__ float2 int8_pair(u32 a0, u32 a1, u64 sx, u64 sw) {
+  return f32x2_get(mul_f32x2(mul_f32x2(f32x2(__int2float_rn((int)a0), __int2float_rn((int)a1)), sx), sw));
+}
+__device__ __forceinline__ void int8_put2(float* d, long long step, u32 a0, u32 a1, u64 sx, u64 sw) {
+  const float2 v = int8_pair(a0, a1, sx, sw);
+  d[0] = v.x;
+  d[step] = v.y;
+}
+__device__ __forceinline__ void int8_put2(bf16* d, long long step, u32 a0, u32 a1, u64 sx, u64 sw) {
+  const float2 v = int8_pair(a0, a1, sx, sw);
+  const u32 h = f2_to_bf16x2(v.x, v.y);
+  unsigned short* o = reinterpret_cast<unsigned short*>(d);
+  o[0] = (unsigned short)h;
+  o[step] = (unsigned short)(h >> 16);
 }
 
 template <typename OUT, bool PAIR>
@@ -461,7 +474,7 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
   u64* drain = bars + 2 * MAX_STAGES + 4;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * MAX_STAGES + 5);
   u32* tmem_slot = reinterpret_cast<u32*>(bars + 2 * MAX_STAGES + 6);
-  float* scales = reinterpret_cast<float*>(smem + RING_BYTES + BAR_BYTES);  // [EPI_WARPS][128]
+  float* scales = reinterpret_cast<float*>(smem + RING_BYTES + BAR_BYTES);  // [EPI_WARPS][EPI_SCALES]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 1) {
@@ -596,13 +609,13 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
       }
     }
   } else {
-    // ------------------------------------------------ epilogue (warps 2..9): a lane is a channel, columns are tokens;
-    // the two warps of a sub-partition take 16 tokens in turn, the next 16 on their way while these are scaled and
-    // stored (a token's 32 channels a warp store).  The tokens' scales come by broadcast from shared memory.
-    const int sub = warp & 3, half = (warp - 2) >> 2;
+    // ------------------------------------------------ epilogue (warps 2 on): a lane is a channel, columns are tokens;
+    // the warps of a sub-partition take 16 tokens in turn, the next 16 on their way while these are scaled and stored
+    // (a token's 32 channels a warp store).  The tokens' scales come by broadcast from shared memory.
+    const int sub = warp & 3, turn = (warp - 2) >> 2;
     const u32 lane_base = (u32)(sub * 32) << 16;
     int* red = reinterpret_cast<int*>(smem);
-    float* sxs = scales + (warp - 2) * 128;  // this warp's tokens: 16 of every 32
+    float* sxs = scales + (warp - 2) * EPI_SCALES;  // this warp's tokens: 16 of every EPI_STEP
     const long long row_step = p.ldo;
     u32 acc_phase = 0;
     int buf = 0;
@@ -611,44 +624,44 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
       if (!w.valid) continue;
       const int ch = w.ch0 + sub * 32 + lane;
       const float swc = ch < p.N ? p.sw[(long long)w.e * p.N + ch] : 0.f;
-      for (int i = lane; i < 128; i += 32) {
-        const int t = (i >> 4) * 32 + half * 16 + (i & 15);
+      for (int i = lane; i < EPI_SCALES; i += 32) {
+        const int t = (i >> 4) * EPI_STEP + turn * 16 + (i & 15);
         sxs[i] = t < w.n ? p.sx[w.row0 + t] : 0.f;
       }
       __syncwarp();
       if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[buf], (acc_phase >> buf) & 1u, abort_flag, p.err, 0xD60u))) break;
       tc_fence_after();
       const u32 acc = tmem_base + lane_base + (u32)(buf * p.bn);
-      int c = half * 16;
+      int c = turn * 16;
       u32 v[16];
       if (c < w.n) i8_ld16(acc + (u32)c, v);
       OUT* dst = reinterpret_cast<OUT*>(p.out) + ((long long)w.row0 + c) * row_step + ch;
       const float* sx = sxs;
       const bool whole = w.ch0 + BM <= p.N;
 #pragma unroll 1
-      for (; c < w.n; c += 32, dst += 32 * row_step, sx += 16) {
+      for (; c < w.n; c += EPI_STEP, dst += EPI_STEP * row_step, sx += 16) {
         tmem_wait_ld();
         u32 x[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] = v[j];
-        if (c + 32 < w.n) i8_ld16(acc + (u32)(c + 32), v);
+        if (c + EPI_STEP < w.n) i8_ld16(acc + (u32)(c + EPI_STEP), v);
         if (!PAIR && p.splits > 1) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) red[(c + j) * BM + sub * 32 + lane] = (int)x[j];
         } else if (whole && c + 16 <= w.n) {
           OUT* d = dst;
+          const u64 sw2 = f32x2(swc, swc);
 #pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            const float4 s = *reinterpret_cast<const float4*>(sx + j);
-            const float q[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i, d += row_step) *d = int8_value<OUT>(x[j + i], q[i], swc);
+          for (int j = 0; j < 16; j += 4, d += 4 * row_step) {
+            const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(sx + j);
+            int8_put2(d, row_step, x[j], x[j + 1], q.x, sw2);
+            int8_put2(d + 2 * row_step, row_step, x[j + 2], x[j + 3], q.y, sw2);
           }
         } else {
           OUT* d = dst;
 #pragma unroll
           for (int j = 0; j < 16; ++j, d += row_step)
-            if (ch < p.N && c + j < w.n) *d = int8_value<OUT>(x[j], sx[j], swc);
+            if (ch < p.N && c + j < w.n) int8_put(d, x[j], sx[j], swc);
         }
       }
       tc_fence_before();
@@ -689,7 +702,7 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
       OUT* dst = reinterpret_cast<OUT*>(p.out) + ((long long)w.row0 + t) * p.ldo + ch;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (ch + i < p.N) dst[i] = int8_value<OUT>((u32)q[i], s, p.sw[ch + i]);
+        if (ch + i < p.N) int8_put(dst + i, (u32)q[i], s, p.sw[ch + i]);
     }
     cluster_sync();  // no block leaves while another reads its part
   }
