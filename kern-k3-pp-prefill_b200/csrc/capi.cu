@@ -331,7 +331,8 @@ template <int SRC, int LANES, int NV, int MINB>
 int launch_quant_int8(const QuantRows& p, cudaStream_t s) {
   const int threads = LANES > 32 ? LANES : 256;
   const long long blocks = cdiv(p.rows, threads / LANES);
-  const int grid = (int)std::min<long long>(blocks, (long long)num_sms(current_device()) * MINB);
+  const int grid = p.cta_limit ? 16 * (int)std::min<long long>(p.max_ctas, cdiv(p.rows, 128))
+                               : (int)std::min<long long>(blocks, (long long)num_sms(current_device()) * MINB);
   return launch_overlapped(p.vec && p.cols % 8 == 0 ? quant_int8_kernel<SRC, LANES, NV, MINB, true>
                                                     : quant_int8_kernel<SRC, LANES, NV, MINB, false>,
                            grid, threads, 0, s, 1, p);
@@ -693,7 +694,7 @@ int k3moe_act_quant_int8(const void* gu_bf16, long long ldg, long long rows, int
                          const int32_t* cta_limit, const int32_t* meta, int max_ctas, int8_t* q, long long ldq,
                          float* scale, k3moe_stream_t stream) {
   if (rows < 0 || I < 1 || ldg < 2LL * I || (activation != K3MOE_ACT_SWIGLU && activation != K3MOE_ACT_SITU) ||
-      (cta_limit == nullptr) != (meta == nullptr) || (meta && max_ctas < 1))
+      (cta_limit == nullptr) != (meta == nullptr) || (meta && (max_ctas < 1 || max_ctas > 1 << 26)))
     return K3MOE_EINVAL;
   if (rows == 0) return K3MOE_OK;
   if (!gu_bf16 || !scale || !int8_rows_ok(q, ldq, I)) return K3MOE_EINVAL;
@@ -782,8 +783,10 @@ int k3moe_grouped_gemm_int8(const int8_t* q_perm, long long ldq, const float* sx
   p.ldo = ldo;
   p.N = N;
   p.err = err;
+  // a pair of blocks on 256 channels of a tile, unless their number would leave too many of the pair's blocks idle
+  const bool pair = 10 * 2 * cdiv(N, 2 * i8::BM) <= 12 * cdiv(N, i8::BM);
   p.bn = 128;
-  p.xbox = 32;
+  p.xbox = pair ? 64 : 32;
   p.splits = 1;
   p.cta_batch = cta_batch;
   p.cta_limit = cta_limit;
@@ -791,8 +794,10 @@ int k3moe_grouped_gemm_int8(const int8_t* q_perm, long long ldq, const float* sx
   p.n_experts = n_experts;
   p.max_ctas = max_ctas;
   p.cap_rows = cap_rows;
-  const int grid = (int)std::min<long long>(max_ctas * cdiv(N, i8::BM), num_sms(current_device()));
-  return int8_launch(q_perm, cap_rows, ldq, w, (long long)n_experts * N, ldw, C, p, false, dtype, grid,
+  const int sms = num_sms(current_device());
+  const int grid = pair ? 2 * (int)std::min<long long>(max_ctas * cdiv(N, 2 * i8::BM), sms / 2)
+                        : (int)std::min<long long>(max_ctas * cdiv(N, i8::BM), sms);
+  return int8_launch(q_perm, cap_rows, ldq, w, (long long)n_experts * N, ldw, C, p, pair, dtype, grid,
                      reinterpret_cast<cudaStream_t>(stream));
 }
 

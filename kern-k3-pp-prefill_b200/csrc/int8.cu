@@ -231,12 +231,18 @@ __global__ void __launch_bounds__(LANES > 32 ? LANES : 256, MINB) quant_int8_ker
   const int lane = threadIdx.x % LANES, sub = threadIdx.x / LANES;
   grid_wait_previous();
   grid_launch_dependents();
-  const int nne = p.cta_limit ? min(p.meta[0], p.max_ctas) : 0;
+  long long first = (long long)blockIdx.x * PER + sub, last = p.rows, next = (long long)gridDim.x * PER;
+  if (p.cta_limit) {  // sixteen blocks a tile of 128 rows, over its real ones
+    const int c = blockIdx.x >> 4;
+    if (c >= min(p.meta[0], p.max_ctas)) return;
+    first = c * 128ll + (blockIdx.x & 15) * PER + sub;
+    last = min(last, min((long long)p.cta_limit[c], c * 128ll + 128));
+    next = 16 * PER;
+  }
   const int shared_row = p.exp2perm ? p.meta[2] : -1;
   const long long row_bytes = p.ldx * (SRC == I8_F32 ? 4 : 2);
   int buf = 0;
-  for (long long r = (long long)blockIdx.x * PER + sub; r < p.rows; r += (long long)gridDim.x * PER) {
-    if (p.cta_limit && ((r >> 7) >= nne || r >= p.cta_limit[r >> 7])) continue;  // the row's LANES threads together
+  for (long long r = first; r < last; r += next) {
     // lane k of a warp holds the row's k-th target, loaded ahead of its elements
     int target = -1;
     if (p.exp2perm) {
@@ -326,7 +332,7 @@ __global__ void __launch_bounds__(LANES > 32 ? LANES : 256, MINB) quant_int8_ker
 // ends are zero-filled by the loads.  Roles: warp 0 lane 0 issues the TMA boxes, warp 1 lane 0 the MMAs
 // into one of two TMEM accumulators, the other warps scale and store the other.  Every wait is bounded and reports.
 //
-// Where there are tokens enough (PAIR) two blocks share a unit of 256 channels x up to 256 tokens (cta_group::2): each
+// Where there is work enough (PAIR) two blocks share a unit of 256 channels x up to 256 tokens (cta_group::2): each
 // loads its 128 channels and half of the tokens, the even block issues M = 256 MMAs over both blocks' shared memory, and
 // each drains its own channels.  One block alone would write and read 96 KB of shared memory for the 512 MMA cycles of a
 // stage, more than its 128 bytes a cycle; a pair halves the tokens' part.
@@ -379,7 +385,7 @@ __device__ __forceinline__ Int8Unit int8_unit(const Int8Params& p, int u, int ra
   Int8Unit w;
   const int c = u / p.n_tiles;
   w.ch0 = PAIR ? (u % p.n_tiles) * 2 * i8::BM + rank * i8::BM : (u % p.n_tiles) * i8::BM;
-  if (!PAIR && p.cta_batch) {
+  if (p.cta_batch) {
     w.e = p.cta_batch[c];
     w.row0 = c * 128;
     w.n = p.cta_limit[c] - w.row0;

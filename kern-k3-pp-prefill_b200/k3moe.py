@@ -496,8 +496,8 @@ def route_backward(S: torch.Tensor, idx: torch.Tensor, alpha: float = 0.0, count
 def _int8_out(rows: int, cols: int, dev, out):
     if out is None:
         ld = -(-cols // 16) * 16
-        q = _empty(rows, ld, dtype=torch.int8, device=dev)
-        return q if ld == cols else q[:, :cols], ld, _empty(rows, dtype=torch.float32, device=dev)
+        q = torch.empty_strided((rows, cols), (ld, 1), dtype=torch.int8, device=dev)
+        return q, ld, _empty(rows, dtype=torch.float32, device=dev)
     q, scale = out
     ld = _int8_rows(q, "out q", dev, cols, rows)
     _vec(scale, "out scale", _F32, rows, dev)
