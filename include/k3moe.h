@@ -360,7 +360,8 @@ int k3moe_quant_int8_permute(const void* x_bf16, long long ldx, int R, int cols,
                              k3moe_stream_t stream);
 /* out[t, n] = sx[t] * sw[n] * sum_c q[t, c] w[n, c]: int8 x int8 on the tensor cores, the int32 sum exact, then two f32
  * products and (dtype K3MOE_BF16) one rounding.  q [T, ldq], w [N, ldw], both 16-byte aligned with leading dimensions
- * a multiple of 16; out [T, ldo].  C (the reduction length) in [1, 131071]: -128 * -128 * C stays inside int32.
+ * a multiple of 16; out [T, ldo].  C (the reduction length) in [1, 131071]: -128 * -128 * C stays inside int32.  T and N
+ * (n_experts * N below) up to 2^31 - 256.
  * err: the device error words (a bounded wait that ran out), or null. */
 int k3moe_gemm_int8(const int8_t* q, long long ldq, const float* sx, const int8_t* w, long long ldw, const float* sw,
                     int T, int N, int C, void* out, long long ldo, int dtype, uint32_t* err, k3moe_stream_t stream);

@@ -163,6 +163,15 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// the sums of N values each over the warp, side by side
+template <int N>
+__device__ __forceinline__ void warp_sums(float (&v)[N]) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], d);
+}
+
 // ---------------------------------------------------------------- forward
 // First pass: a block takes `chunk` consecutive rows, a warp every sixteenth of them, each lane summing its experts' p in
 // registers.  At the end of a sequence, or of the block's rows, the warps' sums are added in order and stored as one
@@ -172,9 +181,123 @@ struct BalanceScratch {
   float* prob;   // [slots, E]
   int* count;    // [slots, E]
   int* rows;     // [slots]
-  float* term;   // [blocks of the second pass]
+  float2* term;  // [blocks of the second pass]: sum of terms, sequences with a counted row
   u32* done;
 };
+
+// Second pass: a team (a warp, where few of the first pass's blocks meet a sequence, or a block) adds up 32 experts of one
+// sequence over the blocks that met it, its warps side by side and joined in order, then the next such group of its
+// share; the last block of all adds up the loss.
+struct BalanceOut {
+  float alpha;
+  int* counts;   // [B, E]
+  float* prob;   // [B, E]
+  int* rows;     // [B]
+  float* loss;
+};
+template <bool WARP_TEAM>
+__global__ void __launch_bounds__(32 * bal::JOIN_WARPS)
+    balance_join_kernel(RouterRows in, BalanceScratch w, int chunk, BalanceOut out) {
+  using namespace bal;
+  __shared__ float s_p[JOIN_WARPS][COLS];
+  __shared__ int s_c[JOIN_WARPS][COLS], s_n[JOIN_WARPS];
+  __shared__ int s_last;
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int groups = (in.E + COLS - 1) / COLS;
+  const int lo = in.seq ? max(in.seq[0], 0) : 0, hi = in.seq ? min(in.seq[in.B], in.T) : in.T;
+  const long long first = WARP_TEAM ? (long long)blockIdx.x * warps + warp : blockIdx.x;
+  const long long step = WARP_TEAM ? (long long)gridDim.x * warps : gridDim.x;
+  float terms = 0.f;
+  int full = 0;  // sequences with a counted row
+  bool waited = false;
+  for (long long unit = first; unit < (long long)in.B * groups; unit += step) {
+    const int b = (int)(unit / groups), g = (int)(unit % groups), e = g * COLS + lane;
+    const int s0 = in.seq ? max(lo, in.seq[b]) : lo, s1 = in.seq ? min(hi, in.seq[b + 1]) : hi;
+    // the first pass's partial rows (it lets this one start after its own wait: the offsets are there before)
+    if (!waited) grid_wait_previous();
+    waited = true;
+    float p = 0.f;
+    int c = 0, n = 0;
+    if (s0 < s1) {
+      const int i1 = (s1 - 1) / chunk;
+#pragma unroll 5
+      for (int i = s0 / chunk + (WARP_TEAM ? 0 : warp); i <= i1; i += WARP_TEAM ? 1 : warps) {
+        const long long slot = (long long)i + b;
+        if (e < in.E) {
+          p += w.prob[slot * in.E + e];
+          c += w.count[slot * in.E + e];
+        }
+        n += w.rows[slot];
+      }
+    }
+    if (!WARP_TEAM) {
+      __syncthreads();  // the group before has been read
+      s_p[warp][lane] = p;
+      s_c[warp][lane] = c;
+      if (lane == 0) s_n[warp] = n;
+      __syncthreads();
+      for (int k = 1; warp == 0 && k < warps; ++k) {
+        p += s_p[k][lane];
+        c += s_c[k][lane];
+        n += s_n[k];
+      }
+    }
+    if (WARP_TEAM || warp == 0) {
+      float term = 0.f;
+      if (e < in.E) {
+        out.counts[(long long)b * in.E + e] = c;
+        out.prob[(long long)b * in.E + e] = p;
+        if (n > 0) term = ((float)in.E * (float)c / ((float)in.K * (float)n)) * (p / (float)n);
+      }
+      terms += term;
+      if (g == 0) {
+        full += n > 0;
+        if (lane == 0) out.rows[b] = n;
+      }
+    }
+  }
+  if (!waited) grid_wait_previous();
+  terms = warp_sum(terms);
+  __syncthreads();
+  if (lane == 0) {
+    s_p[warp][0] = terms;
+    s_c[warp][0] = full;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < warps; ++k) {
+      terms += s_p[k][0];
+      full += s_c[k][0];
+    }
+    w.term[blockIdx.x] = make_float2(terms, __int_as_float(full));
+    __threadfence();
+    s_last = atomicAdd(w.done, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  terms = 0.f;
+  full = 0;
+  for (int i = threadIdx.x; i < gridDim.x; i += blockDim.x) {
+    const float2 t = __ldcg(&w.term[i]);
+    terms += t.x;
+    full += __float_as_int(t.y);
+  }
+  terms = warp_sum(terms);
+  full = __reduce_add_sync(0xffffffffu, full);
+  if (lane == 0) {
+    s_p[warp][1] = terms;
+    s_c[warp][1] = full;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < warps; ++k) {
+      terms += s_p[k][1];
+      full += s_c[k][1];
+    }
+    *out.loss = out.alpha * terms / (float)max(full, 1);
+  }
+}
 
 template <int NV>
 __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
@@ -273,88 +396,6 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
   cp_async_wait_all();
 }
 
-// Second pass: a block adds up 32 experts of one sequence over the first pass's blocks that met it (its warps side by
-// side, joined in order), then the next such group of its share; the last block of all adds up the loss.
-__global__ void __launch_bounds__(32 * bal::JOIN_WARPS)
-    balance_join_kernel(RouterRows in, BalanceScratch w, int chunk, float alpha, int* __restrict__ counts,
-                        float* __restrict__ prob, int* __restrict__ rows, float* __restrict__ loss) {
-  using namespace bal;
-  const int warps = blockDim.x >> 5;
-  __shared__ float s_p[JOIN_WARPS][COLS];
-  __shared__ int s_c[JOIN_WARPS][COLS], s_n[JOIN_WARPS];
-  __shared__ int s_last;
-  const int groups = (in.E + COLS - 1) / COLS;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int lo = in.seq ? max(in.seq[0], 0) : 0, hi = in.seq ? min(in.seq[in.B], in.T) : in.T;
-  float terms = 0.f;
-  for (int unit = blockIdx.x; unit < in.B * groups; unit += gridDim.x) {
-    const int b = unit / groups, g = unit % groups, e = g * COLS + lane;
-    const int s0 = in.seq ? max(lo, in.seq[b]) : lo, s1 = in.seq ? min(hi, in.seq[b + 1]) : hi;
-    // the first pass's partial rows (it lets this one start after its own wait: the offsets are there before)
-    if (unit == blockIdx.x) grid_wait_previous();
-    float p = 0.f;
-    int c = 0, n = 0;
-    if (s0 < s1) {
-      const int i1 = (s1 - 1) / chunk;
-#pragma unroll 5
-      for (int i = s0 / chunk + warp; i <= i1; i += warps) {
-        const long long slot = (long long)i + b;
-        if (e < in.E) {
-          p += w.prob[slot * in.E + e];
-          c += w.count[slot * in.E + e];
-        }
-        n += w.rows[slot];
-      }
-    }
-    s_p[warp][lane] = p;
-    s_c[warp][lane] = c;
-    if (lane == 0) s_n[warp] = n;
-    __syncthreads();
-    if (warp == 0) {
-      for (int k = 1; k < warps; ++k) {
-        p += s_p[k][lane];
-        c += s_c[k][lane];
-        n += s_n[k];
-      }
-      float term = 0.f;
-      if (e < in.E) {
-        counts[(long long)b * in.E + e] = c;
-        prob[(long long)b * in.E + e] = p;
-        if (n > 0) term = ((float)in.E * (float)c / ((float)in.K * (float)n)) * (p / (float)n);
-      }
-      terms += warp_sum(term);
-      if (lane == 0 && g == 0) rows[b] = n;
-    }
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) {
-    w.term[blockIdx.x] = terms;
-    __threadfence();
-    s_last = atomicAdd(w.done, 1u) == gridDim.x - 1;
-  }
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  float sum = 0.f;
-  int full = 0;
-  for (int i = threadIdx.x; i < gridDim.x; i += blockDim.x) sum += __ldcg(&w.term[i]);
-  for (int i = threadIdx.x; i < in.B; i += blockDim.x) full += __ldcg(&rows[i]) > 0;
-  sum = warp_sum(sum);
-  full = __reduce_add_sync(0xffffffffu, full);
-  if (lane == 0) {
-    s_p[warp][0] = sum;
-    s_c[warp][0] = full;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int k = 1; k < warps; ++k) {
-      sum += s_p[k][0];
-      full += s_c[k][0];
-    }
-    *loss = alpha * sum / (float)max(full, 1);
-  }
-}
-
 // ---------------------------------------------------------------- backward
 struct RouteBackward {
   float alpha;
@@ -436,13 +477,33 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
     ring.wait();
     const float* row = ring.slot(at);
     const int b = balance && !(in.mask && in.mask[t] == 0) ? find(t) : -1;
-    u64 d[N];
-    float m = 0.f, inv = 0.f, k = 0.f;
+    const bool term = b >= 0;
+    // the lane's pick: its logit, score and slope, and the gradient of its weight
+    int e = -1;
+    float g = 0.f, pick = 0.f, pick_slope = 0.f;
+    u32 peers = 0;
+    if (weights) {
+      float x = 0.f;
+      if (lane < in.K) {
+        e = reinterpret_cast<const int*>(row + 128 * NV)[lane];
+        if (e < 0 || e >= in.E) e = -1;
+        if (e >= 0) {
+          x = balance ? row[e] : in.S[t * in.lds + e];
+          g = row[128 * NV + PICKS + lane];
+        }
+      }
+      const u64 ex = exp_neg2(f32x2(x, x)), sc = score2(ex);
+      pick = e >= 0 ? f32x2_get(sc).x : 0.f;
+      pick_slope = f32x2_get(slope2(sc, ex)).x;
+      peers = __match_any_sync(0xffffffffu, e);
+    }
+    u64 d[N], slope[N];
+    float k = 0.f;
     const int* cb = nullptr;  // the counts of a sequence other than the block's first and last
     const float* sf = b == b0 ? s_f : s_f + 128 * NV;
-    const bool term = b >= 0;
+    float sums[4] = {0.f, 0.f, pick, g * pick};  // of scores, f scores; of the picks' scores, and with their gradients
     if (term) {
-      u64 z2 = f32x2(0.f, 0.f), m2 = z2, slope[N];
+      u64 z2 = f32x2(0.f, 0.f), m2 = z2;
       if (b != b0 && b != b1) {
         const int n = q.rows[b];
         k = n > 0 ? scale / (float)n / (float)n : 0.f;
@@ -460,24 +521,28 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
         if (cb == nullptr) {
           f = *reinterpret_cast<const ulonglong2*>(sf + c);
         } else {
-          int4 g = make_int4(0, 0, 0, 0);
+          int4 n = make_int4(0, 0, 0, 0);
           if (vec_counts) {
-            if (c < in.E) g = *reinterpret_cast<const int4*>(cb + c);
+            if (c < in.E) n = *reinterpret_cast<const int4*>(cb + c);
           } else {
-            g.x = c < in.E ? cb[c] : 0;
-            g.y = c + 1 < in.E ? cb[c + 1] : 0;
-            g.z = c + 2 < in.E ? cb[c + 2] : 0;
-            g.w = c + 3 < in.E ? cb[c + 3] : 0;
+            n.x = c < in.E ? cb[c] : 0;
+            n.y = c + 1 < in.E ? cb[c + 1] : 0;
+            n.z = c + 2 < in.E ? cb[c + 2] : 0;
+            n.w = c + 3 < in.E ? cb[c + 3] : 0;
           }
-          f = make_ulonglong2(f32x2(k * (float)g.x, k * (float)g.y), f32x2(k * (float)g.z, k * (float)g.w));
+          f = make_ulonglong2(f32x2(k * (float)n.x, k * (float)n.y), f32x2(k * (float)n.z, k * (float)n.w));
         }
         m2 = fma_f32x2(f.x, s0, fma_f32x2(f.y, s1, m2));
         d[2 * j] = f.x;
         d[2 * j + 1] = f.y;
       }
-      const float2 z = f32x2_get(z2), mm = f32x2_get(m2);
-      inv = rcp_ftz(warp_sum(z.x + z.y) + TINY);
-      m = warp_sum(mm.x + mm.y) * inv;
+      const float2 z = f32x2_get(z2), m = f32x2_get(m2);
+      sums[0] = z.x + z.y;
+      sums[1] = m.x + m.y;
+    }
+    warp_sums(sums);
+    const float inv = rcp_ftz(sums[0] + TINY), m = sums[1] * inv;
+    if (term) {
       const u64 minus = f32x2(-m, -m), inv2 = f32x2(inv, inv);
 #pragma unroll
       for (int i = 0; i < N; ++i) d[i] = mul_f32x2(add_f32x2(d[i], minus), mul_f32x2(slope[i], inv2));
@@ -485,29 +550,15 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
 #pragma unroll
       for (int i = 0; i < N; ++i) d[i] = 0ull;
     }
-    // the lane's pick: its element's sum of both terms, stored over the balance term alone
-    int e = -1;
+    // the pick's element: the sum of both terms, stored over the balance term alone
     float total = 0.f;
     if (weights) {
-      float x = 0.f, g = 0.f, f = 0.f;
-      if (lane < in.K) {
-        e = reinterpret_cast<const int*>(row + 128 * NV)[lane];
-        if (e < 0 || e >= in.E) e = -1;
-        if (e >= 0) {
-          x = balance ? row[e] : in.S[t * in.lds + e];
-          g = row[128 * NV + PICKS + lane];
-          f = !term ? 0.f : cb == nullptr ? sf[e] : k * (float)cb[e];
-        }
-      }
-      const u64 ex = exp_neg2(f32x2(x, x)), sc = score2(ex);
-      const float s = e >= 0 ? f32x2_get(sc).x : 0.f, slope = f32x2_get(slope2(sc, ex)).x;
-      const float den = rcp_ftz(warp_sum(s) + TINY);
-      const float mean = warp_sum(g * s) * den;
-      const float mine = rs * den * (g - mean) * slope;
-      const float base = term ? (f - m) * (slope * inv) : 0.f;
+      const float den = rcp_ftz(sums[2] + TINY);
+      const float mine = rs * den * (g - sums[3] * den) * pick_slope;
+      const float f = !term || e < 0 ? 0.f : cb == nullptr ? sf[e] : k * (float)cb[e];
+      const float base = term ? (f - m) * (pick_slope * inv) : 0.f;
       total = base + mine;
       // an expert named twice gets both parts, added in pick order
-      const u32 peers = __match_any_sync(0xffffffffu, e);
       if (!__all_sync(0xffffffffu, e < 0 || (peers & (peers - 1)) == 0)) {
         total = base;
         for (int i = 0; i < in.K; ++i) {

@@ -281,7 +281,7 @@ BalanceLayout balance_layout(int T, int E, int B) {
   L.prob = take(slots * E * 4);
   L.count = take(slots * E * 4);
   L.rows = take(slots * 4);
-  L.term = take((size_t)bal::JOIN_BLOCKS * 4);
+  L.term = take((size_t)bal::JOIN_BLOCKS * 8);
   L.done = take(4);
   L.total = at;
   return L;
@@ -344,12 +344,14 @@ int quant_int8(const QuantRows& p, cudaStream_t s) {
   if (p.rows == 0) return K3MOE_OK;
   if (p.cols <= 512) return launch_quant_int8<SRC, 32, 2, 5>(p, s);
   if (p.cols <= 1024) return launch_quant_int8<SRC, 32, 4, 4>(p, s);
-  if (p.cols <= 2048) return launch_quant_int8<SRC, 128, 2, 10>(p, s);
+  if (p.cols <= 2048) return launch_quant_int8<SRC, 128, 2, 12>(p, s);
   if (p.cols <= 4096) return launch_quant_int8<SRC, 128, 4, SRC == I8_BF16 ? 10 : 7>(p, s);
-  if (p.cols <= 8192) return launch_quant_int8<SRC, 256, 4, SRC == I8_BF16 ? 5 : 3>(p, s);
+  if (p.cols <= 8192) return launch_quant_int8<SRC, 256, 4, SRC == I8_BF16 ? 6 : 3>(p, s);
   if (p.cols <= 16384) return launch_quant_int8<SRC, 512, 4, SRC == I8_BF16 ? 2 : 1>(p, s);
   return launch_quant_int8<SRC, 512, 0, 2>(p, s);
 }
+
+constexpr int kInt8Rows = 0x7fffff00;  // tokens or channels: a tile's last row stays an int
 
 bool int8_rows_ok(const void* q, long long ldq, int cols) {
   return q && reinterpret_cast<uintptr_t>(q) % 16 == 0 && ldq % 16 == 0 && cols >= 1 && ldq >= cols;
@@ -620,10 +622,11 @@ int k3moe_balance_loss(const float* S, int lds, const int32_t* idx, int T, int E
   w.prob = reinterpret_cast<float*>(ws + L.prob);
   w.count = reinterpret_cast<int*>(ws + L.count);
   w.rows = reinterpret_cast<int*>(ws + L.rows);
-  w.term = reinterpret_cast<float*>(ws + L.term);
+  w.term = reinterpret_cast<float2*>(ws + L.term);
   w.done = reinterpret_cast<u32*>(ws + L.done);
   const RouterRows in = router_rows(S, lds, idx, T, E, K, seq, B, mask);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const BalanceOut out = {alpha, counts, prob, rows, loss};
   int rc = K3MOE_ELAUNCH;
   by_experts(E, [&](auto nv) {
     constexpr int NV = decltype(nv)::value, bytes = bal::rows_smem(NV);
@@ -631,11 +634,14 @@ int k3moe_balance_loss(const float* S, int lds, const int32_t* idx, int T, int E
       rc = launch_overlapped(balance_rows_kernel<NV>, L.blocks, 32 * bal::ROW_WARPS, bytes, s, 1, in, w, L.chunk);
   });
   if (rc) return rc;
-  const long long blocks = std::min<long long>(bal::JOIN_BLOCKS, (long long)B * cdiv(E, bal::COLS));
-  // a warp a partial row of the average sequence
-  const int warps = (int)std::min<long long>(bal::JOIN_WARPS, cdiv(cdiv(L.blocks, B) + 1, 4) * 4);
-  return launch_overlapped(balance_join_kernel, (unsigned)blocks, 32 * warps, 0, s, 1, in, w, L.chunk, alpha, counts,
-                           prob, rows, loss);
+  // the average sequence's partial rows: up to four, a warp adds them up by itself; else a warp a row
+  const long long units = (long long)B * cdiv(E, bal::COLS);
+  const int partial = (int)cdiv(L.blocks, B) + 1;
+  if (partial <= 4)
+    return launch_overlapped(balance_join_kernel<true>, (unsigned)std::min<long long>(bal::JOIN_BLOCKS, cdiv(units, 8)),
+                             256, 0, s, 1, in, w, L.chunk, out);
+  return launch_overlapped(balance_join_kernel<false>, (unsigned)std::min<long long>(bal::JOIN_BLOCKS, units),
+                           32 * std::min(bal::JOIN_WARPS, (partial + 3) / 4 * 4), 0, s, 1, in, w, L.chunk, out);
 }
 
 int k3moe_route_backward(const float* S, int lds, const int32_t* idx, int T, int E, int K, const int32_t* seq, int B,
@@ -739,7 +745,7 @@ int k3moe_quant_int8_permute(const void* x_bf16, long long ldx, int R, int cols,
 
 int k3moe_gemm_int8(const int8_t* q, long long ldq, const float* sx, const int8_t* w, long long ldw, const float* sw,
                     int T, int N, int C, void* out, long long ldo, int dtype, uint32_t* err, k3moe_stream_t stream) {
-  if (T < 0 || N < 1 || C < 1 || C > 131071 || ldo < N || (dtype != K3MOE_BF16 && dtype != K3MOE_F32))
+  if (T < 0 || T > kInt8Rows || N < 1 || N > kInt8Rows || C < 1 || C > 131071 || ldo < N || (dtype != K3MOE_BF16 && dtype != K3MOE_F32))
     return K3MOE_EINVAL;
   if (T == 0) return K3MOE_OK;
   if (!sx || !sw || !out || !int8_rows_ok(q, ldq, C) || !int8_rows_ok(w, ldw, C) ||
@@ -773,7 +779,7 @@ int k3moe_grouped_gemm_int8(const int8_t* q_perm, long long ldq, const float* sx
   if (N < 1 || C < 1 || C > 131071 || n_experts < 1 || max_ctas < 1 || (long long)max_ctas * 128 > cap_rows ||
       ldo < N || (dtype != K3MOE_BF16 && dtype != K3MOE_F32) || !sx_perm || !sw || !cta_batch || !cta_limit || !meta ||
       !out || !int8_rows_ok(q_perm, ldq, C) || !int8_rows_ok(w, ldw, C) ||
-      reinterpret_cast<uintptr_t>(out) % (dtype == K3MOE_F32 ? 4 : 2) || (long long)n_experts * N > 0x7fffffffLL ||
+      reinterpret_cast<uintptr_t>(out) % (dtype == K3MOE_F32 ? 4 : 2) || (long long)n_experts * N > kInt8Rows ||
       max_ctas * cdiv(N, i8::BM) > 0x7fffffffLL)
     return K3MOE_EINVAL;
   Int8Params p = {};

@@ -231,6 +231,16 @@ __device__ __forceinline__ float rcp_ftz(float x) {
 }
 constexpr float LOG2E = 1.4426950408889634f;
 
+// ---------------------------------------------------------------- clusters
+__device__ __forceinline__ u32 cluster_rank() {
+  u32 r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
+}
+
 // ---------------------------------------------------------------- programmatic dependent launch
 // Let the next kernel of the stream start its prologue once every block of this one has come here or ended ...
 __device__ __forceinline__ void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

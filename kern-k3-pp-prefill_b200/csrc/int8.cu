@@ -426,14 +426,6 @@ __device__ __forceinline__ void i8_ld16(u32 taddr, u32 (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ u32 cluster_rank() {
-  u32 r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
-}
 __device__ __forceinline__ int4 ld_cluster_v4(u32 saddr, u32 rank) {
   int4 v;
   asm volatile(

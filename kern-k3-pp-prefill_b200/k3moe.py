@@ -398,6 +398,13 @@ def _launch(fn, what: str, dev, *args) -> None:
         _check(rc, what)
 
 
+def _on(stream, t):
+    """The context of the entries' `stream` argument: the call, its allocations included, on that stream."""
+    if stream.device != t.device:
+        raise K3MoeError(f"stream: on {stream.device}, the tensors on {t.device}")
+    return torch.cuda.stream(stream)
+
+
 def _out_dtype(dtype) -> int:
     if dtype is torch.bfloat16:
         return BF16
@@ -445,7 +452,7 @@ def balance_loss(S: torch.Tensor, idx: torch.Tensor, alpha: float, seq: torch.Te
     S f32 [T, E] router logits; idx int32 [T, K] (route_topk's); seq int32 [B + 1] offsets of packed sequences (None:
     one sequence); mask [T] uint8 or bool, rows with 0 are not counted."""
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _on(stream, S):
             return balance_loss(S, idx, alpha, seq, mask)
     dev, T, E, K, B, ld = _router_args(S, idx, seq, mask)
     L = lib()
@@ -468,7 +475,7 @@ def route_backward(S: torch.Tensor, idx: torch.Tensor, alpha: float = 0.0, count
     and mask) are given, dloss its scalar gradient (None: 1); plus the weight term where dwts [T, K], the gradient of
     route_topk's weights, and rs are given."""
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _on(stream, S):
             return route_backward(S, idx, alpha, counts, rows, dloss, dwts, rs, seq, mask, dtype, out)
     dev, T, E, K, B, ld = _router_args(S, idx, seq, mask)
     if counts is not None and rows is not None:
@@ -508,7 +515,7 @@ def quant_int8(x: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = 
     """Rows of x (bf16 or f32 [rows, cols]; tokens, or a weight's channels) to int8 with a scale each
     (k3moe_quant_int8): (q int8 [rows, cols], its rows padded to 16 bytes; scale f32 [rows])."""
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _on(stream, x):
             return quant_int8(x, out)
     ldx = _rows(x, "x", _FLOATS)
     rows, cols = x.shape
@@ -524,7 +531,7 @@ def act_quant_int8(gu: torch.Tensor, activation: int = ACT_SWIGLU, tables: Table
     """act(gate) * up of bf16 rows [gate | up] to int8 (k3moe_act_quant_int8): (q [rows, cols / 2], scale).  With
     tables, gu is [cap_rows, 2I] and only the tables' real rows are read and written."""
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _on(stream, gu):
             return act_quant_int8(gu, activation, tables, out)
     ldg = _rows(gu, "gu", _BF16)
     rows, cols = gu.shape
@@ -544,11 +551,12 @@ def act_quant_int8(gu: torch.Tensor, activation: int = ACT_SWIGLU, tables: Table
     return q, scale
 
 
-def quant_int8_permute(x: torch.Tensor, tables: Tables, out: tuple[torch.Tensor, torch.Tensor] | None = None, stream=None):
+def quant_int8_permute(x: torch.Tensor, tables: Tables, out: tuple[torch.Tensor, torch.Tensor] | None = None,
+                       stream=None):
     """quant_int8 of bf16 rows, each written to every permuted row it is routed to (k3moe_quant_int8_permute):
     (q [cap_rows, cols], scale [cap_rows]); padding rows are not written."""
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _on(stream, x):
             return quant_int8_permute(x, tables, out)
     ldx = _rows(x, "x", _BF16)
     R, cols = x.shape
@@ -587,7 +595,7 @@ def gemm_int8(q: torch.Tensor, sx: torch.Tensor, w: torch.Tensor, sw: torch.Tens
     """out[t, n] = sx[t] sw[n] (q[t] . w[n]) (k3moe_gemm_int8): q int8 [T, C], w int8 [N, C], rows 16-byte aligned as
     quant_int8 gives them; out [T, N] bf16 or f32.  err: the device error words, or None."""
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _on(stream, q):
             return gemm_int8(q, sx, w, sw, dtype, out, err)
     dev, T, C, ldq, ldw = _product_args(q, sx, w, sw, err)
     N = w.shape[0]
@@ -603,7 +611,7 @@ def grouped_gemm_int8(q: torch.Tensor, sx: torch.Tensor, w: torch.Tensor, sw: to
     """The products of routed rows with their experts' weights (k3moe_grouped_gemm_int8): q int8 [cap_rows, C] permuted
     rows, w int8 [n_experts * N, C], out [cap_rows, N]; padding rows of out are not written."""
     if stream is not None:
-        with torch.cuda.stream(stream):
+        with _on(stream, q):
             return grouped_gemm_int8(q, sx, w, sw, tables, n_experts, dtype, out, err)
     dev, cap, C, ldq, ldw = _product_args(q, sx, w, sw, err)
     ctas = tables.max_ctas

@@ -240,20 +240,39 @@ def test_grouped_product_is_exact(dev, R, K, E, first, shared, N, C, dtype):
     assert same_bits(out, want)
 
 
-def test_bad_tiles_are_skipped_and_reported(dev):
+def test_no_row_on_this_rank(dev):
+    """Every pick foreign: no tile, nothing read or written."""
+    idx = torch.full((20, 2), 9, dtype=torch.int32, device=dev)
+    idx[:, 1] = 11
+    t = k3moe.route_tables(idx, 4)
+    x = torch.randn(20, 64, device=dev).to(torch.bfloat16)
+    q = torch.full((t.cap_rows, 64), 99, dtype=torch.int8, device=dev)
+    s = torch.full((t.cap_rows,), -1.0, device=dev)
+    k3moe.quant_int8_permute(x, t, out=(q, s))
+    k3moe.act_quant_int8(torch.zeros((t.cap_rows, 128), dtype=torch.bfloat16, device=dev), tables=t, out=(q, s))
+    out = torch.full((t.cap_rows, 256), 3.0, device=dev)
+    w = torch.zeros((4 * 256, 64), dtype=torch.int8, device=dev)
+    err = torch.zeros(2, dtype=torch.int32, device=dev)
+    k3moe.grouped_gemm_int8(q, s, w, torch.ones(1024, device=dev), t, 4, out=out, err=err)
+    assert int(t.meta[0]) == 0 and err.tolist() == [0, 0]
+    assert bool((q == 99).all()) and bool((s == -1).all()) and bool((out == 3).all())
+
+
+@pytest.mark.parametrize("N", [128, 512])  # a block a tile, a pair of blocks
+def test_bad_tiles_are_skipped_and_reported(dev, N):
     """Tiles whose expert or row limit is out of range: the kernel's own checks record and skip them."""
     g = torch.Generator(device=dev).manual_seed(1)
     idx = torch.arange(4, dtype=torch.int32, device=dev).repeat(100)[:, None].contiguous()
     t = k3moe.route_tables(idx, 4)
-    q, w = rand_codes(g, t.cap_rows, 128, dev), rand_codes(g, 4 * 128, 128, dev)
-    sx, sw = torch.ones(t.cap_rows, device=dev), torch.ones(512, device=dev)
-    good = torch.zeros((t.cap_rows, 128), device=dev)
+    q, w = rand_codes(g, t.cap_rows, 128, dev), rand_codes(g, 4 * N, 128, dev)
+    sx, sw = torch.ones(t.cap_rows, device=dev), torch.ones(4 * N, device=dev)
+    good = torch.zeros((t.cap_rows, N), device=dev)
     k3moe.grouped_gemm_int8(q, sx, w, sw, t, 4, out=good)
     t.cta_batch[1] = 4
     t.cta_batch[2] = -1
     t.cta_limit[3] = 3 * 128 + 129
     err = torch.zeros(2, dtype=torch.int32, device=dev)
-    out = torch.zeros((t.cap_rows, 128), device=dev)
+    out = torch.zeros((t.cap_rows, N), device=dev)
     k3moe.grouped_gemm_int8(q, sx, w, sw, t, 4, out=out, err=err)
     rc, words = k3moe.read_error(err)
     assert rc == -6 and words == (2, 0xD00)

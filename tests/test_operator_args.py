@@ -1,5 +1,7 @@
 """CPU tests of the refusals of the router's training entries and of the 8-bit integer products: the C ABI rejects bad
 arguments before any device work, the Python mirror before the C ABI."""
+import types
+
 import pytest
 import torch
 
@@ -35,11 +37,11 @@ def test_balance_loss_refusals(lib):
 
 def test_balance_scratch_covers_every_block_and_sequence(lib):
     # (blocks + B) partial rows of E f32 and E int32
-    for T, E, B in ((0, 1, 1), (1, 896, 1), (8192, 896, 16), (65536, 1024, 4096), (2 ** 30, 8, 3)):
+    for T, E, B in ((0, 1, 1), (1, 896, 3), (256, 100, 1), (257, 100, 1), (1, 896, 1), (8192, 896, 16), (65536, 1024, 4096), (2 ** 30, 8, 3)):
         nv = -(-E // 128)
         chunk = max(8, -(-T // (148 * (2 if nv <= 2 else 1))))
         blocks = max(1, -(-T // chunk))
-        need = (blocks + B) * E * 8 + (blocks + B) * 4 + 8 * 148 * 4 + 4
+        need = (blocks + B) * E * 8 + (blocks + B) * 4 + 8 * 148 * 8 + 4
         got = lib.k3moe_balance_scratch_bytes(T, E, B)
         assert need <= got <= need + 5 * 256, (T, E, B)
 
@@ -89,7 +91,8 @@ def test_product_refusals(lib):
 
     for kw in (dict(q=None), dict(q=P + 8), dict(ldq=72), dict(ldq=48), dict(sx=None), dict(w=None), dict(w=P + 4),
                dict(ldw=65), dict(sw=None), dict(out=None), dict(out=P + 1), dict(out=P + 2, dtype=1), dict(ldo=7),
-               dict(T=-1), dict(N=0), dict(C=0), dict(C=131072, ldq=131072, ldw=131072), dict(dtype=3)):
+               dict(T=-1), dict(N=0), dict(C=0), dict(C=131072, ldq=131072, ldw=131072), dict(dtype=3),
+               dict(T=2 ** 31 - 255), dict(N=2 ** 31 - 255, ldo=2 ** 31)):
         assert gemm(**kw) == -1, kw
     assert gemm(T=0, q=None, out=None) == 0
 
@@ -148,6 +151,8 @@ def test_the_mirror_refuses_what_the_kernels_do_not_take(dev):
         lambda: k3moe.route_backward(S, idx, dwts=torch.zeros(4, 2, device=dev),
                                      rs=torch.ones(1, dtype=torch.bfloat16, device=dev), dtype=torch.float16),
     ]
+    other = types.SimpleNamespace(device=torch.device("cuda", 7))
+    bad += [lambda: k3moe.quant_int8(S, stream=other), lambda: k3moe.balance_loss(S, idx, 1.0, stream=other)]
     for i, call in enumerate(bad):
         with pytest.raises(k3moe.K3MoeError):
             call()
