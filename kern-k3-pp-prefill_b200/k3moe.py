@@ -10,6 +10,7 @@ exception is raised.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 from dataclasses import dataclass
 
@@ -340,62 +341,23 @@ def read_error(err: torch.Tensor, clear: bool = True, stream=None):
     return rc, (out[0], out[1])
 
 
-# ------------------------------------------------------------------ argument checks of the entries below
-# A decode step calls these entries every few microseconds, so the checks that pass are a few attribute reads; what is
-# wrong with an argument is worked out only when one of them fails.
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise K3MoeError(what)
+# ------------------------------------------------------------------ the entries below
+# Their checks, allocations and C-ABI calls are compiled (csrc/torch_ops.cpp): a call costs the host 4 to 7 us.
+TORCH_OPS_PATH = os.path.join(_HERE, "k3moe_torch.so")
+BF16, F32 = 0, 1  # include/k3moe.h K3MOE_BF16, K3MOE_F32
+
+_ops = None
 
 
-def _rows(t, name: str, dtypes, dev=None, cols: int | None = None, rows: int | None = None) -> int:
-    """Check a matrix argument (dtype, device, shape, rows that are runs of elements, none shared); its row stride."""
-    try:
-        (n, c), (ld, one) = t.shape, t.stride()
-        if (one == 1 and ld >= c and t.dtype in dtypes and t.is_cuda and (dev is None or t.device == dev)
-                and (cols is None or c == cols) and (rows is None or n == rows)):
-            return ld
-    except (AttributeError, TypeError, ValueError):
-        raise K3MoeError(f"{name}: a matrix on a CUDA device is needed") from None
-    _need(t.dtype in dtypes, f"{name}: dtype {t.dtype} (one of {dtypes} is needed)")
-    _need(t.is_cuda, f"{name}: a CUDA tensor is needed")
-    _need(dev is None or t.device == dev, f"{name}: on {t.device}, the other tensors on {dev}")
-    _need(cols in (None, c) and rows in (None, n), f"{name}: shape {(n, c)} ({rows} rows of {cols} are needed)")
-    # one row, or rows of one element, or none: their strides say nothing
-    _need((one == 1 or c <= 1) and (ld >= c or n <= 1), f"{name}: strides {(ld, one)} (contiguous rows are needed)")
-    return max(ld, c) if n > 1 else c
-
-
-def _vec(t, name: str, dtypes, n: int | None, dev) -> None:
-    """Check a contiguous array argument of n elements (None: any number)."""
-    try:
-        if t.dtype in dtypes and t.device == dev and t.is_contiguous() and (n is None or t.numel() == n):
-            return
-    except AttributeError:
-        pass
-    raise K3MoeError(f"{name}: a contiguous tensor of {n} elements of {dtypes} on {dev} is needed")
-
-
-def _int8_rows(t, name: str, dev=None, cols: int | None = None, rows: int | None = None) -> int:
-    """_rows of an int8 operand: 16-byte aligned, row stride a multiple of 16 (of one row: rounded up)."""
-    ld = _rows(t, name, _I8, dev, cols, rows)
-    if ld % 16 and t.shape[0] <= 1:
-        ld = -(-ld // 16) * 16
-    if ld % 16 or t.data_ptr() % 16:
-        raise K3MoeError(f"{name}: 16-byte aligned rows are needed (quant_int8 pads them)")
-    return ld
-
-
-def _launch(fn, what: str, dev, *args) -> None:
-    """Call an entry on `dev`'s current stream, with `dev` the current device."""
-    i = dev.index
-    if i == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
-    if rc:
-        _check(rc, what)
+def _load_ops():
+    global _ops
+    if not os.path.exists(TORCH_OPS_PATH) or not os.path.exists(LIB_PATH):
+        raise K3MoeError(f"{TORCH_OPS_PATH} is missing: build it with `python __graft_entry__.py` (build())")
+    spec = importlib.util.spec_from_file_location("k3moe_torch", TORCH_OPS_PATH)
+    _ops = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(_ops)
+    _ops.set_error(K3MoeError)
+    return _ops
 
 
 def _on(stream, t):
@@ -403,20 +365,6 @@ def _on(stream, t):
     if stream.device != t.device:
         raise K3MoeError(f"stream: on {stream.device}, the tensors on {t.device}")
     return torch.cuda.stream(stream)
-
-
-def _out_dtype(dtype) -> int:
-    if dtype is torch.bfloat16:
-        return BF16
-    if dtype is torch.float32:
-        return F32
-    raise K3MoeError(f"dtype {dtype} (torch.bfloat16 or torch.float32 is needed)")
-
-
-_empty = torch.empty
-_I8, _I32, _F32, _BF16 = (torch.int8,), (torch.int32,), (torch.float32,), (torch.bfloat16,)
-_FLOATS, _FLAGS, _WORDS = (torch.bfloat16, torch.float32), (torch.uint8, torch.bool), (torch.int32, torch.uint32)
-BF16, F32 = 0, 1  # include/k3moe.h K3MOE_BF16, K3MOE_F32
 
 
 # ------------------------------------------------------------------ the router's training side
@@ -428,23 +376,6 @@ class BalanceStats:
     rows: torch.Tensor    # int32 [B]: counted rows
 
 
-def _router_args(S, idx, seq, mask):
-    ld = _rows(S, "S", _F32)
-    dev, (T, E) = S.device, S.shape
-    _vec(idx, "idx", _I32, None, dev)
-    if idx.dim() != 2 or idx.shape[0] != T:
-        raise K3MoeError(f"idx: shape {tuple(idx.shape)} ([{T}, K] is needed)")
-    B = 1
-    if seq is not None:
-        _vec(seq, "seq", _I32, None, dev)
-        B = seq.numel() - 1
-        if B < 1:
-            raise K3MoeError("seq: int32 offsets [B + 1] are needed")
-    if mask is not None:
-        _vec(mask, "mask", _FLAGS, T, dev)
-    return dev, T, E, idx.shape[1], B, ld
-
-
 def balance_loss(S: torch.Tensor, idx: torch.Tensor, alpha: float, seq: torch.Tensor | None = None,
                  mask: torch.Tensor | None = None, stream=None) -> BalanceStats:
     """The router's load-balance loss over the top-k's picks, and its counts (k3moe_balance_loss).
@@ -454,16 +385,7 @@ def balance_loss(S: torch.Tensor, idx: torch.Tensor, alpha: float, seq: torch.Te
     if stream is not None:
         with _on(stream, S):
             return balance_loss(S, idx, alpha, seq, mask)
-    dev, T, E, K, B, ld = _router_args(S, idx, seq, mask)
-    L = lib()
-    scratch = _empty(L.k3moe_balance_scratch_bytes(T, E, B), dtype=torch.uint8, device=dev)
-    prob = _empty(B, E, dtype=torch.float32, device=dev)
-    counts = _empty(B, E, dtype=torch.int32, device=dev)
-    rows = _empty(B, dtype=torch.int32, device=dev)
-    loss = _empty(1, dtype=torch.float32, device=dev)
-    _launch(L.k3moe_balance_loss, "balance_loss", dev, S.data_ptr(), ld, idx.data_ptr(), T, E, K, _p(seq), B, _p(mask),
-            alpha, scratch.data_ptr(), counts.data_ptr(), prob.data_ptr(), rows.data_ptr(), loss.data_ptr())
-    return BalanceStats(loss, counts, prob, rows)
+    return BalanceStats(*(_ops or _load_ops()).balance_loss(S, idx, alpha, seq, mask))
 
 
 def route_backward(S: torch.Tensor, idx: torch.Tensor, alpha: float = 0.0, counts: torch.Tensor | None = None,
@@ -477,53 +399,17 @@ def route_backward(S: torch.Tensor, idx: torch.Tensor, alpha: float = 0.0, count
     if stream is not None:
         with _on(stream, S):
             return route_backward(S, idx, alpha, counts, rows, dloss, dwts, rs, seq, mask, dtype, out)
-    dev, T, E, K, B, ld = _router_args(S, idx, seq, mask)
-    if counts is not None and rows is not None:
-        _vec(counts, "counts", _I32, B * E, dev)
-        _vec(rows, "rows", _I32, B, dev)
-    else:
-        _need(counts is None and rows is None, "counts and rows are given together")
-        _need(dwts is not None, "counts and rows, or dwts and rs, are needed")
-    if dloss is not None:
-        _vec(dloss, "dloss", _F32, 1, dev)
-    if dwts is not None:
-        _vec(dwts, "dwts", _F32, T * K, dev)
-        _vec(rs, "rs", _BF16, 1, dev)
-    if out is None:
-        code, ldd = _out_dtype(dtype), E
-        out = _empty(T, E, dtype=dtype, device=dev)
-    else:
-        code, ldd = _out_dtype(out.dtype), _rows(out, "out", _FLOATS, dev, E, T)
-    _launch(lib().k3moe_route_backward, "route_backward", dev, S.data_ptr(), ld, idx.data_ptr(), T, E, K, _p(seq), B,
-            _p(mask), alpha, _p(counts), _p(rows), _p(dloss), _p(dwts), _p(rs), out.data_ptr(), ldd, code)
-    return out
+    return (_ops or _load_ops()).route_backward(S, idx, alpha, counts, rows, dloss, dwts, rs, seq, mask, dtype, out)
 
 
 # ------------------------------------------------------------------ products in 8-bit integers
-def _int8_out(rows: int, cols: int, dev, out):
-    if out is None:
-        ld = -(-cols // 16) * 16
-        q = torch.empty_strided((rows, cols), (ld, 1), dtype=torch.int8, device=dev)
-        return q, ld, _empty(rows, dtype=torch.float32, device=dev)
-    q, scale = out
-    ld = _int8_rows(q, "out q", dev, cols, rows)
-    _vec(scale, "out scale", _F32, rows, dev)
-    return q, ld, scale
-
-
 def quant_int8(x: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None, stream=None):
     """Rows of x (bf16 or f32 [rows, cols]; tokens, or a weight's channels) to int8 with a scale each
     (k3moe_quant_int8): (q int8 [rows, cols], its rows padded to 16 bytes; scale f32 [rows])."""
     if stream is not None:
         with _on(stream, x):
             return quant_int8(x, out)
-    ldx = _rows(x, "x", _FLOATS)
-    rows, cols = x.shape
-    dev = x.device
-    q, ldq, scale = _int8_out(rows, cols, dev, out)
-    _launch(lib().k3moe_quant_int8, "quant_int8", dev, x.data_ptr(), _out_dtype(x.dtype), ldx, rows, cols, q.data_ptr(),
-            ldq, scale.data_ptr())
-    return q, scale
+    return (_ops or _load_ops()).quant_int8(x, out)
 
 
 def act_quant_int8(gu: torch.Tensor, activation: int = ACT_SWIGLU, tables: Tables | None = None,
@@ -533,22 +419,10 @@ def act_quant_int8(gu: torch.Tensor, activation: int = ACT_SWIGLU, tables: Table
     if stream is not None:
         with _on(stream, gu):
             return act_quant_int8(gu, activation, tables, out)
-    ldg = _rows(gu, "gu", _BF16)
-    rows, cols = gu.shape
-    dev = gu.device
-    if cols % 2:
-        raise K3MoeError(f"gu: {cols} columns (gate and up halves are needed)")
-    limit = meta = None
-    ctas = 0
-    if tables is not None:
-        limit, meta, ctas = tables.cta_limit, tables.meta, tables.max_ctas
-        _need(rows <= ctas * 128, f"gu: {rows} rows, the tables cover {ctas * 128}")
-        _vec(limit, "tables.cta_limit", _I32, ctas, dev)
-        _vec(meta, "tables.meta", _I32, None, dev)
-    q, ldq, scale = _int8_out(rows, cols // 2, dev, out)
-    _launch(lib().k3moe_act_quant_int8, "act_quant_int8", dev, gu.data_ptr(), ldg, rows, cols // 2, activation,
-            _p(limit), _p(meta), ctas, q.data_ptr(), ldq, scale.data_ptr())
-    return q, scale
+    ops = _ops or _load_ops()
+    if tables is None:
+        return ops.act_quant_int8(gu, activation, None, None, 0, out)
+    return ops.act_quant_int8(gu, activation, tables.cta_limit, tables.meta, tables.max_ctas, out)
 
 
 def quant_int8_permute(x: torch.Tensor, tables: Tables, out: tuple[torch.Tensor, torch.Tensor] | None = None,
@@ -558,51 +432,18 @@ def quant_int8_permute(x: torch.Tensor, tables: Tables, out: tuple[torch.Tensor,
     if stream is not None:
         with _on(stream, x):
             return quant_int8_permute(x, tables, out)
-    ldx = _rows(x, "x", _BF16)
-    R, cols = x.shape
-    dev, e2p, cap = x.device, tables.exp2perm, tables.cap_rows
-    K = e2p.shape[1]
-    _vec(e2p, "tables.exp2perm", _I32, R * K, dev)
-    _vec(tables.meta, "tables.meta", _I32, None, dev)
-    q, ldq, scale = _int8_out(cap, cols, dev, out)
-    _launch(lib().k3moe_quant_int8_permute, "quant_int8_permute", dev, x.data_ptr(), ldx, R, cols, K, e2p.data_ptr(),
-            tables.meta.data_ptr(), q.data_ptr(), ldq, scale.data_ptr(), cap)
-    return q, scale
-
-
-def _product_args(q, sx, w, sw, err):
-    ldq = _int8_rows(q, "q")
-    dev, (T, C) = q.device, q.shape
-    ldw = _int8_rows(w, "w", dev, C)
-    _vec(sx, "sx", _F32, T, dev)
-    _vec(sw, "sw", _F32, w.shape[0], dev)
-    if err is not None:
-        _vec(err, "err", _WORDS, None, dev)
-        _need(err.numel() >= 2, "err: two words are needed")
-    return dev, T, C, ldq, ldw
-
-
-def _product_out(T, N, dtype, dev, out):
-    if out is None:
-        code = _out_dtype(dtype)
-        return _empty(T, N, dtype=dtype, device=dev), N, code
-    return out, _rows(out, "out", _FLOATS, dev, N, T), _out_dtype(out.dtype)
+    return (_ops or _load_ops()).quant_int8_permute(x, tables.exp2perm, tables.meta, tables.cap_rows, out)
 
 
 def gemm_int8(q: torch.Tensor, sx: torch.Tensor, w: torch.Tensor, sw: torch.Tensor,
-              dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
-              err: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+              dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None, err: torch.Tensor | None = None,
+              stream=None) -> torch.Tensor:
     """out[t, n] = sx[t] sw[n] (q[t] . w[n]) (k3moe_gemm_int8): q int8 [T, C], w int8 [N, C], rows 16-byte aligned as
     quant_int8 gives them; out [T, N] bf16 or f32.  err: the device error words, or None."""
     if stream is not None:
         with _on(stream, q):
             return gemm_int8(q, sx, w, sw, dtype, out, err)
-    dev, T, C, ldq, ldw = _product_args(q, sx, w, sw, err)
-    N = w.shape[0]
-    out, ldo, code = _product_out(T, N, dtype, dev, out)
-    _launch(lib().k3moe_gemm_int8, "gemm_int8", dev, q.data_ptr(), ldq, sx.data_ptr(), w.data_ptr(), ldw, sw.data_ptr(),
-            T, N, C, out.data_ptr(), ldo, code, _p(err))
-    return out
+    return (_ops or _load_ops()).gemm_int8(q, sx, w, sw, dtype, out, err)
 
 
 def grouped_gemm_int8(q: torch.Tensor, sx: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, tables: Tables,
@@ -613,19 +454,8 @@ def grouped_gemm_int8(q: torch.Tensor, sx: torch.Tensor, w: torch.Tensor, sw: to
     if stream is not None:
         with _on(stream, q):
             return grouped_gemm_int8(q, sx, w, sw, tables, n_experts, dtype, out, err)
-    dev, cap, C, ldq, ldw = _product_args(q, sx, w, sw, err)
-    ctas = tables.max_ctas
-    if n_experts < 1 or w.shape[0] % n_experts or cap != tables.cap_rows:
-        raise K3MoeError(f"q of {cap} rows (capacity {tables.cap_rows}), w of {w.shape[0]} rows for {n_experts} experts")
-    _vec(tables.cta_batch, "tables.cta_batch", _I32, ctas, dev)
-    _vec(tables.cta_limit, "tables.cta_limit", _I32, ctas, dev)
-    _vec(tables.meta, "tables.meta", _I32, None, dev)
-    N = w.shape[0] // n_experts
-    out, ldo, code = _product_out(cap, N, dtype, dev, out)
-    _launch(lib().k3moe_grouped_gemm_int8, "grouped_gemm_int8", dev, q.data_ptr(), ldq, sx.data_ptr(), w.data_ptr(), ldw,
-            sw.data_ptr(), tables.cta_batch.data_ptr(), tables.cta_limit.data_ptr(), tables.meta.data_ptr(), N, C,
-            n_experts, cap, ctas, out.data_ptr(), ldo, code, _p(err))
-    return out
+    return (_ops or _load_ops()).grouped_gemm_int8(q, sx, w, sw, tables.cta_batch, tables.cta_limit, tables.meta,
+                                                   tables.max_ctas, tables.cap_rows, n_experts, dtype, out, err)
 
 
 # ------------------------------------------------------------------ the layer

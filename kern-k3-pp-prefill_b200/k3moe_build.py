@@ -4,17 +4,21 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join(HERE, "csrc", "capi.cu")
 OUT = os.path.join(HERE, "libk3moe.so")
+HEADER = os.path.join(HERE, "..", "include", "k3moe.h")
+TORCH_SRC = os.path.join(HERE, "csrc", "torch_ops.cpp")
+TORCH_OUT = os.path.join(HERE, "k3moe_torch.so")
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17", "-shared",
               "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
 
 
 def sources():
     d = os.path.join(HERE, "csrc")
-    return [os.path.join(d, f) for f in sorted(os.listdir(d))] + [os.path.join(HERE, "..", "include", "k3moe.h")]
+    return [os.path.join(d, f) for f in sorted(os.listdir(d)) if not f.endswith(".cpp")] + [HEADER]
 
 
 def up_to_date() -> bool:
@@ -39,7 +43,36 @@ def build_cubin(nvcc: str) -> str:
     return CUBIN
 
 
+def build_torch(force: bool = False) -> str:
+    """The compiled torch side of the newer entries (csrc/torch_ops.cpp), linked to libk3moe.so beside it."""
+    if not force and os.path.exists(TORCH_OUT) and all(os.path.getmtime(s) <= os.path.getmtime(TORCH_OUT)
+                                                       for s in (TORCH_SRC, HEADER)):
+        return TORCH_OUT
+    import torch
+    from torch.utils import cpp_extension
+
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    inc = [*cpp_extension.include_paths(), os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include"),
+           sysconfig.get_paths()["include"]]
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+           *(f for d in inc for f in ("-isystem", d)), TORCH_SRC, "-o", TORCH_OUT + ".tmp", "-L" + HERE, "-l:libk3moe.so",
+           "-L" + lib, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("g++ failed for k3moe_torch.so")
+    os.replace(TORCH_OUT + ".tmp", TORCH_OUT)
+    return TORCH_OUT
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
+    out = build_library(force, verbose)
+    build_torch(force)
+    return out
+
+
+def build_library(force: bool = False, verbose: bool = False) -> str:
     nvcc = os.environ.get("NVCC", "nvcc")
     if not force and up_to_date():
         if not os.path.exists(CUBIN) or os.path.getmtime(CUBIN) < os.path.getmtime(OUT):
