@@ -504,14 +504,14 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
   if (PAIR) cluster_sync();  // the other block's barriers are there
   tc_fence_after();
   const u32 tmem_base = *tmem_slot;
-  grid_wait_previous();  // the rows (and whatever else an earlier kernel writes) are there from here on
-  const int units = (p.cta_batch ? min(p.meta[0], p.max_ctas) : p.t_tiles) * p.n_tiles;
   // the block's part of K (all of it without a cluster)
   const int rank = PAIR || p.splits > 1 ? (int)cluster_rank() : 0;
   const int k0 = PAIR ? 0 : (int)((long long)rank * p.kstages / p.splits);
   const int k1 = PAIR ? p.kstages : (int)((long long)(rank + 1) * p.kstages / p.splits);
   const int share = PAIR ? 2 : p.splits;  // blocks a unit
   const int first = blockIdx.x / share, stride = gridDim.x / share;
+  grid_wait_previous();  // the rows (and whatever else an earlier kernel writes) are there from here on
+  const int units = (p.cta_batch ? min(p.meta[0], p.max_ctas) : p.t_tiles) * p.n_tiles;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -684,23 +684,30 @@ __global__ void __launch_bounds__(i8::THREADS, 1)
     // one unit a cluster: the parts of K meet
     const Int8Unit w = int8_unit<PAIR>(p, first, rank);
     const u32 red = smem_u32(smem);
+    const int ch = w.ch0 + lane * 4;
+    float sw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sw[i] = ch + i < p.N ? p.sw[ch + i] : 0.f;
     cluster_sync();
     for (int t = warp * p.splits + rank; t < w.n; t += WARPS * p.splits) {
-      int4 a = make_int4(0, 0, 0, 0);
-      for (int r = 0; r < p.splits; ++r) {
-        const int4 b = ld_cluster_v4(red + (u32)(t * BM + lane * 4) * 4, (u32)r);
-        a.x += b.x;
-        a.y += b.y;
-        a.z += b.z;
-        a.w += b.w;
-      }
-      const int ch = w.ch0 + lane * 4;
       const float s = p.sx[w.row0 + t];
-      const int q[4] = {a.x, a.y, a.z, a.w};
+      int4 b[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < p.splits) b[r] = ld_cluster_v4(red + (u32)(t * BM + lane * 4) * 4, (u32)r);
+      int q[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < p.splits) {
+          q[0] += b[r].x;
+          q[1] += b[r].y;
+          q[2] += b[r].z;
+          q[3] += b[r].w;
+        }
       OUT* dst = reinterpret_cast<OUT*>(p.out) + ((long long)w.row0 + t) * p.ldo + ch;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (ch + i < p.N) int8_put(dst + i, (u32)q[i], s, p.sw[ch + i]);
+        if (ch + i < p.N) int8_put(dst + i, (u32)q[i], s, sw[i]);
     }
     cluster_sync();  // no block leaves while another reads its part
   }
