@@ -8,10 +8,10 @@
 #include <ATen/ops/empty_strided.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <climits>
-#include <exception>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -27,12 +27,10 @@ using Quantised = std::optional<std::tuple<Tensor, Tensor>>;
 
 PyObject* g_error = nullptr;  // k3moe.K3MoeError
 
-struct Refused : std::exception {
-  std::string text;
-  explicit Refused(std::string t) : text(std::move(t)) {}
-  const char* what() const noexcept override { return text.c_str(); }
-};
-[[noreturn]] void refuse(std::string text) { throw Refused(std::move(text)); }
+[[noreturn]] void refuse(const std::string& text) {
+  PyErr_SetString(g_error ? g_error : PyExc_RuntimeError, text.c_str());
+  throw py::error_already_set();
+}
 
 int as_int(int64_t v, const char* name) {
   if (v < 0 || v > INT_MAX) refuse(std::string(name) + ": " + std::to_string(v) + " is out of range");
@@ -306,20 +304,14 @@ Tensor grouped_gemm_int8(const Tensor& q, const Tensor& sx, const Tensor& w, con
 
 }  // namespace
 
+// torch's own errors (out of memory among them) reach Python as its types
 PYBIND11_MODULE(k3moe_torch, m) {
   m.def("set_error", [](py::object cls) { g_error = cls.release().ptr(); });
-  py::register_exception_translator([](std::exception_ptr p) {
-    try {
-      if (p) std::rethrow_exception(p);
-    } catch (const Refused& e) {
-      PyErr_SetString(g_error ? g_error : PyExc_RuntimeError, e.what());
-    }
-  });
-  m.def("balance_loss", &balance_loss);
-  m.def("route_backward", &route_backward);
-  m.def("quant_int8", &quant_int8);
-  m.def("act_quant_int8", &act_quant_int8);
-  m.def("quant_int8_permute", &quant_int8_permute);
-  m.def("gemm_int8", &gemm_int8);
-  m.def("grouped_gemm_int8", &grouped_gemm_int8);
+  m.def("balance_loss", torch::wrap_pybind_function(balance_loss));
+  m.def("route_backward", torch::wrap_pybind_function(route_backward));
+  m.def("quant_int8", torch::wrap_pybind_function(quant_int8));
+  m.def("act_quant_int8", torch::wrap_pybind_function(act_quant_int8));
+  m.def("quant_int8_permute", torch::wrap_pybind_function(quant_int8_permute));
+  m.def("gemm_int8", torch::wrap_pybind_function(gemm_int8));
+  m.def("grouped_gemm_int8", torch::wrap_pybind_function(grouped_gemm_int8));
 }

@@ -215,7 +215,8 @@ def test_operands_with_row_strides(dev):
 
 @pytest.mark.parametrize("R,K,E,first,shared,N,C", [
     (1, 1, 1, 0, 0, 128, 128), (5, 2, 16, 0, 0, 200, 256), (300, 4, 16, 0, 1, 256, 300), (128, 1, 1, 0, 0, 130, 144),
-    (500, 2, 3, 0, 0, 384, 512), (64, 8, 112, 224, 0, 512, 1024), (1024, 8, 32, 0, 0, 300, 700), (40, 4, 8, 50, 0, 64, 64)])
+    (500, 2, 3, 0, 0, 384, 512), (64, 8, 112, 224, 0, 512, 1024), (1024, 8, 32, 0, 0, 300, 700),
+    (40, 4, 8, 50, 0, 64, 64)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_grouped_product_is_exact(dev, R, K, E, first, shared, N, C, dtype):
     g = torch.Generator().manual_seed(R + E)

@@ -28,8 +28,8 @@ def balance(lib, **kw):
 
 def test_balance_loss_refusals(lib):
     for kw in (dict(S=None), dict(idx=None), dict(scratch=None), dict(scratch=8), dict(counts=None), dict(prob=None),
-               dict(rows=None), dict(loss=None), dict(T=-1), dict(E=0), dict(E=1025, lds=2000), dict(K=0), dict(K=17), dict(T=2 ** 30 + 1),
-               dict(lds=63), dict(B=0), dict(seq=None, B=2), dict(B=2 ** 31 - 1)):
+               dict(rows=None), dict(loss=None), dict(T=-1), dict(E=0), dict(E=1025, lds=2000), dict(K=0), dict(K=17),
+               dict(T=2 ** 30 + 1), dict(lds=63), dict(B=0), dict(seq=None, B=2), dict(B=2 ** 31 - 1)):
         assert balance(lib, **kw) == -1, kw
     assert lib.k3moe_balance_scratch_bytes(-1, 8, 1) == 0 and lib.k3moe_balance_scratch_bytes(8, 1025, 1) == 0
     assert lib.k3moe_balance_scratch_bytes(8, 8, 0) == 0
@@ -37,7 +37,8 @@ def test_balance_loss_refusals(lib):
 
 def test_balance_scratch_covers_every_block_and_sequence(lib):
     # (blocks + B) partial rows of E f32 and E int32
-    for T, E, B in ((0, 1, 1), (1, 896, 3), (256, 100, 1), (257, 100, 1), (1, 896, 1), (8192, 896, 16), (65536, 1024, 4096), (2 ** 30, 8, 3)):
+    for T, E, B in ((0, 1, 1), (1, 896, 3), (256, 100, 1), (257, 100, 1), (1, 896, 1), (8192, 896, 16),
+                    (65536, 1024, 4096), (2 ** 30, 8, 3)):
         nv = -(-E // 128)
         chunk = max(8, -(-T // (148 * (2 if nv <= 2 else 1))))
         blocks = max(1, -(-T // chunk))
