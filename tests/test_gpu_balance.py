@@ -228,6 +228,25 @@ def test_offsets_that_go_down_stay_in_bounds(dev):
     torch.cuda.synchronize()
 
 
+def test_offsets_past_32_bits(dev):
+    """2.5e9 logits (20 GB with their gradient): a last sequence behind 2^31 elements as by itself."""
+    T, E, n = 2_500_000, 1000, 300
+    S = torch.zeros((T, E), device=dev)
+    g = torch.Generator(device=dev).manual_seed(4)
+    S[-n:] = torch.randn(n, E, generator=g, device=dev)
+    idx = torch.randint(0, E, (T, 2), generator=g, device=dev, dtype=torch.int32)
+    seq = torch.tensor([0, T - n, T], dtype=torch.int32, device=dev)
+    st = k3moe.balance_loss(S, idx, 1.0, seq)
+    tail, tail_idx = S[-n:].contiguous(), idx[-n:].contiguous()
+    one = k3moe.balance_loss(tail, tail_idx, 1.0)
+    assert torch.equal(st.counts[1:], one.counts) and st.rows.tolist() == [T - n, n]
+    np.testing.assert_allclose(st.prob[1].cpu().numpy(), one.prob[0].cpu().numpy(), rtol=RTOL)
+    np.testing.assert_allclose(st.prob[0].cpu().numpy(), (T - n) / E, rtol=RTOL)
+    dS = k3moe.route_backward(S, idx, 1.0, st.counts, st.rows, seq=seq)
+    half = k3moe.route_backward(tail, tail_idx, 0.5, one.counts, one.rows)  # the loss is a mean over two sequences
+    assert torch.equal(dS[-n:], half)
+
+
 def test_captured_and_on_another_stream(dev):
     S, idx, seq, mask = make(dev, 400, 96, 4, 6, True, 21)
     st = k3moe.balance_loss(S, idx, 1.0, seq, mask)

@@ -280,6 +280,20 @@ def test_bad_tiles_are_skipped_and_reported(dev, N):
     assert same_bits(out[:100], good[:100]) and bool((out[128:] == 0).all())
 
 
+def test_offsets_past_32_bits(dev):
+    """2.4e9 elements in, as codes and out (about 17 GB): the last rows as the same rows by themselves."""
+    rows, cols = 36000, 65536
+    x = torch.zeros((rows, cols), dtype=torch.bfloat16, device=dev)
+    g = torch.Generator(device=dev).manual_seed(2)
+    x[-3:] = torch.randn(3, cols, generator=g, device=dev).to(torch.bfloat16)
+    q, s = k3moe.quant_int8(x)
+    rq, rs = k3moe.quant_int8(x[-3:].contiguous())
+    assert torch.equal(q[-3:], rq) and torch.equal(s[-3:], rs) and float(s[:-3].abs().max()) == 0
+    w, sw = rand_codes(g, cols, 16, dev), torch.rand(cols, generator=g, device=dev)
+    y = k3moe.gemm_int8(q[:, :16], s, w, sw)
+    assert same_bits(y[-3:], product(rq[:, :16], rs, w, sw, torch.bfloat16)) and bool((y[:-3] == 0).all())
+
+
 def test_captured_and_on_another_stream(dev):
     g = torch.Generator(device=dev).manual_seed(8)
     x = torch.randn(70, 1500, generator=g, device=dev).to(torch.bfloat16)
