@@ -273,12 +273,13 @@ __global__ void __launch_bounds__(32 * bal::JOIN_WARPS)
       full += s_c[k][0];
     }
     w.term[blockIdx.x] = make_float2(terms, __int_as_float(full));
-    __threadfence();
-    s_last = atomicAdd(w.done, 1u) == gridDim.x - 1;
+    // releases this thread's store above and acquires those of the blocks that counted before
+    u32 before;
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(w.done) : "memory");
+    s_last = before == gridDim.x - 1;
   }
   __syncthreads();
   if (!s_last) return;
-  __threadfence();
   terms = 0.f;
   full = 0;
   for (int i = threadIdx.x; i < gridDim.x; i += blockDim.x) {
