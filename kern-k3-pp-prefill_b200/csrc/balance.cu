@@ -10,9 +10,9 @@
 //   dS_{t, idx_k} += rs / den (g_k - sum_j g_j s_j / den) s_k (1 - s_k),    g = dloss/dw.
 // No counterpart in the reference: it serves only.
 //
-// Measured on a B200, 8192 x 896 logits, top-8, 16 sequences: loss and counts 18.5 us (fixed part about 10, then 29 MB in
-// 5 us; read alone 4.5 us), gradient of both terms 20 us (59 MB, of which the 29 written take 8.7 us at the 3.4 TB/s that
-// pure writes reach; a copy of the same bytes 10.3 us).
+// Measured on a B200, 8192 x 896 logits, top-8, 16 sequences: loss and counts 17.9 us (11 us at 2048 rows, 5 of them the
+// join; 29 MB more cost 5 us; reading them takes 4.5), gradient of both terms 18-20 us (4 us a round of 16 rows an SM behind
+// 6 us of prologue and first rows; a copy of the same 59 MB takes 10.3 us).
 // Both passes read S once.  Sums run in f32 in a fixed order (no floating-point atomics), so equal inputs give equal
 // bytes.  A score is 1 / (1 + 2^(-S log2 e)) by the approximate exponential and reciprocal: its relative error grows
 // with |S|, to 1.5e-6 at S = -10, where the score itself is below 5e-5.
