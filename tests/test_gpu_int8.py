@@ -317,6 +317,62 @@ def test_captured_and_on_another_stream(dev):
     assert same_bits(y, y3)
 
 
+def test_captured_behind_a_join(dev):
+    """A captured call that follows work on two streams: rows from one, weights from the other."""
+    g = torch.Generator(device=dev).manual_seed(18)
+    xf = torch.randn(40, 512, generator=g, device=dev)
+    wf = torch.randn(300, 512, generator=g, device=dev)
+    idx = torch.randint(0, 64, (40, 2), generator=g, device=dev, dtype=torch.int32)
+    q, sx = k3moe.quant_int8(xf * 2)
+    w, sw = k3moe.quant_int8(wf * 3)
+    want = k3moe.gemm_int8(q, sx, w, sw)
+    loss = k3moe.balance_loss(xf[:, :64], idx, 1.0).loss
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            w2, sw2 = k3moe.quant_int8(wf * 3)
+        q2, sx2 = k3moe.quant_int8(xf * 2)
+        main.wait_stream(side)
+        y = k3moe.gemm_int8(q2, sx2, w2, sw2)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            b = k3moe.balance_loss(xf[:, :64], idx, 1.0)
+        z = y * 2
+        main.wait_stream(side)
+        dS = k3moe.route_backward(xf[:, :64], idx, 1.0, b.counts, b.rows)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert same_bits(y, want) and torch.equal(b.loss, loss) and same_bits(z, want * 2)
+    assert same_bits(dS, k3moe.route_backward(xf[:, :64], idx, 1.0, b.counts, b.rows))
+
+
+def test_weights_from_a_late_stream(dev):
+    """An overlapped launch still waits for an event that stands between it and the kernel before it: weights written
+    late on another stream, rows written right before on this one."""
+    g = torch.Generator(device=dev).manual_seed(19)
+    x = torch.randn(40, 512, generator=g, device=dev)
+    wf = torch.randn(300, 512, generator=g, device=dev)
+    q, sx = k3moe.quant_int8(x)
+    w, sw = k3moe.quant_int8(wf)
+    want = k3moe.gemm_int8(q, sx, w, sw)
+    w2, sw2 = torch.zeros_like(w), torch.zeros_like(sw)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        w2.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(5_000_000)  # a few milliseconds
+            k3moe.quant_int8(wf, out=(w2, sw2))
+        q2, sx2 = k3moe.quant_int8(x)
+        torch.cuda.current_stream().wait_stream(side)
+        assert same_bits(k3moe.gemm_int8(q2, sx2, w2, sw2), want)
+
+
 def test_two_products_at_once(dev):
     """Calls share no state: split reductions on two streams at the same time."""
     g = torch.Generator(device=dev).manual_seed(5)
