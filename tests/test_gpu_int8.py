@@ -82,6 +82,26 @@ def test_every_bf16_quotient_of_some_maxima(dev):
     assert np.array_equal(s.cpu().numpy(), rs)
 
 
+def test_rows_at_the_ends_of_the_range(dev):
+    """f32 rows from subnormal to the largest magnitudes, in registers and read twice, and gated rows far from 1."""
+    g = torch.Generator().manual_seed(6)
+    top = torch.tensor([1e-44, 1e-42, 1e-38, 3e-30, 2.0 ** -60, 2.0 ** -61, 2.0 ** 60, 2.0 ** 61, 1e30, 3.4e38])
+    for cols in (96, 20001):
+        x = (torch.rand(10, cols, generator=g, dtype=torch.float64) * 2 - 1)
+        x[:, 5] = 1
+        x = (x * top[:, None].double()).float()
+        q, s = k3moe.quant_int8(x.to(dev))
+        rq, rs = codes(x.numpy())
+        assert np.array_equal(q.cpu().numpy(), rq) and np.array_equal(s.cpu().numpy(), rs)
+    scale = torch.tensor([1e-15, 1e-10, 1e10, 1e17])[:, None]
+    gu = torch.cat([torch.rand(4, 64, generator=g) * scale, torch.randn(4, 64, generator=g) * scale], 1).to(torch.bfloat16)
+    q, s = k3moe.act_quant_int8(gu.to(dev))
+    h = gate64(gu, k3moe.ACT_SWIGLU)
+    amax = h.abs().amax(1, keepdim=True)
+    np.testing.assert_allclose(s.double().cpu().numpy(), (amax[:, 0] / 127).numpy(), rtol=2 ** -18)
+    assert bool(((q.cpu().double() - 127 * h / amax).abs() <= 0.5 + 127 * 2 ** -17).all())
+
+
 def test_zero_and_non_finite_rows(dev):
     x = torch.randn(6, 100, generator=torch.Generator().manual_seed(0))
     x[1] = 0
