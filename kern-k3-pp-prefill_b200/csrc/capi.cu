@@ -634,7 +634,9 @@ int k3moe_balance_loss(const float* S, int lds, const int32_t* idx, int T, int E
       rc = launch_overlapped(balance_rows_kernel<NV>, L.blocks, 32 * bal::ROW_WARPS, bytes, s, 1, in, w, L.chunk);
   });
   if (rc) return rc;
-  // the average sequence's partial rows: up to four, a warp adds them up by itself; else a warp a row
+  // The average sequence's partial rows: up to four, a warp adds them up by itself; else a block's warps share them.
+  // Both calls' time, block against warp, at 8192 x 896: 17.5 against 50.5 us for one sequence, 16.9 against 18.5 for 16,
+  // equal within 0.3 us about 37 (the limit), 20.4 against 17.7 for 74, 130 against 57 for 2048.
   const long long units = (long long)B * cdiv(E, bal::COLS);
   const int partial = (int)cdiv(L.blocks, B) + 1;
   if (partial <= 4)
