@@ -15,14 +15,14 @@ namespace k3 {
 // bf16: with 127 / amax bracketed, 2^-21 of it above and below, one FMA each (1.5 * 2^23 + x inv) rounds the quotient seen
 // from either side.  The quotient of two 8-bit mantissas is a half exactly or at least 2^-17 of itself from one, so the two
 // integers are equal, or the neighbours of an exact half: then the even one is it, bit arithmetic on pairs, no branch (ties
-// are common: rows whose maximum has few mantissa bits have them by the hundred).  The gate's values are rounded
-// themselves, so the same rule serves there, a quotient within 2^-13 of a half taken as one.
-// f32: one FMA, and the elements whose x inv is within 1e-5 of a half (inv moves the quotient by 7.6e-6 at most) compare
-// 254 |x| with (2k + 1) amax, both exact in double.
+// are common: rows whose maximum has few mantissa bits have them by the hundred).
+// f32, and the gate's values (f32 too: their quotients come as near to a half as 2^-24): one FMA, and the elements whose
+// x inv is within 1e-5 of a half (inv moves the quotient by 7.6e-6 at most) compare 254 |x| with (2k + 1) amax, both exact
+// in double.
 // A row with an infinity or a NaN has scale NaN and q = 0, so every result it enters is NaN; a zero row scale 0, q = 0.
 // HBM-bound: a row is read once and kept in registers (bf16 as it came) between the maximum and the codes; what counts
 // beside the bytes is the instructions an element, about 7, and blocks enough an SM.  Measured: 8192 x 7168 bf16 29.0 us
-// (6.1 TB/s), gated 8192 x 2 x 2048 18.3 us (4.6 TB/s, its exponential and reciprocal an element beside the bytes).
+// (6.1 TB/s), gated 8192 x 2 x 2048 18.7 us (4.5 TB/s, its exponential and reciprocal an element beside the bytes).
 enum { I8_BF16 = 0, I8_F32 = 1, I8_GATED = 2 };
 
 struct QuantRows {
@@ -138,7 +138,7 @@ __device__ __forceinline__ RowScale row_scale(u32 amax_bits) {
   s.pre = s.inv = 0.f;
   if (amax_bits < 0x7f800000u && amax_bits != 0u) {
     s.pre = s.amax < 0x1p-60f ? 0x1p64f : s.amax > 0x1p60f ? 0x1p-64f : 1.f;
-    s.inv = SRC == I8_F32 ? __fdiv_rn(127.f, s.amax * s.pre) : 127.f * rcp_ftz(s.amax * s.pre);
+    s.inv = SRC == I8_BF16 ? 127.f * rcp_ftz(s.amax * s.pre) : __fdiv_rn(127.f, s.amax * s.pre);
   }
   return s;
 }
@@ -168,7 +168,7 @@ __device__ __forceinline__ int code_near_half(float x, int k, float amax) {
 
 template <int SRC>
 __device__ __forceinline__ uint2 encode8(const RowScale& s, const Kept<SRC>& v) {
-  if (SRC != I8_F32) {
+  if (SRC == I8_BF16) {
     constexpr float ROUND = 12582912.f + 256.f;  // the integer, plus 256, in the low 16 bits
     const float above = s.inv * (1.f + 0x1p-21f), below = s.inv * (1.f - 0x1p-21f);
     const u64 up = f32x2(above, above), down = f32x2(below, below), round = f32x2(ROUND, ROUND);
@@ -188,13 +188,16 @@ __device__ __forceinline__ uint2 encode8(const RowScale& s, const Kept<SRC>& v) 
   }
   constexpr float ROUND = 12582912.f;  // 1.5 * 2^23: the integer sits in the low bits
   constexpr float NEAR = 0.5f - 1e-5f;
+  const u64 inv = f32x2(s.inv, s.inv), round = f32x2(ROUND, ROUND), minus = f32x2(-1.f, -1.f);
   u32 k[8];
   float far = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float t = __fmaf_rn(v[i], s.inv, ROUND);
-    far = fmaxf(far, fabsf(__fmaf_rn(v[i], s.inv, ROUND - t)));  // x inv - its integer
-    k[i] = __float_as_uint(t);
+  for (int i = 0; i < 4; ++i) {
+    const u64 x = f32x2(v[2 * i], v[2 * i + 1]), t = fma_f32x2(x, inv, round);
+    const float2 n = f32x2_get(t), d = f32x2_get(fma_f32x2(x, inv, fma_f32x2(t, minus, round)));  // d: x inv - its integer
+    far = fmaxf(far, fmaxf(fabsf(d.x), fabsf(d.y)));
+    k[2 * i] = __float_as_uint(n.x);
+    k[2 * i + 1] = __float_as_uint(n.y);
   }
   if (far > NEAR) {  // one group in some thousands
 #pragma unroll
