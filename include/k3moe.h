@@ -347,8 +347,8 @@ int k3moe_route_backward(const float* S, int lds, const int32_t* idx, int T, int
  * cols >= 1. */
 int k3moe_quant_int8(const void* x, int dtype, long long ldx, long long rows, int cols, int8_t* q, long long ldq,
                      float* scale, k3moe_stream_t stream);
-/* The same of act(gate) * up (K3MOE_ACT_SWIGLU or K3MOE_ACT_SITU; in f32, whose values are rounded to codes as f32 rows
- * are): gu bf16 [rows, ldg] holds a row's I gate and
+/* The same of act(gate) * up (K3MOE_ACT_SWIGLU or K3MOE_ACT_SITU; in f32, within 2^-21 of the value for SwiGLU and 2^-19 for
+ * SiTU at gates from -87 on, 0 further down; those f32 values are rounded to codes as f32 rows are): gu bf16 [rows, ldg] holds a row's I gate and
  * then its I up values.  With cta_limit and meta (k3moe_route_tables, tile 128; at most max_ctas tiles) only the
  * tables' real rows are read and written; with both null, all. */
 int k3moe_act_quant_int8(const void* gu_bf16, long long ldg, long long rows, int I, int activation,

@@ -22,7 +22,8 @@ namespace k3 {
 // A row with an infinity or a NaN has scale NaN and q = 0, so every result it enters is NaN; a zero row scale 0, q = 0.
 // HBM-bound: a row is read once and kept in registers (bf16 as it came) between the maximum and the codes; what counts
 // beside the bytes is the instructions an element, about 7, and blocks enough an SM.  Measured: 8192 x 7168 bf16 29.0 us
-// (6.1 TB/s), gated 8192 x 2 x 2048 18.7 us (4.5 TB/s, its exponential and reciprocal an element beside the bytes).
+// (6.1 TB/s), f32 47.6 us (6.2 TB/s), gated 8192 x 2 x 2048 SwiGLU 19.5 us (4.3 TB/s: instructions, about 2 an element more
+// than its exponential without the correction, 18.7 us), SiTU 38.6 us (two tanhf an element).
 enum { I8_BF16 = 0, I8_F32 = 1, I8_GATED = 2 };
 
 struct QuantRows {
@@ -45,14 +46,19 @@ struct QuantRows {
   long long cap_rows;  // output rows
 };
 
-// act(g) * u of two elements; SwiGLU's sigmoid by one exponential and one reciprocal instruction (g = -inf: 0 * -inf, a
-// NaN, as for any row that holds an infinity)
-__device__ __forceinline__ float2 gate_of(float2 g, float2 u, int act) {
-  if (act != 0) return make_float2(gated_act(g.x, u.x, act), gated_act(g.y, u.y, act));
-  const u64 x = f32x2(g.x, g.y);
-  const float2 t = f32x2_get(mul_f32x2(x, f32x2(-LOG2E, -LOG2E)));
-  const float2 d = f32x2_get(add_f32x2(f32x2(ex2_ftz(t.x), ex2_ftz(t.y)), f32x2(1.f, 1.f)));
-  return f32x2_get(mul_f32x2(mul_f32x2(x, f32x2(rcp_ftz(d.x), rcp_ftz(d.y))), f32x2(u.x, u.y)));
+// act(g) * u of two elements, bf16 pairs; the sigmoid by one exponential and one reciprocal instruction, within 2^-21 of
+// its value.  Gates are clamped to +-88 for it: below, the sigmoid is under the smallest normal f32 and 0 here (g = -inf:
+// 0 * -inf, a NaN, as for any row that holds an infinity).
+__device__ __forceinline__ float2 gate_of(u32 gate, u32 up, int act) {
+  u32 y = gate ^ 0x80008000u;  // -g
+  asm("min.bf16x2 %0, %0, %1;" : "+r"(y) : "r"(0x42b042b0u));
+  asm("max.bf16x2 %0, %0, %1;" : "+r"(y) : "r"(0xc2b0c2b0u));
+  const float2 ny = bf16x2_to_f2(y), g = bf16x2_to_f2(gate), u = bf16x2_to_f2(up);
+  const float2 d = f32x2_get(add_f32x2(exp_f32x2(f32x2(ny.x, ny.y)), f32x2(1.f, 1.f)));
+  const u64 sg = f32x2(rcp_ftz(d.x), rcp_ftz(d.y));
+  if (act == 0) return f32x2_get(mul_f32x2(mul_f32x2(f32x2(g.x, g.y), sg), f32x2(u.x, u.y)));
+  const u64 a = f32x2(4.f * tanhf(0.25f * g.x), 4.f * tanhf(0.25f * g.y));
+  return f32x2_get(mul_f32x2(mul_f32x2(a, sg), f32x2(25.f * tanhf(0.04f * u.x), 25.f * tanhf(0.04f * u.y))));
 }
 
 // 8 consecutive elements of a row as they are kept: bf16 pairs, or f32
@@ -105,7 +111,7 @@ __device__ __forceinline__ void load8(const QuantRows& p, const void* x, int c, 
   const u32 u[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 h = gate_of(bf16x2_to_f2(g[i]), bf16x2_to_f2(u[i]), p.act);
+    const float2 h = gate_of(g[i], u[i], p.act);
     v.w[(2 * i) % M] = __float_as_uint(h.x);
     v.w[(2 * i + 1) % M] = __float_as_uint(h.y);
   }
