@@ -71,6 +71,12 @@ void array(const Tensor& t, const char* name, Types types, int64_t n, const c10:
          types.text() + " on " + dev.str() + " is needed");
 }
 
+// the tables' four words, which the kernels read by index
+void meta_words(const Tensor& t, const c10::Device& dev) {
+  array(t, "tables.meta", kI32, -1, dev);
+  if (t.numel() < 4) refuse("tables.meta: " + std::to_string(t.numel()) + " elements, four are needed");
+}
+
 // rows_of an int8 operand: 16-byte aligned, its row stride a multiple of 16 (of a single row: rounded up)
 int64_t int8_rows(const Tensor& t, const char* name, const c10::Device* dev, int64_t cols = -1, int64_t n = -1) {
   int64_t ld = rows_of(t, name, kI8, dev, cols, n);
@@ -214,7 +220,7 @@ std::tuple<Tensor, Tensor> act_quant_int8(const Tensor& gu, int activation, cons
   if (limit) {
     if (gu.size(0) > max_ctas * 128) refuse("gu: " + std::to_string(gu.size(0)) + " rows, more than the tables' tiles hold");
     array(*limit, "tables.cta_limit", kI32, max_ctas, dev);
-    array(meta.value(), "tables.meta", kI32, -1, dev);
+    meta_words(meta.value(), dev);
   }
   const c10::cuda::CUDAGuard guard(dev);
   const Int8Out o = int8_out(out, gu.size(0), gu.size(1) / 2, dev);
@@ -231,7 +237,7 @@ std::tuple<Tensor, Tensor> quant_int8_permute(const Tensor& x, const Tensor& exp
   const c10::Device dev = x.device();
   array(exp2perm, "tables.exp2perm", kI32, -1, dev);
   if (exp2perm.dim() != 2 || exp2perm.size(0) != x.size(0)) refuse("tables.exp2perm: a row for each of x is needed");
-  array(meta, "tables.meta", kI32, -1, dev);
+  meta_words(meta, dev);
   const c10::cuda::CUDAGuard guard(dev);
   const Int8Out o = int8_out(out, cap, x.size(1), dev);
   check(k3moe_quant_int8_permute(ptr(x), ldx, as_int(x.size(0), "x"), as_int(x.size(1), "x"), as_int(exp2perm.size(1), "K"),
@@ -289,7 +295,7 @@ Tensor grouped_gemm_int8(const Tensor& q, const Tensor& sx, const Tensor& w, con
            std::to_string(w.size(0)) + " rows for " + std::to_string(n_experts) + " experts");
   array(cta_batch, "tables.cta_batch", kI32, max_ctas, p.dev);
   array(cta_limit, "tables.cta_limit", kI32, max_ctas, p.dev);
-  array(meta, "tables.meta", kI32, -1, p.dev);
+  meta_words(meta, p.dev);
   const int64_t N = w.size(0) / n_experts;
   const c10::cuda::CUDAGuard guard(p.dev);
   const ProductOut o = product_out(p, N, dtype, out);

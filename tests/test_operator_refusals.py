@@ -1,0 +1,29 @@
+"""Refusals of the router's training entries and of the 8-bit integer products that need more than one argument's own
+check: each is raised before any device work."""
+import dataclasses
+
+import pytest
+import torch
+
+import k3moe
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("words", [0, 1, 3])
+def test_tables_with_a_short_meta(dev, words):
+    """The kernels read meta[0] and meta[2]: a shorter array is refused, as every other table of a wrong length is."""
+    idx = torch.randint(0, 4, (30, 2), generator=torch.Generator().manual_seed(0)).to(torch.int32).to(dev)
+    good = k3moe.route_tables(idx, 4)
+    t = dataclasses.replace(good, meta=good.meta[:words].contiguous())
+    x = torch.zeros((30, 64), dtype=torch.bfloat16, device=dev)
+    gu = torch.zeros((t.cap_rows, 128), dtype=torch.bfloat16, device=dev)
+    q = torch.zeros((t.cap_rows, 64), dtype=torch.int8, device=dev)
+    s, w, sw = torch.zeros(t.cap_rows, device=dev), torch.zeros((4 * 8, 64), dtype=torch.int8, device=dev), torch.zeros(32, device=dev)
+    for call in (lambda: k3moe.quant_int8_permute(x, t), lambda: k3moe.act_quant_int8(gu, tables=t),
+                 lambda: k3moe.grouped_gemm_int8(q, s, w, sw, t, 4)):
+        with pytest.raises(k3moe.K3MoeError, match="meta"):
+            call()
+    k3moe.quant_int8_permute(x, good)
+    k3moe.act_quant_int8(gu, tables=good)
+    k3moe.grouped_gemm_int8(q, s, w, sw, good, 4)
+    torch.cuda.synchronize()
