@@ -415,13 +415,15 @@ def quant_int8(x: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = 
 def act_quant_int8(gu: torch.Tensor, activation: int = ACT_SWIGLU, tables: Tables | None = None,
                    out: tuple[torch.Tensor, torch.Tensor] | None = None, stream=None):
     """act(gate) * up of bf16 rows [gate | up] to int8 (k3moe_act_quant_int8): (q [rows, cols / 2], scale).  With
-    tables, gu is [cap_rows, 2I] and only the tables' real rows are read and written."""
+    tables (tile 128), gu is [cap_rows, 2I] and only the tables' real rows are read and written."""
     if stream is not None:
         with _on(stream, gu):
             return act_quant_int8(gu, activation, tables, out)
     ops = _ops or _load_ops()
     if tables is None:
         return ops.act_quant_int8(gu, activation, None, None, 0, out)
+    if tables.cap_rows < 128 * tables.max_ctas:
+        raise K3MoeError(f"tables: {tables.cap_rows} rows for {tables.max_ctas} tiles, tables of 128-row tiles are needed")
     return ops.act_quant_int8(gu, activation, tables.cta_limit, tables.meta, tables.max_ctas, out)
 
 

@@ -8,6 +8,17 @@ import torch
 import k3moe
 
 
+def test_tables_of_other_tiles():
+    """Tables of 64-row tiles (route_tables takes any) would leave most real rows without codes: refused."""
+    n = 3
+    words = [torch.zeros(n, dtype=torch.int32) for _ in range(3)]
+    t = k3moe.Tables(counts=words[0], cta_batch=words[1], cta_limit=words[2], meta=torch.zeros(4, dtype=torch.int32),
+                     route_map=torch.zeros(64 * n, dtype=torch.int32), exp2perm=torch.zeros((5, 1), dtype=torch.int32),
+                     max_ctas=n, cap_rows=64 * n)
+    with pytest.raises(k3moe.K3MoeError, match="128-row tiles"):
+        k3moe.act_quant_int8(torch.zeros((64 * n, 32), dtype=torch.bfloat16), tables=t)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("words", [0, 1, 3])
 def test_tables_with_a_short_meta(dev, words):
