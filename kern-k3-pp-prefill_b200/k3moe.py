@@ -388,17 +388,21 @@ def balance_loss(S: torch.Tensor, idx: torch.Tensor, alpha: float, seq: torch.Te
     return BalanceStats(*(_ops or _load_ops()).balance_loss(S, idx, alpha, seq, mask))
 
 
-def route_backward(S: torch.Tensor, idx: torch.Tensor, alpha: float = 0.0, counts: torch.Tensor | None = None,
+def route_backward(S: torch.Tensor, idx: torch.Tensor, alpha: float | None = None, counts: torch.Tensor | None = None,
                    rows: torch.Tensor | None = None, dloss: torch.Tensor | None = None,
                    dwts: torch.Tensor | None = None, rs: torch.Tensor | None = None, seq: torch.Tensor | None = None,
                    mask: torch.Tensor | None = None, dtype: torch.dtype = torch.float32,
                    out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
-    """dS [T, E] (k3moe_route_backward): the balance term where counts and rows (balance_loss's, with its alpha, seq
-    and mask) are given, dloss its scalar gradient (None: 1); plus the weight term where dwts [T, K], the gradient of
-    route_topk's weights, and rs are given."""
+    """dS [T, E] (k3moe_route_backward): the balance term where counts and rows (balance_loss's, with its seq and mask)
+    are given, then with its alpha; dloss is the loss's scalar gradient (None: 1); plus the weight term where dwts
+    [T, K], the gradient of route_topk's weights, and rs are given."""
     if stream is not None:
         with _on(stream, S):
             return route_backward(S, idx, alpha, counts, rows, dloss, dwts, rs, seq, mask, dtype, out)
+    if alpha is None:
+        if counts is not None:
+            raise K3MoeError("route_backward: counts need balance_loss's alpha")
+        alpha = 0.0
     return (_ops or _load_ops()).route_backward(S, idx, alpha, counts, rows, dloss, dwts, rs, seq, mask, dtype, out)
 
 

@@ -19,6 +19,17 @@ def test_tables_of_other_tiles():
         k3moe.act_quant_int8(torch.zeros((64 * n, 32), dtype=torch.bfloat16), tables=t)
 
 
+def test_counts_without_alpha():
+    """A balance term whose weight was left out is refused, not taken as zero."""
+    S, idx = torch.zeros(4, 8), torch.zeros((4, 2), dtype=torch.int32)
+    c, n = torch.zeros((1, 8), dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(k3moe.K3MoeError, match="alpha"):
+        k3moe.route_backward(S, idx, counts=c, rows=n)
+    for alpha in (0.0, 0.5):  # given: the host tensor is what is refused
+        with pytest.raises(k3moe.K3MoeError, match="CUDA tensor"):
+            k3moe.route_backward(S, idx, alpha, c, n)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("words", [0, 1, 3])
 def test_tables_with_a_short_meta(dev, words):
