@@ -381,7 +381,11 @@ def balance_loss(S: torch.Tensor, idx: torch.Tensor, alpha: float, seq: torch.Te
     """The router's load-balance loss over the top-k's picks, and its counts (k3moe_balance_loss).
 
     S f32 [T, E] router logits; idx int32 [T, K] (route_topk's); seq int32 [B + 1] offsets of packed sequences (None:
-    one sequence); mask [T] uint8 or bool, rows with 0 are not counted."""
+    one sequence); mask [T] uint8 or bool, rows with 0 are not counted.  The loss is a number without an autograd graph
+    (route_backward makes its gradient): logits that autograd follows are refused, pass S.detach()."""
+    if S.requires_grad and torch.is_grad_enabled():
+        raise K3MoeError("balance_loss: S requires a gradient, which the loss would not carry: pass S.detach() and take "
+                         "the gradient of the logits from route_backward")
     if stream is not None:
         with _on(stream, S):
             return balance_loss(S, idx, alpha, seq, mask)

@@ -30,6 +30,17 @@ def test_counts_without_alpha():
             k3moe.route_backward(S, idx, alpha, c, n)
 
 
+def test_logits_that_autograd_follows():
+    """The loss carries no graph: added to another one it would drop out of the backward pass without a word."""
+    S, idx = torch.zeros(4, 8, requires_grad=True), torch.zeros((4, 2), dtype=torch.int32)
+    with pytest.raises(k3moe.K3MoeError, match="detach"):
+        k3moe.balance_loss(S, idx, 1.0)
+    with pytest.raises(k3moe.K3MoeError, match="CUDA tensor"):  # the host tensor is what is refused
+        k3moe.balance_loss(S.detach(), idx, 1.0)
+    with torch.no_grad(), pytest.raises(k3moe.K3MoeError, match="CUDA tensor"):
+        k3moe.balance_loss(S, idx, 1.0)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("words", [0, 1, 3])
 def test_tables_with_a_short_meta(dev, words):
