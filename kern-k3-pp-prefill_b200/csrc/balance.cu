@@ -25,13 +25,16 @@ namespace bal {
 constexpr int JOIN_WARPS = 32;   // of a block of the join, at most
 constexpr int JOIN_BLOCKS = 8 * 148;
 constexpr int ROW_WARPS = 16;    // of a block that walks rows
+constexpr int FLUSH = 256;       // rows a warp sums in f32
 constexpr int PICKS = 16;        // K at most
 // Row slots a warp: as many as fit, four at most.  One block an SM where a row is long, two where it is short.
 __host__ __device__ constexpr int slots(int nv) { return nv <= 5 ? 4 : nv <= 7 ? 3 : 2; }
 __host__ __device__ constexpr int blocks_per_sm(int nv) { return nv <= 2 ? 2 : 1; }
 __host__ __device__ constexpr int slot_floats(int nv) { return 128 * nv + 2 * PICKS; }
 __host__ __device__ constexpr int ring_bytes(int nv) { return ROW_WARPS * slots(nv) * slot_floats(nv) * 4; }
-__host__ __device__ constexpr int rows_smem(int nv) { return ring_bytes(nv) + (ROW_WARPS / 2) * 128 * nv * 4 + 128 * nv * 4; }
+__host__ __device__ constexpr int rows_smem(int nv) {
+  return ring_bytes(nv) + (ROW_WARPS / 2) * 128 * nv * 4 + 128 * nv * 8 + 128 * nv * 4;
+}
 __host__ __device__ constexpr int grad_smem(int nv) { return ring_bytes(nv) + 2 * 128 * nv * 4; }
 constexpr float TINY = 1e-20f;  // the top-k's guard of its own sum
 constexpr int COLS = 32;        // experts a block of the second pass
@@ -178,8 +181,10 @@ __device__ __forceinline__ void warp_sums(float (&v)[N]) {
 // ---------------------------------------------------------------- forward
 // First pass: a block takes `chunk` consecutive rows, a warp every sixteenth of them, each lane summing its experts' p in
 // registers.  At the end of a sequence, or of the block's rows, the warps' sums are added in order and stored as one
-// partial row.  Block i and sequence b meet in slot i + b: along the rows either i or b goes up, so no two pairs share a
-// slot and nothing needs zeroing.
+// partial row; where a sequence goes on for longer, every 16 * FLUSH rows they go into a sum in double, so that no f32 sum
+// has more than FLUSH + 1 rows however many there are (one sum over the 14000 rows a warp takes of 64 million was off by
+// 1e-4; up to 600 thousand rows nothing is flushed).  Block i and sequence b meet in slot i + b: along the rows either i or
+// b goes up, so no two pairs share a slot and nothing needs zeroing.
 struct BalanceScratch {
   float* prob;   // [slots, E]
   int* count;    // [slots, E]
@@ -309,8 +314,9 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
   using namespace bal;
   constexpr int N = 2 * NV;  // pairs of experts a lane
   extern __shared__ __align__(16) float ring_smem[];
-  float* s_acc = ring_smem + ring_bytes(NV) / 4;                              // [ROW_WARPS / 2][128 NV]
-  int* s_hist = reinterpret_cast<int*>(s_acc + ROW_WARPS / 2 * 128 * NV);  // [128 NV]
+  float* s_acc = ring_smem + ring_bytes(NV) / 4;                                 // [ROW_WARPS / 2][128 NV]
+  double* s_long = reinterpret_cast<double*>(s_acc + ROW_WARPS / 2 * 128 * NV);  // [128 NV]
+  int* s_hist = reinterpret_cast<int*>(s_long + 128 * NV);                       // [128 NV]
   __shared__ int s_rows[ROW_WARPS];
   grid_wait_previous();
   grid_launch_dependents();
@@ -332,69 +338,78 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
   while (r < last) {
     const int b = find(r), end = in.seq ? min(last, in.seq[b + 1]) : last;
     if (end <= r) break;  // offsets that go down: nothing more is counted
-    u64 acc[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] = f32x2(0.f, 0.f);
     int n = 0;
     for (int e = threadIdx.x; e < in.E; e += 32 * ROW_WARPS) s_hist[e] = 0;
     __syncthreads();
-    for (; t < end; t += ROW_WARPS, ++at) {
-      ring.fetch(in, at + slots(NV) - 1, ahead(slots(NV) - 1), true, true, nullptr);
-      ring.wait();
-      if (t < r || (in.mask && in.mask[t] == 0)) continue;
-      ++n;
-      const float* row = ring.slot(at);
-      u64 z2 = f32x2(0.f, 0.f), s[N];
+    for (int from = r, stop; from < end; from = stop) {
+      stop = min(end, from + ROW_WARPS * FLUSH);
+      u64 acc[N];
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(row + (j * 32 + lane) * 4);
-        s[2 * j] = score2(exp_neg2(v.x));
-        s[2 * j + 1] = score2(exp_neg2(v.y));
-        z2 = add_f32x2(z2, add_f32x2(s[2 * j], s[2 * j + 1]));
+      for (int i = 0; i < N; ++i) acc[i] = f32x2(0.f, 0.f);
+      for (; t < stop; t += ROW_WARPS, ++at) {
+        ring.fetch(in, at + slots(NV) - 1, ahead(slots(NV) - 1), true, true, nullptr);
+        ring.wait();
+        if (t < r || (in.mask && in.mask[t] == 0)) continue;
+        ++n;
+        const float* row = ring.slot(at);
+        u64 z2 = f32x2(0.f, 0.f), s[N];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(row + (j * 32 + lane) * 4);
+          s[2 * j] = score2(exp_neg2(v.x));
+          s[2 * j + 1] = score2(exp_neg2(v.y));
+          z2 = add_f32x2(z2, add_f32x2(s[2 * j], s[2 * j + 1]));
+        }
+        const float2 z = f32x2_get(z2);
+        if (lane < in.K) {
+          const int e = reinterpret_cast<const int*>(row + 128 * NV)[lane];
+          if (e >= 0 && e < in.E) atomicAdd(&s_hist[e], 1);
+        }
+        const float inv = rcp_ftz(warp_sum(z.x + z.y) + TINY);
+        const u64 inv2 = f32x2(inv, inv);
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = fma_f32x2(s[i], inv2, acc[i]);
+        __syncwarp();  // every lane has read the slot that the next fetch fills
       }
-      const float2 z = f32x2_get(z2);
-      if (lane < in.K) {
-        const int e = reinterpret_cast<const int*>(row + 128 * NV)[lane];
-        if (e >= 0 && e < in.E) atomicAdd(&s_hist[e], 1);
+      // the upper half of the warps, then the lower half onto them
+      float* mine = s_acc + warp % (ROW_WARPS / 2) * 128 * NV;
+      if (warp >= ROW_WARPS / 2) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          *reinterpret_cast<ulonglong2*>(mine + (j * 32 + lane) * 4) = make_ulonglong2(acc[2 * j], acc[2 * j + 1]);
       }
-      const float inv = rcp_ftz(warp_sum(z.x + z.y) + TINY);
-      const u64 inv2 = f32x2(inv, inv);
+      if (lane == 0) s_rows[warp] = n;
+      __syncthreads();
+      if (warp < ROW_WARPS / 2) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] = fma_f32x2(s[i], inv2, acc[i]);
-      __syncwarp();  // every lane has read the slot that the next fetch fills
-    }
-    // the upper half of the warps, then the lower half onto them
-    float* mine = s_acc + warp % (ROW_WARPS / 2) * 128 * NV;
-    if (warp >= ROW_WARPS / 2) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-        *reinterpret_cast<ulonglong2*>(mine + (j * 32 + lane) * 4) = make_ulonglong2(acc[2 * j], acc[2 * j + 1]);
-    }
-    if (lane == 0) s_rows[warp] = n;
-    __syncthreads();
-    if (warp < ROW_WARPS / 2) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        ulonglong2* q = reinterpret_cast<ulonglong2*>(mine + (j * 32 + lane) * 4);
-        const ulonglong2 o = *q;
-        *q = make_ulonglong2(add_f32x2(o.x, acc[2 * j]), add_f32x2(o.y, acc[2 * j + 1]));
+        for (int j = 0; j < NV; ++j) {
+          ulonglong2* q = reinterpret_cast<ulonglong2*>(mine + (j * 32 + lane) * 4);
+          const ulonglong2 o = *q;
+          *q = make_ulonglong2(add_f32x2(o.x, acc[2 * j]), add_f32x2(o.y, acc[2 * j + 1]));
+        }
       }
-    }
-    __syncthreads();
-    const long long slot = (long long)blockIdx.x + b;
-    for (int e = threadIdx.x; e < in.E; e += 32 * ROW_WARPS) {
-      float p = 0.f;
+      __syncthreads();
+      const long long slot = (long long)blockIdx.x + b;
+      for (int e = threadIdx.x; e < in.E; e += 32 * ROW_WARPS) {
+        float p = 0.f;
 #pragma unroll
-      for (int k = 0; k < ROW_WARPS / 2; ++k) p += s_acc[k * 128 * NV + e];
-      w.prob[slot * in.E + e] = p;
-      w.count[slot * in.E + e] = s_hist[e];
+        for (int k = 0; k < ROW_WARPS / 2; ++k) p += s_acc[k * 128 * NV + e];
+        if (from > r || stop < end) {
+          const double sum = (from > r ? s_long[e] : 0.0) + p;
+          s_long[e] = sum;
+          p = (float)sum;
+        }
+        if (stop < end) continue;
+        w.prob[slot * in.E + e] = p;
+        w.count[slot * in.E + e] = s_hist[e];
+      }
+      if (stop == end && threadIdx.x == 0) {
+        int total = 0;
+        for (int k = 0; k < ROW_WARPS; ++k) total += s_rows[k];
+        w.rows[slot] = total;
+      }
+      __syncthreads();
     }
-    if (threadIdx.x == 0) {
-      int total = 0;
-      for (int k = 0; k < ROW_WARPS; ++k) total += s_rows[k];
-      w.rows[slot] = total;
-    }
-    __syncthreads();
     r = end;
   }
   cp_async_wait_all();
