@@ -14,8 +14,8 @@
 // join; 29 MB more cost 5 us; reading them takes 4.5), gradient of both terms 18-20 us (4 us a round of 16 rows an SM behind
 // 6 us of prologue and first rows; a copy of the same 59 MB takes 10.3 us).
 // Both passes read S once.  Sums run in f32 in a fixed order (no floating-point atomics), so equal inputs give equal
-// bytes.  A score is 1 / (1 + 2^(-S log2 e)) by the approximate exponential and reciprocal: its relative error grows
-// with |S|, to 1.5e-6 at S = -10, where the score itself is below 5e-5.
+// bytes.  A score is 1 / (1 + exp(-S)) by one exponential and one reciprocal instruction, the rounding of the exponential's
+// argument put right: within 2^-20 of itself from S = -87 on, 0 further down.
 #pragma once
 #include "common.cuh"
 
@@ -148,19 +148,28 @@ struct RowRing {
 };
 
 // With e = exp(-x) the score is 1 / (1 + e) and its slope e / (1 + e)^2, without cancellation at either end; two at a time,
-// four multifunction instructions a pair, which bound the passes once the loads keep up.
+// four multifunction instructions a pair.  The exponential's argument is put right but for ln 2's low part (with it the
+// gradient of 65536 x 896 logits takes 103 us, without 92.7, with the argument left as rounded 90.4).  Logits are clamped to +-FAR for it (NaN stays): from there on the score is 1 with
+// slope 0, or below the smallest normal f32 and 0, infinities among them.
+constexpr float FAR = 88.f;
+__device__ __forceinline__ float clamp_logit(float x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-FAR));
+  asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(FAR));
+  return x;
+}
 __device__ __forceinline__ u64 exp_neg2(u64 x) {
-  const float2 v = f32x2_get(mul_f32x2(x, f32x2(-LOG2E, -LOG2E)));
-  return f32x2(ex2_ftz(v.x), ex2_ftz(v.y));
+  const float2 v = f32x2_get(x);
+  return exp_f32x2<false>(f32x2(-clamp_logit(v.x), -clamp_logit(v.y)));
 }
 __device__ __forceinline__ u64 score2(u64 e) {
   const float2 v = f32x2_get(add_f32x2(e, f32x2(1.f, 1.f)));
   return f32x2(rcp_ftz(v.x), rcp_ftz(v.y));
 }
-__device__ __forceinline__ u64 slope2(u64 score, u64 e) {
-  const float2 v = f32x2_get(e);
-  constexpr float MOST = 3.402823466e38f;  // score 0 (x = -inf): slope 0, not inf * 0
-  return mul_f32x2(mul_f32x2(f32x2(fminf(v.x, MOST), fminf(v.y, MOST)), score), score);
+__device__ __forceinline__ u64 slope2(u64 score, u64 e) { return mul_f32x2(mul_f32x2(e, score), score); }
+// 1 / x of a sum: the instruction and one step of Newton's iteration
+__device__ __forceinline__ float reciprocal(float x) {
+  const float r = rcp_ftz(x);
+  return __fmaf_rn(r, __fmaf_rn(-x, r, 1.f), r);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -365,7 +374,7 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
           const int e = reinterpret_cast<const int*>(row + 128 * NV)[lane];
           if (e >= 0 && e < in.E) atomicAdd(&s_hist[e], 1);
         }
-        const float inv = rcp_ftz(warp_sum(z.x + z.y) + TINY);
+        const float inv = reciprocal(warp_sum(z.x + z.y) + TINY);
         const u64 inv2 = f32x2(inv, inv);
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] = fma_f32x2(s[i], inv2, acc[i]);
@@ -560,7 +569,7 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
       sums[1] = m.x + m.y;
     }
     warp_sums(sums);
-    const float inv = rcp_ftz(sums[0] + TINY), m = sums[1] * inv;
+    const float inv = reciprocal(sums[0] + TINY), m = sums[1] * inv;
     if (term) {
       const u64 minus = f32x2(-m, -m), inv2 = f32x2(inv, inv);
 #pragma unroll
@@ -572,7 +581,7 @@ __global__ void __launch_bounds__(32 * bal::ROW_WARPS, bal::blocks_per_sm(NV))
     // the pick's element: the sum of both terms, stored over the balance term alone
     float total = 0.f;
     if (weights) {
-      const float den = rcp_ftz(sums[2] + TINY);
+      const float den = reciprocal(sums[2] + TINY);
       const float mine = rs * den * (g - sums[3] * den) * pick_slope;
       const float f = !term || e < 0 ? 0.f : cb == nullptr ? sf[e] : k * (float)cb[e];
       const float base = term ? (f - m) * (pick_slope * inv) : 0.f;

@@ -232,11 +232,14 @@ __device__ __forceinline__ float rcp_ftz(float x) {
 constexpr float LOG2E = 1.4426950408889634f;
 // e^y of two y in [-88, 88] (NaN stays).  With t = y log2 e rounded to f32, e^y = 2^t e^c for c = y - t ln 2, which is below
 // 2^-17; 1 + c takes its place (off by c^2 / 2 < 2^-35).  ln 2 as two f32, so that c itself is good to 2^-40: what is left is
-// the 2 ulp of 2^t and one rounding, where 2^t alone is off by |y| 2^-24 more, 88 ulp at the ends.
+// the 2 ulp of 2^t and one rounding, where 2^t alone is off by |y| 2^-24 more, 88 ulp at the ends.  LOW false: ln 2 as one
+// f32, one instruction a pair less, |y| 2.8e-9 more (2^-24 at 21, 2 ulp at the ends).
+template <bool LOW = true>
 __device__ __forceinline__ u64 exp_f32x2(u64 y) {
   constexpr float LN2 = 0.693147180559945309f, LN2_LOW = (float)(0.693147180559945309 - (double)LN2);
   const u64 t = mul_f32x2(y, f32x2(LOG2E, LOG2E));
-  const u64 c = fma_f32x2(t, f32x2(-LN2_LOW, -LN2_LOW), fma_f32x2(t, f32x2(-LN2, -LN2), y));
+  u64 c = fma_f32x2(t, f32x2(-LN2, -LN2), y);
+  if (LOW) c = fma_f32x2(t, f32x2(-LN2_LOW, -LN2_LOW), c);
   const float2 v = f32x2_get(t);
   const u64 e = f32x2(ex2_ftz(v.x), ex2_ftz(v.y));
   return fma_f32x2(e, c, e);
