@@ -12,6 +12,7 @@ OUT = os.path.join(HERE, "libk3moe.so")
 HEADER = os.path.join(HERE, "..", "include", "k3moe.h")
 TORCH_SRC = os.path.join(HERE, "csrc", "torch_ops.cpp")
 TORCH_OUT = os.path.join(HERE, "k3moe_torch.so")
+TORCH_STAMP = os.path.join(HERE, "k3moe_torch.stamp")  # the torch and Python that k3moe_torch.so was built against
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17", "-shared",
               "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
 
@@ -43,10 +44,24 @@ def build_cubin(nvcc: str) -> str:
     return CUBIN
 
 
+def torch_stamp() -> str:
+    import torch
+
+    return f"torch {torch.__version__}, {sysconfig.get_config_var('SOABI')}\n"
+
+
+def torch_up_to_date() -> bool:
+    """Newer than its sources, and built against this torch and Python (their binary interfaces change)."""
+    if not os.path.exists(TORCH_OUT) or not os.path.exists(TORCH_STAMP):
+        return False
+    with open(TORCH_STAMP) as f:
+        same = f.read() == torch_stamp()
+    return same and all(os.path.getmtime(s) <= os.path.getmtime(TORCH_OUT) for s in (TORCH_SRC, HEADER))
+
+
 def build_torch(force: bool = False) -> str:
     """The compiled torch side of the newer entries (csrc/torch_ops.cpp), linked to libk3moe.so beside it."""
-    if not force and os.path.exists(TORCH_OUT) and all(os.path.getmtime(s) <= os.path.getmtime(TORCH_OUT)
-                                                       for s in (TORCH_SRC, HEADER)):
+    if not force and torch_up_to_date():
         return TORCH_OUT
     import torch
     from torch.utils import cpp_extension
@@ -63,6 +78,8 @@ def build_torch(force: bool = False) -> str:
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError("g++ failed for k3moe_torch.so")
     os.replace(TORCH_OUT + ".tmp", TORCH_OUT)
+    with open(TORCH_STAMP, "w") as f:
+        f.write(torch_stamp())
     return TORCH_OUT
 
 
