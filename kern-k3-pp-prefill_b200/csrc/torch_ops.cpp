@@ -3,8 +3,12 @@
 // only caller.  A decode step makes such calls every few microseconds, and in Python the checks, the allocations and the
 // argument conversion took longer than the kernels (8.9 us for a quantiser call, 18 us for the balance loss): here they
 // take 1 to 3 us.
+#include <ATen/Context.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/empty_strided.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -101,10 +105,25 @@ T* ptr(const MaybeTensor& t) {
   return t ? reinterpret_cast<T*>(t->data_ptr()) : nullptr;
 }
 
-// straight from torch's CUDA allocator: its dispatcher would take another third of a microsecond an output
-Tensor empty(at::IntArrayRef shape, ScalarType type, const c10::Device& dev) {
-  return at::detail::empty_cuda(shape, type, dev, std::nullopt);
-}
+// A call's outputs, straight from torch's CUDA allocator: its dispatcher would take another third of a microsecond each.
+// It is asked where somebody listens: a dispatch mode is on, or new tensors are filled for determinism.
+struct Outputs {
+  c10::Device dev;
+  bool dispatched;
+  explicit Outputs(const c10::Device& d) : dev(d), dispatched(c10::impl::TorchDispatchModeTLS::any_modes_set()) {
+    const auto& c = at::globalContext();
+    dispatched = dispatched || (c.deterministicAlgorithms() && c.deterministicFillUninitializedMemory());
+  }
+  Tensor empty(at::IntArrayRef shape, ScalarType type) const {
+    if (dispatched) return at::empty(shape, at::TensorOptions().dtype(type).device(dev));
+    return at::detail::empty_cuda(shape, type, dev, std::nullopt);
+  }
+  Tensor empty_rows(int64_t rows, int64_t cols, int64_t ld, ScalarType type) const {
+    if (ld == cols) return empty({rows, cols}, type);
+    if (dispatched) return at::empty_strided({rows, cols}, {ld, 1}, at::TensorOptions().dtype(type).device(dev));
+    return Tensor(at::detail::empty_strided_cuda({rows, cols}, {ld, 1}, type, dev));
+  }
+};
 
 k3moe_stream_t stream_of(const c10::Device& dev) {
   return reinterpret_cast<k3moe_stream_t>(c10::cuda::getCurrentCUDAStream(dev.index()).stream());
@@ -146,9 +165,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> balance_loss(const Tensor& S, const T
   const c10::cuda::CUDAGuard guard(r.dev);
   const size_t bytes = k3moe_balance_scratch_bytes(r.T, r.E, r.B);
   if (bytes == 0) check(K3MOE_EINVAL, "balance_loss");
-  const Tensor scratch = empty({(int64_t)bytes}, ScalarType::Byte, r.dev);
-  const Tensor loss = empty({1}, ScalarType::Float, r.dev), rows = empty({r.B}, ScalarType::Int, r.dev);
-  const Tensor counts = empty({r.B, r.E}, ScalarType::Int, r.dev), prob = empty({r.B, r.E}, ScalarType::Float, r.dev);
+  const Outputs make(r.dev);
+  const Tensor scratch = make.empty({(int64_t)bytes}, ScalarType::Byte);
+  const Tensor loss = make.empty({1}, ScalarType::Float), rows = make.empty({r.B}, ScalarType::Int);
+  const Tensor counts = make.empty({r.B, r.E}, ScalarType::Int), prob = make.empty({r.B, r.E}, ScalarType::Float);
   check(k3moe_balance_loss(ptr<float>(S), r.lds, ptr<int32_t>(idx), r.T, r.E, r.K, ptr<int32_t>(seq), r.B,
                            ptr<uint8_t>(mask), (float)alpha, ptr(scratch), ptr<int32_t>(counts), ptr<float>(prob),
                            ptr<int32_t>(rows), ptr<float>(loss), stream_of(r.dev)),
@@ -175,7 +195,7 @@ Tensor route_backward(const Tensor& S, const Tensor& idx, double alpha, const Ma
   const int code = dtype_code(out ? out->scalar_type() : dtype);
   const int ldd = out ? as_int(rows_of(*out, "out", kFloats, &r.dev, r.E, r.T), "out's row stride") : r.E;
   const c10::cuda::CUDAGuard guard(r.dev);
-  const Tensor dS = out ? *out : empty({r.T, r.E}, dtype, r.dev);
+  const Tensor dS = out ? *out : Outputs(r.dev).empty({r.T, r.E}, dtype);
   check(k3moe_route_backward(ptr<float>(S), r.lds, ptr<int32_t>(idx), r.T, r.E, r.K, ptr<int32_t>(seq), r.B,
                              ptr<uint8_t>(mask), (float)alpha, ptr<int32_t>(counts), ptr<int32_t>(rows), ptr<float>(dloss),
                              ptr<float>(dwts), ptr(rs), ptr(dS), ldd, code, stream_of(r.dev)),
@@ -196,9 +216,8 @@ Int8Out int8_out(const Quantised& out, int64_t rows, int64_t cols, const c10::De
     return {q, scale, ld};
   }
   const int64_t ld = (cols + 15) / 16 * 16;
-  return {ld == cols ? empty({rows, cols}, ScalarType::Char, dev)
-                     : Tensor(at::detail::empty_strided_cuda({rows, cols}, {ld, 1}, ScalarType::Char, dev)),
-          empty({rows}, ScalarType::Float, dev), ld};
+  const Outputs make(dev);
+  return {make.empty_rows(rows, cols, ld, ScalarType::Char), make.empty({rows}, ScalarType::Float), ld};
 }
 
 std::tuple<Tensor, Tensor> quant_int8(const Tensor& x, const Quantised& out) {
@@ -271,7 +290,7 @@ struct ProductOut {
 ProductOut product_out(const Product& p, int64_t N, ScalarType dtype, const MaybeTensor& out) {
   if (out) return {*out, rows_of(*out, "out", kFloats, &p.dev, N, p.T), dtype_code(out->scalar_type())};
   const int code = dtype_code(dtype);
-  return {empty({p.T, N}, dtype, p.dev), N, code};
+  return {Outputs(p.dev).empty({p.T, N}, dtype), N, code};
 }
 
 Tensor gemm_int8(const Tensor& q, const Tensor& sx, const Tensor& w, const Tensor& sw, ScalarType dtype,
