@@ -38,6 +38,7 @@ __host__ __device__ constexpr int rows_smem(int nv) {
 __host__ __device__ constexpr int grad_smem(int nv) { return ring_bytes(nv) + 2 * 128 * nv * 4; }
 constexpr float TINY = 1e-20f;  // the top-k's guard of its own sum
 constexpr int COLS = 32;        // experts a block of the second pass
+constexpr int WIDE = 16;        // partial rows that a lone warp adds up, at most
 }  // namespace bal
 
 struct RouterRows {
@@ -202,9 +203,11 @@ struct BalanceScratch {
   u32* done;
 };
 
-// Second pass: a team (a warp, where few of the first pass's blocks meet a sequence, or a block) adds up 32 experts of one
-// sequence over the blocks that met it, its warps side by side and joined in order, then the next such group of its
-// share; the last block of all adds up the loss.
+// Second pass: a team (a warp, where few of the first pass's blocks meet the average sequence, or a block) adds up 32
+// experts of one sequence over the blocks that met it, its warps side by side and joined in order, then the next such group
+// of its share; the last block of all adds up the loss.  A warp that meets a long sequence among short or empty ones (a
+// batch padded to a fixed number of offsets) leaves it to its whole block; the groups of a sequence go to blocks in turn, so
+// that a block has one of them.
 struct BalanceOut {
   float alpha;
   int* counts;   // [B, E]
@@ -218,27 +221,31 @@ __global__ void __launch_bounds__(32 * bal::JOIN_WARPS)
   using namespace bal;
   __shared__ float s_p[JOIN_WARPS][COLS];
   __shared__ int s_c[JOIN_WARPS][COLS], s_n[JOIN_WARPS];
+  __shared__ int s_wide[WARP_TEAM ? JOIN_WARPS : 1][4];  // i0, i1 (-1: not wide), sequence and group of a warp's unit
   __shared__ int s_last;
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int groups = (in.E + COLS - 1) / COLS;
   const int lo = in.seq ? max(in.seq[0], 0) : 0, hi = in.seq ? min(in.seq[in.B], in.T) : in.T;
-  const long long first = WARP_TEAM ? (long long)blockIdx.x * warps + warp : blockIdx.x;
-  const long long step = WARP_TEAM ? (long long)gridDim.x * warps : gridDim.x;
+  const long long units = (long long)in.B * groups, turn = (long long)gridDim.x * (WARP_TEAM ? warps : 1);
   float terms = 0.f;
   int full = 0;  // sequences with a counted row
   bool waited = false;
-  for (long long unit = first; unit < (long long)in.B * groups; unit += step) {
-    const int b = (int)(unit / groups), g = (int)(unit % groups), e = g * COLS + lane;
+  for (long long base = 0; base + blockIdx.x < units; base += turn) {
+    const long long unit = base + blockIdx.x + (WARP_TEAM ? (long long)gridDim.x * warp : 0);
+    const bool mine = !WARP_TEAM || unit < units;
+    const int b = mine ? (int)(unit / groups) : 0, g = (int)(unit % groups), e = g * COLS + lane;
     const int s0 = in.seq ? max(lo, in.seq[b]) : lo, s1 = in.seq ? min(hi, in.seq[b + 1]) : hi;
-    // the first pass's partial rows (it lets this one start after its own wait: the offsets are there before)
+    // the first pass's blocks that met the sequence
+    const int i0 = s0 / chunk, i1 = mine && s0 < s1 ? (s1 - 1) / chunk : -1;
+    const bool wide = !WARP_TEAM || i1 - i0 >= WIDE;
+    // its partial rows (the first pass lets this one start after its own wait: the offsets are there before)
     if (!waited) grid_wait_previous();
     waited = true;
     float p = 0.f;
     int c = 0, n = 0;
-    if (s0 < s1) {
-      const int i1 = (s1 - 1) / chunk;
+    if (!WARP_TEAM || !wide) {
 #pragma unroll 5
-      for (int i = s0 / chunk + (WARP_TEAM ? 0 : warp); i <= i1; i += WARP_TEAM ? 1 : warps) {
+      for (int i = i0 + (WARP_TEAM ? 0 : warp); i <= i1; i += WARP_TEAM ? 1 : warps) {
         const long long slot = (long long)i + b;
         if (e < in.E) {
           p += w.prob[slot * in.E + e];
@@ -258,8 +265,41 @@ __global__ void __launch_bounds__(32 * bal::JOIN_WARPS)
         c += s_c[k][lane];
         n += s_n[k];
       }
+    } else if (__syncthreads_or(wide)) {
+      if (lane == 0) {
+        s_wide[warp][0] = wide ? i0 : 0;
+        s_wide[warp][1] = wide ? i1 : -1;
+        s_wide[warp][2] = b;
+        s_wide[warp][3] = g;
+      }
+      __syncthreads();
+      for (int k = 0; k < warps; ++k) {
+        const int j1 = s_wide[k][1], bk = s_wide[k][2], ek = s_wide[k][3] * COLS + lane;
+        if (j1 < 0) continue;
+        float pk = 0.f;
+        int ck = 0, nk = 0;
+#pragma unroll 5
+        for (int i = s_wide[k][0] + warp; i <= j1; i += warps) {
+          const long long slot = (long long)i + bk;
+          if (ek < in.E) {
+            pk += w.prob[slot * in.E + ek];
+            ck += w.count[slot * in.E + ek];
+          }
+          nk += w.rows[slot];
+        }
+        s_p[warp][lane] = pk;
+        s_c[warp][lane] = ck;
+        if (lane == 0) s_n[warp] = nk;
+        __syncthreads();
+        for (int j = 0; warp == k && j < warps; ++j) {
+          p += s_p[j][lane];
+          c += s_c[j][lane];
+          n += s_n[j];
+        }
+        __syncthreads();
+      }
     }
-    if (WARP_TEAM || warp == 0) {
+    if (WARP_TEAM ? mine : warp == 0) {
       float term = 0.f;
       if (e < in.E) {
         out.counts[(long long)b * in.E + e] = c;

@@ -634,12 +634,14 @@ int k3moe_balance_loss(const float* S, int lds, const int32_t* idx, int T, int E
       rc = launch_overlapped(balance_rows_kernel<NV>, L.blocks, 32 * bal::ROW_WARPS, bytes, s, 1, in, w, L.chunk);
   });
   if (rc) return rc;
-  // The average sequence's partial rows: up to four, a warp adds them up by itself; else a block's warps share them.
-  // Both calls' time, block against warp, at 8192 x 896: 17.5 against 50.5 us for one sequence, 16.9 against 18.5 for 16,
-  // equal within 0.3 us about 37 (the limit), 20.4 against 17.7 for 74, 130 against 57 for 2048.
+  // The average sequence's partial rows: up to five, a warp adds them up by itself; else a block's warps share them.
+  // Both calls' time, block against warp, at 8192 x 896: 16.9 against 18.5 us for 16 even sequences, equal within 0.3 us
+  // about 37 (the limit there), 19.7 against 18.0 for 48, 20.4 against 17.7 for 74, 130 against 57 for 2048.  A warp that
+  // meets a sequence of many more leaves it to its block: one sequence among 63 empty ones takes 18.8 us (51.4 by a warp
+  // alone), among 255 of 2048 x 256 logits 12.0 (72.8).
   const long long units = (long long)B * cdiv(E, bal::COLS);
   const int partial = (int)cdiv(L.blocks, B) + 1;
-  if (partial <= 4)
+  if (partial <= 5)
     return launch_overlapped(balance_join_kernel<true>, (unsigned)std::min<long long>(bal::JOIN_BLOCKS, cdiv(units, 8)),
                              256, 0, s, 1, in, w, L.chunk, out);
   return launch_overlapped(balance_join_kernel<false>, (unsigned)std::min<long long>(bal::JOIN_BLOCKS, units),
