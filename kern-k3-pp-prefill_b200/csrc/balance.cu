@@ -10,9 +10,10 @@
 //   dS_{t, idx_k} += rs / den (g_k - sum_j g_j s_j / den) s_k (1 - s_k),    g = dloss/dw.
 // No counterpart in the reference: it serves only.
 //
-// Measured on a B200, 8192 x 896 logits, top-8, 16 sequences: loss and counts 17.9 us (11 us at 2048 rows, 5 of them the
-// join; 29 MB more cost 5 us; reading them takes 4.5), gradient of both terms 18-20 us (4 us a round of 16 rows an SM behind
-// 6 us of prologue and first rows; a copy of the same 59 MB takes 10.3 us).
+// Measured on a B200, 8192 x 896 logits, top-8, 16 sequences: loss and counts 17.2 us (11.8 us at 2048 rows, 5 of them the
+// join; 22 MB more cost 5 us; reading them takes 3.4), gradient of both terms 16.9 us into one buffer, 19-21 us into a new
+// one a call (4 us a round of 16 rows an SM behind 6 us of prologue and first rows; a copy of the same 59 MB takes 10.3 us),
+// of the weight term alone 10.0 us.
 // Both passes read S once.  Sums run in f32 in a fixed order (no floating-point atomics), so equal inputs give equal
 // bytes.  A score is 1 / (1 + exp(-S)) by one exponential and one reciprocal instruction, the rounding of the exponential's
 // argument put right: within 2^-20 of itself from S = -87 on, 0 further down.

@@ -796,8 +796,8 @@ int k3moe_grouped_gemm_int8(const int8_t* q_perm, long long ldq, const float* sx
   // A pair of blocks on 256 channels of a tile, unless more than a sixth of the pairs' blocks would have channels past N
   // only.  Single blocks against pairs, 32 experts, C = 2048, top-8, in us: of 4096 tokens 52 / 56 at N = 384 (a quarter of
   // the blocks idle), 80 / 79 at 640 (a sixth), 101 / 97 at 896, 130 / 118 at 1152, 67 / 58 at 512 (none); of 1024 tokens
-  // 25.6 / 29.7, 31.7 / 34.8, 37.9 / 40.0, 46.1 / 46.1, 31.7 / 29.7; of 64 (how many rows
-  // the tables hold, the device alone knows) single blocks are up to 4 us ahead: 17.5 / 19.5 at 512, 33.8 / 37.9 at 1664.
+  // 25.6 / 29.7, 31.7 / 34.8, 37.9 / 40.0, 46.1 / 46.1, 31.7 / 29.7; of 64 (how many rows the tables hold, the device alone
+  // knows) single blocks are up to 4 us ahead: 17.5 / 19.5 at 512, 33.8 / 37.9 at 1664.
   const bool pair = 10 * 2 * cdiv(N, 2 * i8::BM) <= 12 * cdiv(N, i8::BM);
   p.bn = 128;
   p.xbox = pair ? 64 : 32;
