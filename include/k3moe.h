@@ -315,9 +315,10 @@ int k3moe_synth_mxfp4(uint64_t seed, long long row0, long long rows, int K, floa
  *   loss = alpha / B' * sum_b sum_e (E counts / (K n_b)) (prob / n_b), B' = sequences with n_b > 0 (0 if none).
  * S f32 [T, lds]; idx int32 [T, K], ids outside [0, E) not counted; seq int32 [B + 1], non-decreasing offsets in
  * [0, T] (rows before the first and from the last on are not counted), or null with B = 1: all T rows are one
- * sequence; mask uint8 [T] or null.  What S holds in rows that are not counted has no effect.  counts int32 [B, E], prob f32
+ * sequence; mask uint8 [T] or null.  What S holds in rows that are not counted has no effect; a score below 2^-126 (S < -87)
+ * is 0, here and in the gradient.  counts int32 [B, E], prob f32
  * [B, E], rows int32 [B], loss f32 [1].  T <= 2^30, E <= 1024, K <= 16.  Fixed summation order: equal inputs give equal bytes;
- * the rounding of prob's sums is below 2^-14 of them at any T (at most 257 rows, then at most 300 partial sums, in f32).
+ * the rounding of prob's sums is below 2^-14 of them at any T (256 rows at most in f32, then 300 partial sums at most).
  * scratch: k3moe_balance_scratch_bytes(T, E, B) bytes, 16-byte aligned, one per call in flight (0: bad sizes).
  * No counterpart in the reference, which serves only. */
 size_t k3moe_balance_scratch_bytes(int T, int E, int B);

@@ -14,7 +14,7 @@
 // join; 22 MB more cost 5 us; reading them takes 3.4), gradient of both terms 16.9 us into one buffer, 19-21 us into a new
 // one a call (4 us a round of 16 rows an SM behind 6 us of prologue and first rows; a copy of the same 59 MB takes 10.3 us),
 // of the weight term alone 10.0 us.
-// Both passes read S once.  Sums run in f32 in a fixed order (no floating-point atomics), so equal inputs give equal
+// Both passes read S once.  Sums run in a fixed order (no floating-point atomics), so equal inputs give equal
 // bytes.  A score is 1 / (1 + exp(-S)) by one exponential and one reciprocal instruction, the rounding of the exponential's
 // argument put right: within 2^-20 of itself from S = -87 on, 0 further down.
 #pragma once
@@ -193,7 +193,7 @@ __device__ __forceinline__ void warp_sums(float (&v)[N]) {
 // First pass: a block takes `chunk` consecutive rows, a warp every sixteenth of them, each lane summing its experts' p in
 // registers.  At the end of a sequence, or of the block's rows, the warps' sums are added in order and stored as one
 // partial row; where a sequence goes on for longer, every 16 * FLUSH rows they go into a sum in double, so that no f32 sum
-// has more than FLUSH + 1 rows however many there are (one sum over the 14000 rows a warp takes of 64 million was off by
+// has more than FLUSH rows however many there are (one sum over the 14000 rows a warp takes of 64 million was off by
 // 1e-4; up to 600 thousand rows nothing is flushed).  Block i and sequence b meet in slot i + b: along the rows either i or
 // b goes up, so no two pairs share a slot and nothing needs zeroing.
 struct BalanceScratch {
